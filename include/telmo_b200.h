@@ -35,18 +35,22 @@ extern "C" {
 #define TELMO_PRECISION_BF16 2
 #define TELMO_PRECISION_INT8 3
 #define TELMO_PRECISION_Q8_0 4
+/* 4-bit weights with a scale per group of inputs (telmo_weights_upload_q4); no precision of the
+ * reference's. */
+#define TELMO_PRECISION_Q4 5
 
 /* Epilogue activations, as telmo's Act (src/kernels/mod.rs:366-373). */
 #define TELMO_ACT_NONE 0
 #define TELMO_ACT_RELU 1
 #define TELMO_ACT_SILU 2
 
-/* Output element types of telmo_linear. TELMO_DTYPE_I32_PAIR writes the two exact int32 sums of
+/* Element types (telmo_linear's outputs are f32, bf16 or an i32 pair). TELMO_DTYPE_I32_PAIR writes the two exact int32 sums of
  * the split-int8 product instead of the scaled result: plane 0 (rows 0..m-1, ldc apart) holds
  * the high level's sums and plane 1 (starting m * ldc elements later) the low level's. */
 #define TELMO_DTYPE_F32 0
 #define TELMO_DTYPE_BF16 1
 #define TELMO_DTYPE_I32_PAIR 2
+#define TELMO_DTYPE_F16 3
 
 typedef struct telmo_ctx telmo_ctx;
 typedef struct telmo_weights telmo_weights;
@@ -88,6 +92,24 @@ int telmo_weights_upload(telmo_ctx *ctx, int precision, size_t n, size_t k,
 void telmo_weights_free(telmo_weights *w);
 int telmo_weights_shape(const telmo_weights *w, size_t *n, size_t *k);
 
+/* 4-bit weights: w[o, i] = (code[o, i] - zero[o, i / group]) * scale[o, i / group], with groups of
+ * 32, 64 or 128 inputs (the last one may be short), codes and zero points 0..15, and scales that
+ * are finite f16 values. There is no such precision in the reference; this is the step below
+ * its Q8_0 (src/quant.rs:8-13), for products that read more weight bytes than they compute.
+ *
+ * telmo_encode_q4 rounds a row-major f32 [n, k] matrix to them on the host: codes receives n rows
+ * of ceil(k / 2) bytes (the even input in the low half), scales [n, ceil(k / group)], and zeros,
+ * where not NULL, as many zero points: with zeros, codes span the group's range (0 included) in 15
+ * steps; without, every zero point is 8. TELMO_ERR_ARGUMENT for weights that are not finite or
+ * whose scale passes the f16 range. */
+int telmo_encode_q4(const float *rows, size_t n, size_t k, size_t group, uint8_t *codes,
+                    float *scales, uint8_t *zeros);
+/* Uploads such weights (host memory, laid out as telmo_encode_q4 writes them; zeros NULL: 8
+ * everywhere). telmo_linear and telmo_linear_q4 take the handle; telmo_linear_q and
+ * telmo_linear_noalloc do not (TELMO_ERR_UNSUPPORTED), nor do the models. */
+int telmo_weights_upload_q4(telmo_ctx *ctx, size_t n, size_t k, size_t group, const uint8_t *codes,
+                            const float *scales, const uint8_t *zeros, telmo_weights **out);
+
 /* ---- the matrix product -------------------------------------------------------------------- */
 
 /* Kernels::linear / Kernels::matmul with packed int8 weights (src/kernels/mod.rs:657-701):
@@ -98,6 +120,17 @@ int telmo_weights_shape(const telmo_weights *w, size_t *n, size_t *k);
 int telmo_linear(telmo_ctx *ctx, const float *a, size_t lda, size_t m, const telmo_weights *w,
                  const float *bias, int act, float scale, int accumulate, void *c, int c_dtype,
                  size_t ldc, void *stream);
+
+/* telmo_linear with 4-bit weights (telmo_weights_upload_q4) and activations of a_dtype (F32, BF16 or
+ * F16), c of c_dtype (the same three): the same Epilogue, c[m, n] = (accumulate ? c : 0) + scale *
+ * act(a[m, k] . w^T + bias). Activations are not quantized: bf16 and fp16 are multiplied as they
+ * are and f32 to at least 22 significant bits, codes exactly, sums and scales in f32; c is rounded
+ * once. A row of a that holds an infinity or a NaN gives outputs that are not finite in that row
+ * alone. a and c need no more than their elements' alignment; rows that start on 16-byte
+ * boundaries are read fastest. a and c must not overlap. */
+int telmo_linear_q4(telmo_ctx *ctx, const void *a, int a_dtype, size_t lda, size_t m,
+                    const telmo_weights *w, const float *bias, int act, float scale, int accumulate,
+                    void *c, int c_dtype, size_t ldc, void *stream);
 
 /* The activation quantization telmo_linear applies, exposed for checking: row r of a (k
  * values) becomes scale[r] * (hi + lo / 254): scale = amax / 127 as quantize_row_int8
@@ -144,6 +177,48 @@ int telmo_linear_q(telmo_ctx *ctx, const int8_t *hi, const int8_t *lo, size_t ld
                    const float *row_scale, size_t m, const telmo_weights *w, const float *bias,
                    int act, float scale, int accumulate, void *c, int c_dtype, size_t ldc,
                    void *stream);
+
+/* ---- logits --------------------------------------------------------------------------------- */
+
+/* What a decoder lays over a row's logits before it chooses. All arrays are device memory; a NULL
+ * array leaves its rule out. The value of token v of row r, each step rounded to f32, with n the
+ * number of times v stands among the row's tokens so far:
+ *   x = logit;  if n > 0: x = x > 0 ? x / repetition[r] : x * repetition[r], then
+ *   x = x - frequency[r] * n, then x = x - presence[r];  x = x + the biases listed for v;
+ *   x = -infinity where the row's mask does not allow v. */
+typedef struct telmo_logit_rules {
+    const int32_t *history;     /* [rows, history_ld] tokens so far, up to n_history of a row; one */
+    size_t n_history, history_ld; /* outside the vocabulary (a padding of -1, say) counts for nothing */
+    const int32_t *history_len; /* [rows] how many of them a row has (held to 0..n_history) */
+    const float *repetition;    /* [rows] above 0; NULL: 1. The penalties need history */
+    const float *frequency;     /* [rows]; NULL: 0 */
+    const float *presence;      /* [rows]; NULL: 0 */
+    const int32_t *bias_ids;    /* [rows, bias_ld], n_bias of them used; one outside the vocabulary */
+    const float *bias;          /* is left out. Biases of one token add up, 32 entries of the list */
+    size_t n_bias, bias_ld;     /* at a time, in list order */
+    const uint32_t *allowed;    /* [n_states, allowed_ld] bit masks: bit v % 32 of word v / 32 */
+    size_t n_states, allowed_ld;
+    const int32_t *state;       /* [rows] the row's mask; negative: every token, n_states or more: */
+                                /* none. NULL: row r has mask r */
+} telmo_logit_rules;
+
+/* The values above for logits [rows, ld] of dtype (F32, BF16 or F16), vocab of each row, into out
+ * [rows, out_ld] of the same type; what lies behind a row's vocab is left as it is. out may be
+ * logits itself with the same ld, but must not overlap them otherwise. rules NULL: none. There is no
+ * counterpart in the reference, whose decoders choose from the logits as they are or search with
+ * word bonuses (src/biasing.rs). */
+int telmo_logits_constrain(telmo_ctx *ctx, const void *logits, int dtype, size_t ld, size_t rows,
+                           size_t vocab, const telmo_logit_rules *rules, void *out, size_t out_ld,
+                           void *stream);
+/* The k (1..8) tokens of each row with the largest of these values, in f32, largest first and the
+ * lowest token first where several tie (as telmo_granite_frame_ids), into ids [rows, k], and their
+ * log-probabilities x - log(sum over the vocabulary of e^x) into logprobs [rows, k] (NULL: not
+ * wanted). A token whose value is -infinity is never chosen: where fewer than k are left, the rest
+ * of ids is -1 and of logprobs -infinity. A NaN value is not chosen; a NaN or
+ * +infinity makes its row's log-probabilities NaN. */
+int telmo_logits_choose(telmo_ctx *ctx, const void *logits, int dtype, size_t ld, size_t rows,
+                        size_t vocab, const telmo_logit_rules *rules, size_t k, int32_t *ids,
+                        float *logprobs, void *stream);
 
 /* ---- log-mel front ends ---------------------------------------------------------------------- */
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -20,7 +21,7 @@ import numpy as np
 from . import _lib
 from ._lib import TelmoError, check
 
-__all__ = ["Act", "Context", "Epilogue", "Kernels", "PackedWeights", "Precision", "TelmoError",
+__all__ = ["Act", "Context", "Epilogue", "Kernels", "LogitRules", "PackedWeights", "Precision", "TelmoError",
            "DeviceWeights"]
 
 
@@ -31,6 +32,7 @@ class Precision(enum.IntEnum):
     BF16 = 2
     INT8 = 3
     Q8_0 = 4
+    Q4 = 5  # codes 0..15 with a scale, and if given a zero point, per group of inputs
 
 
 class Act(enum.IntEnum):
@@ -44,6 +46,7 @@ class DType(enum.IntEnum):
     F32 = 0
     BF16 = 1
     I32_PAIR = 2
+    F16 = 3
 
 
 @dataclass
@@ -76,6 +79,54 @@ def _stream(stream) -> Optional[int]:
     if stream is None:
         import torch
         return torch.cuda.current_stream().cuda_stream
+    return getattr(stream, "cuda_stream", stream)
+
+
+def _refuse(message: str):
+    raise TelmoError(_lib.TELMO_ERR_ARGUMENT, message)
+
+
+def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
+    """The address of a [rows, cols] matrix with rows `ld` elements apart that starts at tensor `t`,
+    which must lie on the context's device, be of one of `dtypes` and reach to the last element."""
+    if not t.is_cuda or t.get_device() != ctx.device:
+        _refuse(f"{name}: a tensor on {t.device}, the context is on cuda:{ctx.device}")
+    if t.dtype not in dtypes:
+        _refuse(f"{name}: {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+    if rows > 0 and cols > 0:
+        if ld < cols:
+            _refuse(f"{name}: rows {ld} elements apart hold no {cols} elements")
+        have = t.numel() if t.is_contiguous() else \
+            t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+        if have < (rows - 1) * ld + cols:
+            _refuse(f"{name}: {have} elements, {(rows - 1) * ld + cols} are needed")
+    return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=None)
+def _float_types() -> dict:
+    """torch dtype -> TELMO_DTYPE_* of the entry points that take f32, bf16 and f16."""
+    import torch
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}
+
+
+@functools.lru_cache(maxsize=None)
+def _f32_only() -> tuple:
+    import torch
+    return (torch.float32,)
+
+
+@functools.lru_cache(maxsize=None)
+def _i32_only() -> tuple:
+    import torch
+    return (torch.int32,)
+
+
+def _stream_on(ctx, stream) -> Optional[int]:
+    """The given stream, or torch's current stream on the context's device."""
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(ctx.device).cuda_stream
     return getattr(stream, "cuda_stream", stream)
 
 
@@ -112,8 +163,8 @@ class Context:
 class DeviceWeights:
     """A weight matrix uploaded to one context (tensor-core layout)."""
 
-    def __init__(self, ctx: Context, handle, n: int, k: int):
-        self.ctx, self._h, self.n, self.k = ctx, handle, n, k
+    def __init__(self, ctx: Context, handle, n: int, k: int, precision: Precision = Precision.INT8):
+        self.ctx, self._h, self.n, self.k, self.precision = ctx, handle, n, k, precision
 
     @property
     def handle(self):
@@ -134,10 +185,20 @@ class DeviceWeights:
 class PackedWeights:
     """A weight matrix of ``n`` outputs and ``k`` inputs in the reference's panel layout
     (src/kernels/mod.rs:177-304): 16-output panels of int8 values with one f32 scale per output
-    (Int8) or per block of 32 inputs of each output (Q8_0, src/quant.rs:8-13)."""
+    (Int8) or per block of 32 inputs of each output (Q8_0, src/quant.rs:8-13).
+
+    Q4, which the reference does not have, is row-major: ``values`` holds n rows of ceil(k / 2) bytes
+    (two codes 0..15 each, the even input in the low half), ``scales`` [n, ceil(k / group)] f16
+    values and ``zeros``, where given, as many zero points 0..15 (8 where not), for groups of 32, 64
+    or 128 inputs: ``w = (code - zero) * scale``."""
 
     def __init__(self, n: int, k: int, precision: Precision, values: np.ndarray,
-                 scales: np.ndarray):
+                 scales: np.ndarray, zeros: Optional[np.ndarray] = None, group: int = 32):
+        if precision == Precision.Q4:
+            self._init_q4(n, k, values, scales, zeros, group)
+            return
+        if zeros is not None:
+            _refuse(f"{precision.name}: only Q4 has zero points")
         panels = (n + 15) // 16
         if precision not in (Precision.INT8, Precision.Q8_0):
             raise TelmoError(_lib.TELMO_ERR_UNSUPPORTED,
@@ -151,11 +212,39 @@ class PackedWeights:
         self.values = np.ascontiguousarray(values, dtype=np.int8)
         self.scales = np.ascontiguousarray(scales, dtype=np.float32)
 
+    def _init_q4(self, n, k, values, scales, zeros, group) -> None:
+        if group not in (32, 64, 128):
+            _refuse(f"Q4: groups of 32, 64 or 128 inputs, not {group}")
+        if n < 1 or k < 1:
+            _refuse(f"Q4: bad sizes n={n} k={k}")
+        groups = -(-k // group)
+        if values.size != n * (-(-k // 2)) or scales.size != n * groups:
+            _refuse("Q4: sizes do not match n, k and group")
+        if zeros is not None and (zeros.size != n * groups or zeros.dtype != np.uint8):
+            _refuse("Q4: zero points are uint8, one per scale")
+        if values.dtype != np.uint8:
+            _refuse("Q4: values are uint8, two codes to a byte")
+        self.n, self.k, self.precision, self.group = n, k, Precision.Q4, group
+        self.values = np.ascontiguousarray(values)
+        self.scales = np.ascontiguousarray(scales, dtype=np.float32)
+        self.zeros = None if zeros is None else np.ascontiguousarray(zeros)
+
     @staticmethod
-    def encode(rows: np.ndarray, n: int, k: int,
-               precision: Precision = Precision.INT8) -> "PackedWeights":
-        """quant::encode (src/quant.rs:202-269) of a row-major f32 [n, k] matrix."""
+    def encode(rows: np.ndarray, n: int, k: int, precision: Precision = Precision.INT8,
+               group: int = 32, zeros: bool = False) -> "PackedWeights":
+        """quant::encode (src/quant.rs:202-269) of a row-major f32 [n, k] matrix; for Q4 (groups of
+        ``group`` inputs, with zero points if ``zeros``) telmo_encode_q4."""
         rows = np.ascontiguousarray(rows, dtype=np.float32).reshape(n, k)
+        if precision == Precision.Q4:
+            if group not in (32, 64, 128):
+                _refuse(f"Q4: groups of 32, 64 or 128 inputs, not {group}")
+            groups = -(-k // group)
+            values = np.zeros((n, -(-k // 2)), np.uint8)
+            scales = np.zeros((n, groups), np.float32)
+            z = np.zeros((n, groups), np.uint8) if zeros else None
+            check(_lib.load().telmo_encode_q4(rows.ctypes.data, n, k, group, values.ctypes.data,
+                                              scales.ctypes.data, _ptr(z)))
+            return PackedWeights(n, k, precision, values, scales, z, group)
         panels = (n + 15) // 16
         values = np.zeros(panels * 16 * k, np.int8)
         if precision == Precision.Q8_0:
@@ -169,15 +258,87 @@ class PackedWeights:
 
     def upload(self, ctx: Context) -> DeviceWeights:
         h = ctypes.c_void_p()
+        if self.precision == Precision.Q4:
+            check(_lib.load().telmo_weights_upload_q4(ctx.handle, self.n, self.k, self.group,
+                                                      self.values.ctypes.data,
+                                                      self.scales.ctypes.data, _ptr(self.zeros),
+                                                      ctypes.byref(h)), ctx.handle)
+            return DeviceWeights(ctx, h, self.n, self.k, self.precision)
         check(_lib.load().telmo_weights_upload(ctx.handle, int(self.precision), self.n, self.k,
                                                self.values.ctypes.data, self.scales.ctypes.data,
                                                ctypes.byref(h)), ctx.handle)
-        return DeviceWeights(ctx, h, self.n, self.k)
+        return DeviceWeights(ctx, h, self.n, self.k, self.precision)
+
+
+@dataclass
+class LogitRules:
+    """What a decoder lays over logits before it chooses (telmo_logit_rules): penalties for the
+    row's tokens so far, biases, and the masks of a grammar's states. Tensors on the context's
+    device, ``None`` for a rule left out."""
+    history: Optional[object] = None      # int32 [rows, width]
+    history_len: Optional[object] = None  # int32 [rows]
+    repetition: Optional[object] = None   # f32 [rows], above 0
+    frequency: Optional[object] = None    # f32 [rows]
+    presence: Optional[object] = None     # f32 [rows]
+    bias_ids: Optional[object] = None     # int32 [rows, entries], negative: unused
+    bias: Optional[object] = None         # f32 [rows, entries]
+    allowed: Optional[object] = None      # int32 (or uint32) [states, ceil(vocab / 32)] bit masks
+    state: Optional[object] = None        # int32 [rows], negative: no mask; None: row r has mask r
+
+    def _struct(self, ctx, rows: int, vocab: int) -> "_lib.LogitRules":
+        import torch
+        i32, f32 = (torch.int32,), (torch.float32,)
+
+        def row(t, name, types):
+            return None if t is None else _matrix(ctx, t, name, types, 1, rows, rows)
+
+        def table(t, name, types, least_rows, least_cols):
+            if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < least_rows or t.shape[1] < least_cols:
+                _refuse(f"{name}: a matrix of at least [{least_rows}, {least_cols}] with unit stride "
+                        f"along its rows, not {list(t.shape)}")
+            ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+            return _matrix(ctx, t, name, types, t.shape[0], t.shape[1], ld), ld
+
+        s = _lib.LogitRules()
+        if self.history is not None:
+            if self.history_len is None:
+                _refuse("history: its lengths are missing")
+            s.history, s.history_ld = table(self.history, "history", i32, rows, 0)
+            s.n_history = self.history.shape[1]
+            s.history_len = row(self.history_len, "history_len", i32)
+            s.repetition = row(self.repetition, "repetition", f32)
+            s.frequency = row(self.frequency, "frequency", f32)
+            s.presence = row(self.presence, "presence", f32)
+            if s.n_history == 0:  # an empty tensor has no address; without tokens no penalty applies
+                s.history = s.repetition = s.frequency = s.presence = None
+        elif not (self.history_len is self.repetition is self.frequency is self.presence is None):
+            _refuse("penalties need the tokens so far (history)")
+        if self.bias_ids is not None or self.bias is not None:
+            if self.bias_ids is None or self.bias is None or self.bias_ids.shape != self.bias.shape:
+                _refuse("bias_ids and bias are two matrices of one shape")
+            s.bias_ids, s.bias_ld = table(self.bias_ids, "bias_ids", i32, rows, 0)
+            s.bias, ld = table(self.bias, "bias", f32, rows, 0)
+            if ld != s.bias_ld:
+                _refuse("bias_ids and bias must have the same stride")
+            s.n_bias = self.bias.shape[1]
+        if self.allowed is not None:
+            s.allowed, s.allowed_ld = table(self.allowed, "allowed", (torch.int32, torch.uint32), 1,
+                                            -(-vocab // 32))
+            s.n_states = self.allowed.shape[0]
+            s.state = row(self.state, "state", i32)
+            if self.state is None and s.n_states < rows:
+                _refuse(f"{s.n_states} masks for {rows} rows, and no states")
+        elif self.state is not None:
+            _refuse("state needs the masks (allowed)")
+        return s
 
 
 class Kernels:
     """The matrix product of src/kernels/mod.rs on the GPU: ``linear`` and ``matmul`` over
-    packed int8 weights, with the reference's Epilogue. Tensors are torch CUDA tensors."""
+    packed int8 weights, with the reference's Epilogue. Tensors are torch CUDA tensors.
+
+    With Q4 weights ``a`` and ``c`` may each be f32, bf16 or f16 and must lie on the context's
+    device; ``stream`` defaults to torch's current stream there."""
 
     def __init__(self, ctx: Context):
         self.ctx = ctx
@@ -185,11 +346,16 @@ class Kernels:
     def linear(self, a, m: int, w: DeviceWeights, c, epi: Epilogue = Epilogue.PLAIN,
                stream=None) -> None:
         """``c = epilogue(a * w^T)`` with ``a`` and ``c`` contiguous (src/kernels/mod.rs:691)."""
+        if w.precision == Precision.Q4 and not (a.is_contiguous() and c.is_contiguous()):
+            _refuse("linear takes contiguous tensors (matmul takes strides)")
         self.matmul(a, w.k, m, w, c, w.n, epi, stream)
 
     def matmul(self, a, lda: int, m: int, w: DeviceWeights, c, ldc: int,
                epi: Epilogue = Epilogue.PLAIN, stream=None, out_dtype: DType = None) -> None:
         """``c[m, n] = epilogue(a[m, k] * w^T)`` with strides (src/kernels/mod.rs:657)."""
+        if w.precision == Precision.Q4:
+            self._matmul_q4(a, lda, m, w, c, ldc, epi, stream, out_dtype)
+            return
         import torch
         if out_dtype is None:
             out_dtype = DType.BF16 if c.dtype == torch.bfloat16 else \
@@ -197,6 +363,47 @@ class Kernels:
         check(_lib.load().telmo_linear(self.ctx.handle, _ptr(a), lda, m, w.handle, _ptr(epi.bias),
                                        int(epi.act), float(epi.scale), int(epi.accumulate),
                                        _ptr(c), int(out_dtype), ldc, _stream(stream)),
+              self.ctx.handle)
+
+    def _matmul_q4(self, a, lda, m, w, c, ldc, epi, stream, out_dtype) -> None:
+        types = _float_types()
+        pa = _matrix(self.ctx, a, "a", types, m, w.k, lda)
+        pc = _matrix(self.ctx, c, "c", types, m, w.n, ldc)
+        if out_dtype is not None and out_dtype != types[c.dtype]:
+            _refuse(f"c is {c.dtype}, not {out_dtype!r}")
+        pb = None
+        if epi.bias is not None:
+            pb = _matrix(self.ctx, epi.bias, "bias", _f32_only(), 1, w.n, w.n)
+        check(_lib.load().telmo_linear_q4(self.ctx.handle, pa, types[a.dtype], lda, m, w.handle, pb,
+                                          int(epi.act), float(epi.scale), int(epi.accumulate), pc,
+                                          types[c.dtype], ldc, _stream_on(self.ctx, stream)),
+              self.ctx.handle)
+
+    def constrain_logits(self, logits, ld: int, rows: int, vocab: int, rules: Optional[LogitRules],
+                         out, out_ld: int, stream=None) -> None:
+        """``rules`` laid over ``logits`` [rows, ld] (f32, bf16 or f16, ``vocab`` of each row) into
+        ``out`` [rows, out_ld] of the same type, which may be ``logits`` itself
+        (telmo_logits_constrain)."""
+        types = _float_types()
+        pl = _matrix(self.ctx, logits, "logits", types, rows, vocab, ld)
+        po = _matrix(self.ctx, out, "out", (logits.dtype,), rows, vocab, out_ld)
+        st = None if rules is None else ctypes.byref(rules._struct(self.ctx, rows, vocab))
+        check(_lib.load().telmo_logits_constrain(self.ctx.handle, pl, types[logits.dtype], ld, rows,
+                                                 vocab, st, po, out_ld, _stream_on(self.ctx, stream)),
+              self.ctx.handle)
+
+    def choose_tokens(self, logits, ld: int, rows: int, vocab: int, rules: Optional[LogitRules],
+                      k: int, ids, logprobs=None, stream=None) -> None:
+        """The ``k`` (1..8) best tokens of each row of ``logits`` under ``rules``, best first and the
+        lowest first where several tie, into ``ids`` (int32 [rows, k], -1 where nothing is left),
+        and their log-probabilities into ``logprobs`` (f32 [rows, k]) (telmo_logits_choose)."""
+        types = _float_types()
+        pl = _matrix(self.ctx, logits, "logits", types, rows, vocab, ld)
+        pi = _matrix(self.ctx, ids, "ids", _i32_only(), rows, k, k)
+        pp = None if logprobs is None else _matrix(self.ctx, logprobs, "logprobs", _f32_only(), rows, k, k)
+        st = None if rules is None else ctypes.byref(rules._struct(self.ctx, rows, vocab))
+        check(_lib.load().telmo_logits_choose(self.ctx.handle, pl, types[logits.dtype], ld, rows, vocab,
+                                              st, k, pi, pp, _stream_on(self.ctx, stream)),
               self.ctx.handle)
 
     def quantize_x2(self, a, lda: int, m: int, k: int, hi, lo, ldq: int, scale,

@@ -22,6 +22,7 @@ TELMO_ERR_MODEL = -5
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_I32_PAIR = 2
+DTYPE_F16 = 3
 
 # Weight precisions (include/telmo_b200.h, telmo's Precision).
 PRECISIONS = {"f32": 0, "f16": 1, "bf16": 2, "int8": 3, "q8_0": 4}
@@ -50,6 +51,15 @@ class Boost(ctypes.Structure):
                 ("spotting_margin", ctypes.c_float), ("short_word_margin", ctypes.c_float)]
 
 
+class LogitRules(ctypes.Structure):
+    """telmo_logit_rules (include/telmo_b200.h)."""
+    _fields_ = [("history", _vp), ("n_history", _sz), ("history_ld", _sz),
+                ("history_len", _vp), ("repetition", _vp),
+                ("frequency", _vp), ("presence", _vp), ("bias_ids", _vp), ("bias", _vp),
+                ("n_bias", _sz), ("bias_ld", _sz), ("allowed", _vp), ("n_states", _sz),
+                ("allowed_ld", _sz), ("state", _vp)]
+
+
 # name -> (restype, argtypes); every function include/telmo_b200.h declares.
 SIGNATURES = {
     "telmo_ctx_create": (_int, [_int, _c.POINTER(_vp)]),
@@ -64,6 +74,12 @@ SIGNATURES = {
     "telmo_weights_shape": (_int, [_vp, _c.POINTER(_sz), _c.POINTER(_sz)]),
     "telmo_linear": (_int, [_vp, _vp, _sz, _sz, _vp, _vp, _int, _float, _int, _vp, _int, _sz,
                             _vp]),
+    "telmo_encode_q4": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "telmo_weights_upload_q4": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _c.POINTER(_vp)]),
+    "telmo_linear_q4": (_int, [_vp, _vp, _int, _sz, _sz, _vp, _vp, _int, _float, _int, _vp, _int,
+                               _sz, _vp]),
+    "telmo_logits_constrain": (_int, [_vp, _vp, _int, _sz, _sz, _sz, _vp, _vp, _sz, _vp]),
+    "telmo_logits_choose": (_int, [_vp, _vp, _int, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp]),
     "telmo_quantize_x2": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _vp, _vp]),
     "telmo_conv_module_rows": (_int, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "telmo_linear_noalloc": (_int, [_vp, _vp, _sz, _sz, _vp, _vp, _int, _float, _int, _vp, _int,

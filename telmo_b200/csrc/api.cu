@@ -382,6 +382,7 @@ extern "C" void telmo_weights_free(telmo_weights* wp) {
     if (!w) return;
     cudaSetDevice(w->ctx->device);
     free_weights(&w->dev);
+    free_q4_weights(w);
     delete w;
 }
 
@@ -478,6 +479,8 @@ extern "C" int telmo_linear_q(telmo_ctx* c, const int8_t* hi, const int8_t* lo, 
     auto* w = reinterpret_cast<const Weights*>(wp);
     if (!ctx || !w) return TELMO_ERR_ARGUMENT;
     if (w->ctx != ctx) return ctx->fail(TELMO_ERR_ARGUMENT, "the weights belong to another context");
+    if (w->q4)
+        return ctx->fail(TELMO_ERR_UNSUPPORTED, "telmo_linear_q: 4-bit weights take unsplit activations (telmo_linear_q4)");
     if (m == 0) return TELMO_OK;
     if (int rc = check_out(ctx, c_dtype, ldc, static_cast<size_t>(w->dev.n), out)) return rc;
     if (!hi || !lo || !row_scale || ldq < static_cast<size_t>(w->dev.k) || ldq % 16 || m > (1u << 30))
@@ -500,6 +503,9 @@ extern "C" int telmo_linear(telmo_ctx* c, const float* a, size_t lda, size_t m, 
     auto* w = reinterpret_cast<const Weights*>(wp);
     if (!ctx || !w) return TELMO_ERR_ARGUMENT;
     if (w->ctx != ctx) return ctx->fail(TELMO_ERR_ARGUMENT, "the weights belong to another context");
+    if (w->q4)
+        return linear_q4(ctx, a, TELMO_DTYPE_F32, lda, m, w, bias, act, scale, accumulate, out, c_dtype, ldc,
+                         static_cast<cudaStream_t>(stream));
     if (m == 0) return TELMO_OK;
     const size_t k = static_cast<size_t>(w->dev.k), n = static_cast<size_t>(w->dev.n);
     if (!a || lda < k || m > (1u << 30))

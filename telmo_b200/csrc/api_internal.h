@@ -53,10 +53,34 @@ struct Ctx {
     void* workspace(size_t bytes, cudaStream_t stream);
 };
 
+struct Q4Weights;
+
 struct Weights {
     Ctx* ctx = nullptr;
     DevWeights dev;
+    Q4Weights* q4 = nullptr;  // 4-bit weights (q4.h); then dev holds the shape alone
 };
+
+// Makes a context's device current for the time of a call and the caller's again at its end.
+struct DeviceScope {
+    int before = -1;
+    int enter(Ctx* ctx) {
+        int now = -1;
+        if (int rc = ctx->cuda(cudaGetDevice(&now), "cudaGetDevice")) return rc;
+        if (now == ctx->device) return 0;
+        if (int rc = ctx->use_device()) return rc;
+        before = now;
+        return 0;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// The product with 4-bit weights: telmo_linear_q4 after its handles are known (q4_api.cu).
+int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const Weights* w, const float* bias, int act,
+              float scale, int accumulate, void* out, int c_dtype, size_t ldc, cudaStream_t stream);
+void free_q4_weights(Weights* w);
 
 inline Ctx* as_ctx(telmo_ctx* c) { return reinterpret_cast<Ctx*>(c); }
 

@@ -61,6 +61,8 @@ extern "C" int telmo_linear_noalloc(telmo_ctx* c, const float* a, size_t lda, si
     auto* w = reinterpret_cast<const Weights*>(wp);
     if (!ctx || !w) return TELMO_ERR_ARGUMENT;
     if (w->ctx != ctx) return ctx->fail(TELMO_ERR_ARGUMENT, "the weights belong to another context");
+    if (w->q4)
+        return ctx->fail(TELMO_ERR_UNSUPPORTED, "telmo_linear_noalloc: 8-bit weights only (4-bit: telmo_linear_q4)");
     if (m == 0) return TELMO_OK;
     const size_t k = static_cast<size_t>(w->dev.k), n = static_cast<size_t>(w->dev.n);
     if (!a || lda < k) return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_noalloc: a is NULL or lda %zu < k %zu", lda, k);

@@ -1,0 +1,58 @@
+// q4.h -- 4-bit weights with a scale (and, where given, a zero point) per group of inputs:
+// their device layout and the products that read it (internal to libtelmo_b200).
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace telmo {
+
+// w[o, i] = (code[o, i] - zero[o, i / group]) * scale[o, i / group], codes and zero points 0..15.
+//
+// Codes are stored in tiles of 8 outputs by 128 inputs (a chunk), 512 bytes each, the chunks of
+// 8 outputs one after another. Lane l = 4 g + t of a warp owns bytes 16 l .. 16 l + 15 of a
+// tile: four 32-bit words of output row g, word w holding inputs 32 w + 8 t + 0..7 of the chunk
+// (input 2 p in nibble p, input 2 p + 1 in nibble p + 4). So a tile is one coalesced 16-byte load
+// per lane; (word >> 4 p) & 0x000f000f leaves two neighbouring inputs in the two halves of a
+// register; and one word of the four lanes of a row spans 32 inputs, the smallest group, so a
+// 16-input matrix instruction never mixes two groups. Scales and zero points lie tile by tile
+// too, [8 outputs][128 / group]. Outputs are padded to a multiple of 16 and inputs to one of 128,
+// with code 8, zero point 8 and scale 0.
+struct Q4Weights {
+    int n = 0, k = 0, group = 0;
+    int chunks = 0;             // 128-input chunks per output
+    uint4* codes = nullptr;     // [round_up(n, 16) / 8][chunks][32 lanes]
+    __half* scales = nullptr;   // [round_up(n, 16) / 8][chunks][8][128 / group]
+    uint8_t* zeros = nullptr;   // the same shape, or null: 8 everywhere
+};
+
+enum Q4Type : int { kQ4F32 = 0, kQ4BF16 = 1, kQ4F16 = 2 };
+
+struct Q4Args {
+    const Q4Weights* w = nullptr;
+    const void* a = nullptr;  // [m, lda] of a_type
+    int a_type = kQ4F32;
+    int64_t lda = 0;
+    int m = 0;
+    const float* bias = nullptr;  // [n] or null
+    int act = 0;                  // Act
+    float scale = 1.0f;
+    int accumulate = 0;
+    void* c = nullptr;  // [m, ldc] of c_type
+    int c_type = kQ4F32;
+    int64_t ldc = 0;
+    int sms = 148;
+    uint32_t* error = nullptr;  // device error word
+};
+
+// Codes as the host gives them ([n, ceil(k / 2)] bytes, the even input in the low half), scales
+// and zero points [n, groups], all in device memory, into the layout above.
+cudaError_t q4_repack(const uint8_t* codes, const float* scales, const uint8_t* zeros, const Q4Weights& w,
+                      cudaStream_t stream);
+
+// The product for few rows: every warp multiplies 16 or 32 outputs by up to 32 rows.
+cudaError_t q4_linear_rows(const Q4Args& g, cudaStream_t stream);
+
+}  // namespace telmo

@@ -1,0 +1,262 @@
+"""The product with 4-bit weights against its definition in 64 bits.
+
+Tolerance, per output, before any output rounding: with S = sum_i |a_i w_i|, the kernels add at most
+`adds` terms one after another in f32 (the matrix instructions' steps of 16 inputs within a group,
+three of them for f32 activations, then one per group and a few across warps), each off by at
+most 2^-23 of a partial sum that S bounds (the matrix unit may truncate), and an f32 activation is
+represented to 2^-22. The activation function's slope is at most 1.1, its own f32 steps cost at most
+2^-20 of the value. Then half a step of the output type, relative to the value; for f16 below 2^-14
+half a step is 2^-25.
+"""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def types():
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def weights(ctx, n, k, group, zeros, seed):
+    """A handle and the weights in 64 bits."""
+    from telmo_b200 import PackedWeights, Precision
+    from test_q4 import decode
+    g = np.random.default_rng(seed)
+    groups = -(-k // group)
+    values = g.integers(0, 256, (n, -(-k // 2)), dtype=np.uint8)
+    scales = ((g.random((n, groups)) + 0.5) * g.choice([0.01, 0.1, 1.0], (n, groups))).astype(np.float16)
+    scales = (scales * g.choice([1, 1, 1, -1], (n, groups))).astype(np.float32)
+    z = g.integers(0, 16, (n, groups), dtype=np.uint8) if zeros else None
+    p = PackedWeights(n, k, Precision.Q4, values, scales, zeros=z, group=group)
+    return p.upload(ctx), decode(p)
+
+
+def reference(a, w, bias, act, scale, c0):
+    y = a @ w.T
+    if bias is not None:
+        y = y + bias
+    if act == "RELU":
+        y = np.maximum(y, 0)
+    elif act == "SILU":
+        y = y / (1 + np.exp(-y))
+    y = y * scale
+    return y if c0 is None else y + c0
+
+
+def bound(a, w, y, bias, scale, c0, group, out):
+    k = a.shape[1]
+    adds = 3 * group / 16 + -(-k // 128) * (128 // group) + 16
+    s = np.abs(a) @ np.abs(w).T
+    b = 1.1 * abs(scale) * (s * (adds * 2.0 ** -23 + 2.0 ** -22) + (0 if bias is None else np.abs(bias) * 2.0 ** -24))
+    b = b + np.abs(y) * 2.0 ** -20 + (0 if c0 is None else np.abs(c0) * 2.0 ** -23)
+    half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[out]
+    return b + (np.abs(y) + b) * half + (2.0 ** -25 if out == "f16" else 1e-37)
+
+
+def run(ctx, m, n, k, group=32, zeros=False, dtype="f32", out="f32", act="NONE", scale=1.0, with_bias=False,
+        accumulate=False, lda=None, ldc=None, offset=0, seed=0, stream=None):
+    import torch
+    from telmo_b200 import Act, Epilogue, Kernels
+    t = types()
+    dev, w = weights(ctx, n, k, group, zeros, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    lda, ldc = lda or k, ldc or n
+    store = torch.randn(offset + m * lda + 8, generator=g).to(t[dtype]).cuda()
+    a = store[offset:offset + m * lda].view(m, lda)
+    c = torch.randn((m, ldc), generator=g).to(t[out]).cuda()
+    before = c.clone()
+    bias = torch.randn(n, generator=g).cuda() if with_bias else None
+    Kernels(ctx).matmul(a, lda, m, dev, c, ldc, Epilogue(bias=bias, act=Act[act], scale=scale, accumulate=accumulate),
+                        stream=stream)
+    ctx.check(stream)
+    av = a[:, :k].double().cpu().numpy()
+    bv = None if bias is None else bias.double().cpu().numpy()
+    c0 = before[:, :n].double().cpu().numpy() if accumulate else None
+    y = reference(av, w, bv, act, scale, c0)
+    off = np.abs(c[:, :n].double().cpu().numpy() - y)
+    assert (off <= bound(av, w, y, bv, scale, c0, group, out)).all(), float(off.max())
+    assert torch.equal(c[:, n:], before[:, n:])  # what lies between the rows stays as it was
+    dev.free()
+
+
+ROWS = [1, 2, 3, 8, 9, 17, 31, 32, 33, 64, 65, 130, 257]
+
+
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_types_groups(ctx, m, dtype, group, zeros):
+    n, k = (130, 1000) if m % 2 else (257, 1024)
+    run(ctx, m, n, k, group, zeros, dtype, dtype, with_bias=bool(m % 3), seed=m)
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 128), (7, 31), (15, 32), (16, 33), (17, 127), (31, 129), (33, 255),
+                                 (129, 640), (640, 2049), (2049, 97)])
+@pytest.mark.parametrize("m", [1, 5, 20, 40, 150])
+@pytest.mark.parametrize("dtype,out,group,zeros", [("f32", "f32", 32, True), ("bf16", "f32", 128, False),
+                                                   ("f16", "f16", 64, True), ("f32", "bf16", 64, False)])
+def test_odd_sizes(ctx, n, k, m, dtype, out, group, zeros):
+    run(ctx, m, n, k, group, zeros, dtype, out, seed=n + k)
+
+
+@pytest.mark.parametrize("m", [1, 4, 19, 70])
+@pytest.mark.parametrize("act,scale,with_bias,accumulate", [
+    ("NONE", 0.5, True, True), ("RELU", 1.0, True, False), ("SILU", 2.0, True, True), ("SILU", 1.0, False, False),
+    ("RELU", -1.5, False, True)])
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+def test_epilogues(ctx, m, act, scale, with_bias, accumulate, dtype, out):
+    run(ctx, m, 150, 300, 32, True, dtype, out, act, scale, with_bias, accumulate, seed=m)
+
+
+@pytest.mark.parametrize("m", [1, 3, 12, 24, 50, 200])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lda,ldc,offset", [(1001, 151, 0), (1001, 150, 1), (1000, 152, 3), (1004, 150, 2),
+                                            (1008, 160, 8)])
+def test_strides_and_alignment(ctx, m, dtype, lda, ldc, offset):
+    run(ctx, m, 150, 1000, 64, True, dtype, dtype, lda=lda, ldc=ldc, offset=offset, seed=lda)
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 4096, 4096, 128), (8, 1024, 4096, 32), (32, 2049, 1024, 64),
+                                         (300, 4096, 1024, 32), (1024, 1024, 4096, 128)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_model_sizes(ctx, m, n, k, group, dtype):
+    run(ctx, m, n, k, group, True, dtype, "f32", with_bias=True, seed=n)
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 30, 100, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_row_that_is_not_finite_stays_alone(ctx, m, dtype):
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 70, 200
+    dev, w = weights(ctx, n, k, 32, True, 5)
+    a = torch.randn((m, k), generator=torch.Generator().manual_seed(6)).to(types()[dtype]).cuda()
+    clean, c = (torch.empty((m, n), device="cuda") for _ in range(2))
+    Kernels(ctx).linear(a, m, dev, clean)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        b = a.clone()
+        b[m // 2, 77] = bad
+        Kernels(ctx).linear(b, m, dev, c)
+        ctx.check()
+        assert not torch.isfinite(c[m // 2]).any()
+        keep = torch.arange(m, device="cuda") != m // 2
+        assert torch.equal(c[keep], clean[keep])
+    dev.free()
+
+
+@pytest.mark.parametrize("m", [1, 16, 100])
+def test_f32_activations_of_very_different_size(ctx, m):
+    """Rows from 2^-100 to 2^100 and a row with one large value: each row keeps its own accuracy."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 64, 512
+    dev, w = weights(ctx, n, k, 128, False, 9)
+    a = torch.randn((m, k), generator=torch.Generator().manual_seed(1))
+    a *= torch.exp2(torch.linspace(-100, 100, m))[:, None] if m > 1 else 2.0 ** -100
+    a[m // 2, 3] *= 1e5
+    c = torch.empty((m, n), device="cuda")
+    Kernels(ctx).linear(a.cuda(), m, dev, c)
+    ctx.check()
+    av = a.double().numpy()
+    y = av @ w.T
+    off = np.abs(c.double().cpu().numpy() - y)
+    assert (off <= bound(av, w, y, None, 1.0, None, 128, "f32")).all()
+    dev.free()
+
+
+def test_no_rows_and_refusals(ctx):
+    import torch
+    from telmo_b200 import Epilogue, Kernels, TelmoError, _lib
+    kern = Kernels(ctx)
+    dev, _ = weights(ctx, 40, 64, 32, False, 1)
+    a = torch.randn((4, 64), device="cuda")
+    c = torch.full((4, 40), 3.0, device="cuda")
+    kern.linear(a, 0, dev, c)
+    ctx.check()
+    assert (c == 3).all()
+    bad = [
+        lambda: kern.linear(a.double(), 4, dev, c),
+        lambda: kern.linear(a, 4, dev, c.double()),
+        lambda: kern.linear(a.cpu(), 4, dev, c),
+        lambda: kern.linear(a, 5, dev, c),
+        lambda: kern.linear(a[:, :63], 4, dev, c),
+        lambda: kern.matmul(a, 63, 4, dev, c, 40),
+        lambda: kern.matmul(a, 64, 4, dev, c, 39),
+        lambda: kern.linear(a, 4, dev, c[:, :39]),
+        lambda: kern.linear(a, 4, dev, c, Epilogue(bias=torch.zeros(39, device="cuda"))),
+        lambda: kern.linear(a, 4, dev, c, Epilogue(bias=torch.zeros(40, device="cuda").bfloat16())),
+        lambda: kern.linear_q(c, c, 64, c, 4, dev, c, 40),
+    ]
+    for call in bad:
+        with pytest.raises(TelmoError):
+            call()
+    L, h, s = _lib.load(), ctx.handle, None
+    pa, pc = a.data_ptr(), c.data_ptr()
+    arg = _lib.TELMO_ERR_ARGUMENT
+    assert L.telmo_linear_q4(h, pa, 2, 64, 4, dev.handle, None, 0, 1.0, 0, pc, 0, 40, s) == arg
+    assert L.telmo_linear_q4(h, pa, 0, 64, 4, dev.handle, None, 0, 1.0, 0, pc, 2, 40, s) == arg
+    assert L.telmo_linear_q4(h, pa, 0, 64, 4, dev.handle, None, 3, 1.0, 0, pc, 0, 40, s) == arg
+    assert L.telmo_linear_q4(h, pa + 2, 0, 64, 4, dev.handle, None, 0, 1.0, 0, pc, 0, 40, s) == arg
+    assert L.telmo_linear_q4(h, pa, 1, 64, 4, dev.handle, None, 0, 1.0, 0, pc + 1, 1, 40, s) == arg
+    assert L.telmo_linear_q4(h, None, 0, 64, 4, dev.handle, None, 0, 1.0, 0, pc, 0, 40, s) == arg
+    assert L.telmo_linear_q4(h, pa, 0, 64, 4, dev.handle, None, 0, 1.0, 0, None, 0, 40, s) == arg
+    assert L.telmo_linear_noalloc(h, pa, 64, 4, dev.handle, None, 0, 1.0, 0, pc, 0, 40, s) == _lib.TELMO_ERR_UNSUPPORTED
+    v = np.zeros((4, 32), np.uint8)
+    sc = np.ones((4, 2), np.float32)
+    out = __import__("ctypes").c_void_p()
+
+    def upload(n=4, k=64, group=32, codes=v.ctypes.data, scales=sc.ctypes.data, zeros=None):
+        return L.telmo_weights_upload_q4(h, n, k, group, codes, scales, zeros, __import__("ctypes").byref(out))
+    for more in ({"n": 0}, {"k": 0}, {"group": 16}, {"codes": None}, {"scales": None}):
+        assert upload(**more) == arg and not out.value
+    for wrong in (0.1, np.nan, np.inf, 1e6):
+        s2 = sc.copy()
+        s2[3, 1] = wrong
+        assert upload(scales=s2.ctypes.data) == arg and not out.value
+    z = np.full((4, 2), 16, np.uint8)
+    assert upload(zeros=z.ctypes.data) == arg and not out.value
+    assert (c == 3).all()
+    dev.free()
+
+
+@pytest.mark.parametrize("m", [1, 24, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_streams_and_graphs(ctx, m, dtype):
+    """On another stream; captured into two graphs that are replayed one after the other and at once."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 200, 515
+    side = torch.cuda.Stream()
+    run(ctx, m, n, k, 64, True, dtype, "f32", seed=3, stream=side)
+    kern = Kernels(ctx)
+    dev, w = weights(ctx, n, k, 64, True, 4)
+    inputs = [torch.randn((m, k), device="cuda").to(types()[dtype]) for _ in range(2)]
+    outs = [torch.zeros((m, n), device="cuda") for _ in range(2)]
+    want = [torch.zeros((m, n), device="cuda") for _ in range(2)]
+    for x, y in zip(inputs, want):
+        kern.linear(x, m, dev, y)
+    torch.cuda.synchronize()
+    graphs = []
+    for x, y in zip(inputs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kern.linear(x, m, dev, y)
+        graphs.append(g)
+    for _ in range(3):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for y, e in zip(outs, want):
+            assert torch.equal(y, e)
+    del graphs
+    dev.free()
