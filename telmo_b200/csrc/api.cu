@@ -139,6 +139,7 @@ extern "C" void telmo_ctx_destroy(telmo_ctx* c) {
     delete ctx->parakeet_fe;
     if (ctx->ws) cudaFree(ctx->ws);
     if (ctx->error_word) cudaFree(ctx->error_word);
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
     delete ctx;
 }
 

@@ -55,4 +55,9 @@ cudaError_t q4_repack(const uint8_t* codes, const float* scales, const uint8_t* 
 // The product for few rows: every warp multiplies 16 or 32 outputs by up to 32 rows.
 cudaError_t q4_linear_rows(const Q4Args& g, cudaStream_t stream);
 
+// The product for many rows on tcgen05 tiles, and the bytes of workspace (16-byte aligned) it needs
+// for activations that it cannot read where they are: f32, or rows off 16-byte boundaries.
+size_t q4_gemm_workspace(const Q4Args& g);
+cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream);
+
 }  // namespace telmo

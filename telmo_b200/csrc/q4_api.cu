@@ -99,7 +99,7 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     const size_t n = static_cast<size_t>(w->q4->n), k = static_cast<size_t>(w->q4->k);
     if (at < 0) return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: unknown activation dtype %d", a_dtype);
     if (ct < 0) return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: unknown output dtype %d", c_dtype);
-    if (!a || lda < k || m > (1u << 30) || lda > (size_t(1) << 40))
+    if (!a || lda < k || m > (1u << 29) || lda > (size_t(1) << 40))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: a is NULL, lda %zu < k %zu or too many rows (%zu)", lda,
                          k, m);
     if (!out || ldc < n || ldc > (size_t(1) << 40))
@@ -125,7 +125,25 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     g.ldc = static_cast<int64_t>(ldc);
     g.sms = ctx->sms;
     g.error = ctx->error_word;
-    return ctx->cuda(q4_linear_rows(g, stream), "telmo_linear_q4");
+    if (m <= 32) return ctx->cuda(q4_linear_rows(g, stream), "telmo_linear_q4");
+    const size_t bytes = q4_gemm_workspace(g);
+    if (bytes == 0) return ctx->cuda(q4_linear_gemm(g, nullptr, stream), "telmo_linear_q4");
+    // Workspace in stream order from the context's own pool: calls on several streams and captured
+    // graphs each have their own, and a graph keeps its own while it lives.
+    if (!ctx->pool) {
+        cudaMemPoolProps props = {};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = ctx->device;
+        if (int rc = ctx->cuda(cudaMemPoolCreate(&ctx->pool, &props), "telmo_linear_q4: memory pool")) return rc;
+        uint64_t keep = UINT64_MAX;  // what a call gave back stays for the next
+        cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    }
+    void* ws = nullptr;
+    if (int rc = ctx->cuda(cudaMallocFromPoolAsync(&ws, bytes, ctx->pool, stream), "telmo_linear_q4: workspace")) return rc;
+    const cudaError_t e = q4_linear_gemm(g, ws, stream);
+    const cudaError_t f = cudaFreeAsync(ws, stream);
+    return ctx->cuda(e != cudaSuccess ? e : f, "telmo_linear_q4");
 }
 
 }  // namespace telmo

@@ -1,0 +1,47 @@
+// q4_device.cuh -- what the kernels that read 4-bit weights share on the device.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "q4.h"
+
+namespace telmo {
+
+// Codes 2 p and 2 p + 1 of a word less their zero point, as two exact operands; `base` is
+// code_base of the zero point: a pair of 128 + zero (bf16) or 1024 + zero (fp16).
+template <bool BF16>
+__device__ __forceinline__ uint32_t code_base(uint32_t zero) {
+    return (BF16 ? 0x43004300u : 0x64006400u) | (zero * 0x00010001u);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t base) {
+    const uint32_t v = ((word >> (4 * p)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+    if (BF16) {
+        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&base));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&base));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+__device__ __forceinline__ float q4_act(float v, int act) {
+    if (act == kActRelu) return fmaxf(v, 0.0f);
+    if (act == kActSilu) return mul_sigmoid(v, v);
+    return v;
+}
+
+__device__ __forceinline__ float q4_load(const void* c, int type, int64_t at) {
+    if (type == kQ4F32) return static_cast<const float*>(c)[at];
+    if (type == kQ4BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(c)[at]);
+    return __half2float(static_cast<const __half*>(c)[at]);
+}
+__device__ __forceinline__ void q4_store(void* c, int type, int64_t at, float v) {
+    if (type == kQ4F32) static_cast<float*>(c)[at] = v;
+    else if (type == kQ4BF16) static_cast<__nv_bfloat16*>(c)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(c)[at] = __float2half_rn(v);
+}
+
+}  // namespace telmo

@@ -17,10 +17,8 @@
 // parts of 8 significant bits by truncation, x = hi + mid + lo, which is exact (24 bits; parts
 // below 2^-126 vanish), and three products are summed: in three instructions, or for one and two
 // rows in one, the parts in columns of their own.
-#include "kernels.h"
-#include "q4.h"
+#include "q4_device.cuh"
 
-#include <cuda_bf16.h>
 #include <algorithm>
 
 namespace telmo {
@@ -70,20 +68,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes 2 p and 2 p + 1 of a word less their zero point, as two exact operands; `base` is the pair
-// of 128 + zero (bf16) or 1024 + zero (fp16).
-template <bool BF16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t base) {
-    const uint32_t v = ((word >> (4 * p)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
-    if (BF16) {
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                         *reinterpret_cast<const __nv_bfloat162*>(&base));
-        return *reinterpret_cast<const uint32_t*>(&d);
-    }
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&base));
-    return *reinterpret_cast<const uint32_t*>(&d);
-}
-
 // Eight 16-bit activations of one row from input i on; 0 outside the row and the matrix.
 __device__ __forceinline__ uint4 load_a16(const RowsParams& p, int row, int i) {
     if (row >= p.m) return make_uint4(0, 0, 0, 0);
@@ -131,23 +115,6 @@ __device__ __forceinline__ void split_parts(const float (&x)[8], uint32_t (&hi)[
         mid[j] = bf16_tops(r0, r1);
         lo[j] = bf16_tops(bf16_rest(r0), bf16_rest(r1));
     }
-}
-
-__device__ __forceinline__ float apply_act(float v, int act) {
-    if (act == kActRelu) return fmaxf(v, 0.0f);
-    if (act == kActSilu) return v / (1.0f + expf(-v));
-    return v;
-}
-
-__device__ __forceinline__ float load_c(const void* c, int type, int64_t at) {
-    if (type == kQ4F32) return static_cast<const float*>(c)[at];
-    if (type == kQ4BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(c)[at]);
-    return __half2float(static_cast<const __half*>(c)[at]);
-}
-__device__ __forceinline__ void store_c(void* c, int type, int64_t at, float v) {
-    if (type == kQ4F32) static_cast<float*>(c)[at] = v;
-    else if (type == kQ4BF16) static_cast<__nv_bfloat16*>(c)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(c)[at] = __float2half_rn(v);
 }
 
 // One tile's scales and zero points of this lane's row: GROUPS of each.
@@ -225,9 +192,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) q4_rows_kernel(const RowsParam
                                                                                               : words[2 * r].w;
                     const uint32_t x1 = w == 0 ? words[2 * r + 1].x : w == 1 ? words[2 * r + 1].y
                                                 : w == 2 ? words[2 * r + 1].z : words[2 * r + 1].w;
-                    const uint32_t one = BF16 ? 0x43004300u : 0x64006400u;
-                    const uint32_t z0 = one | (sc[2 * r].z[q] * 0x00010001u);
-                    const uint32_t z1 = one | (sc[2 * r + 1].z[q] * 0x00010001u);
+                    const uint32_t z0 = code_base<BF16>(sc[2 * r].z[q]), z1 = code_base<BF16>(sc[2 * r + 1].z[q]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t a[4] = {code_pair<BF16>(x0, 2 * h, z0), code_pair<BF16>(x1, 2 * h, z1),
@@ -281,10 +246,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps) q4_rows_kernel(const RowsParam
         float v = 0.0f;
         for (int w = 0; w < warps; ++w) v += sums[w][o][col];
         if (p.bias) v += __ldg(p.bias + out);
-        v = apply_act(v, p.act) * p.scale;
+        v = q4_act(v, p.act) * p.scale;
         const int64_t at = static_cast<int64_t>(row) * p.ldc + out;
-        if (p.accumulate) v += load_c(p.c, p.c_type, at);
-        store_c(p.c, p.c_type, at, v);
+        if (p.accumulate) v += q4_load(p.c, p.c_type, at);
+        q4_store(p.c, p.c_type, at, v);
     }
 }
 
