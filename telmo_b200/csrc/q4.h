@@ -11,22 +11,27 @@ namespace telmo {
 
 // w[o, i] = (code[o, i] - zero[o, i / group]) * scale[o, i / group], codes and zero points 0..15.
 //
-// Codes are stored in tiles of 8 outputs by 128 inputs (a chunk), 512 bytes each, the chunks of
-// 8 outputs one after another. Lane l = 4 g + t of a warp owns bytes 16 l .. 16 l + 15 of a
-// tile: four 32-bit words of output row g, word w holding inputs 32 w + 8 t + 0..7 of the chunk
-// (input 2 p in nibble p, input 2 p + 1 in nibble p + 4). So a tile is one coalesced 16-byte load
-// per lane; (word >> 4 p) & 0x000f000f leaves two neighbouring inputs in the two halves of a
-// register; and one word of the four lanes of a row spans 32 inputs, the smallest group, so a
-// 16-input matrix instruction never mixes two groups. Scales and zero points lie tile by tile
-// too, [8 outputs][128 / group]. Outputs are padded to a multiple of 16 and inputs to one of 128,
-// with code 8, zero point 8 and scale 0.
+// Codes are stored in tiles of 8 outputs by 128 inputs (a chunk), 512 bytes each; the 16 tiles of
+// 128 outputs and one chunk lie together (8 KB, one bulk copy), chunk after chunk. Lane l = 4 g + t
+// of a warp owns bytes 16 l .. 16 l + 15 of a tile: four 32-bit words of output row g, word w holding
+// inputs 32 w + 8 t + 0..7 of the chunk (input 2 p in nibble p, input 2 p + 1 in nibble p + 4). So a
+// tile is one coalesced 16-byte load per lane; (word >> 4 p) & 0x000f000f leaves two neighbouring
+// inputs in the two halves of a register; and one word of the four lanes of a row spans 32 inputs, the
+// smallest group, so a 16-input matrix instruction never mixes two groups. Scales and zero points lie
+// in the tiles' order, [8 outputs][128 / group] a tile. Outputs and inputs are padded to multiples of
+// 128 with code 8, zero point 8 and scale 0.
 struct Q4Weights {
     int n = 0, k = 0, group = 0;
     int chunks = 0;             // 128-input chunks per output
-    uint4* codes = nullptr;     // [round_up(n, 16) / 8][chunks][32 lanes]
-    __half* scales = nullptr;   // [round_up(n, 16) / 8][chunks][8][128 / group]
+    uint4* codes = nullptr;     // [ceil(n / 128)][chunks][16 tiles][32 lanes]
+    __half* scales = nullptr;   // [ceil(n / 128)][chunks][16 tiles][8][128 / group]
     uint8_t* zeros = nullptr;   // the same shape, or null: 8 everywhere
 };
+
+// The tile of outputs 8 t8 .. 8 t8 + 7 and chunk c.
+__host__ __device__ inline int64_t q4_tile(int64_t t8, int chunks, int c) {
+    return (t8 / 16 * chunks + c) * 16 + t8 % 16;
+}
 
 enum Q4Type : int { kQ4F32 = 0, kQ4BF16 = 1, kQ4F16 = 2 };
 

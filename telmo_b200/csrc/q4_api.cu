@@ -43,7 +43,7 @@ struct Staged {
 
 int upload_q4(Ctx* ctx, size_t n, size_t k, size_t group, const uint8_t* codes, const float* scales,
               const uint8_t* zeros, Weights* w) {
-    const size_t groups = (k + group - 1) / group, rows = (n + 15) / 16 * 16, chunks = (k + 127) / 128;
+    const size_t groups = (k + group - 1) / group, rows = (n + 127) / 128 * 128, chunks = (k + 127) / 128;
     for (size_t i = 0; i < n * groups; ++i)
         if (!(scales[i] == f16_value(scales[i])))
             return ctx->fail(TELMO_ERR_ARGUMENT,

@@ -17,15 +17,17 @@
 // share of the L2 reads is halved.
 //
 // One CTA per SM, persistent, 16 warps:
-//   warp 0        TMA producer: 64 inputs of BN / CG activation rows (per plane) a stage
-//   warp 1        MMA issuer: four K = 16 instructions per stage and plane
-//   warps 4-7     take the codes of 128 outputs apart: 16-byte loads of the tiled layout, one
-//                 chunk ahead in registers, and 16-byte stores into the stage's swizzled A tile
+//   warp 0        TMA: 64 inputs of BN / CG activation rows (per plane) a stage
+//   warp 1        issues the products: four K = 16 instructions per stage and plane
+//   warp 2        bulk copies of the codes (and zero points): 8 KB per 128 outputs and 128 inputs
+//   warps 4-7     take the codes apart and store them into the stage's swizzled A tile
 //   warps 8-15    add up: a group's sums from TMEM times its scale into registers (each thread one
 //                 output and BN / 2 rows), and after the last group the epilogue
 // TMEM holds several groups' accumulators, so the additions run behind the products. Registers are
-// dealt out by role (setmaxnreg; 40 + 104 + 2 * 184 a thread and warpgroup = 4 * 128 at launch). Every
-// wait is bounded; on timeout the kernel records kErrWaitTimeout and returns.
+// dealt out by role (setmaxnreg; 56 + 88 + 2 * 184 a thread and warpgroup = 4 * 128 at launch). Few
+// tiles are split along the inputs: the CTAs of a cluster take a share of the chunks each, exchange
+// their sums through distributed shared memory and finish a slice of the rows each, adding in rank
+// order. Every wait is bounded; on timeout the kernel records kErrWaitTimeout and returns.
 #include "ptx.cuh"
 #include "q4_device.cuh"
 #include "tma.h"
@@ -40,26 +42,30 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kStepK = 64;                    // inputs per stage: one 128-byte swizzled row of 16-bit values
 constexpr int kABytes = 128 * kStepK * 2;     // one CTA's A tile
+constexpr int kCodeBytes = 128 * 64;          // the codes of 128 outputs and one 128-input chunk
+constexpr int kCodeStage = kCodeBytes + 512;  // and their zero points
+constexpr int kCodeStages = 3;
 constexpr int kDrainWarps = 8;
 constexpr int kDequantWarps = 4;
-constexpr int kSmemBudget = 224 << 10;
+constexpr int kStageBudget = 192 << 10;
 
 template <int P, int BN, int CG>
 struct Shape {
-    static constexpr int kBRows = BN / CG;                     // activation rows a CTA stages, per plane
+    static constexpr int kBRows = BN / CG;  // activation rows a CTA stages, per plane
     static constexpr int kBPlane = kBRows * kStepK * 2;
     static constexpr int kStageBytes = kABytes + P * kBPlane;
-    static constexpr int kStages = std::min(8, (kSmemBudget - 2048) / kStageBytes);
-    static constexpr int kBufs = std::min(4, 512 / BN);        // accumulators in TMEM
+    static constexpr int kStages = std::min(8, kStageBudget / kStageBytes);
+    static constexpr int kBufs = std::min(4, 512 / BN);  // accumulators in TMEM
     static constexpr int kTmemCols = kBufs * BN;
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kCodeStages * kCodeStage + 1024 + 512;
 };
 
 struct GemmParams {
     const uint4* codes;
     const __half* scales;
     const uint8_t* zeros;
-    int n, k, chunks, tiles8;  // tiles8: 8-output tile rows of the layout
+    int n, k, chunks;
+    int per_chunk;  // groups per 128 inputs
     int m;
     const float* row_scale;  // [m] with two planes
     const float* bias;
@@ -69,6 +75,9 @@ struct GemmParams {
     void* c;
     int c_type;
     int64_t ldc;
+    int tiles, num_n;
+    int splits;        // CTAs (one cluster) that share a tile's inputs; 1 with pairs
+    int split_chunks;  // chunks of each
     uint32_t* error;
 };
 
@@ -82,76 +91,214 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint4 v) {
                  : "memory");
 }
 
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
 // (x, y) = (x, y) + d (a, b), each rounded once.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t d2, uint32_t a, uint32_t b) {
     const uint64_t ab = (static_cast<uint64_t>(b) << 32) | a;
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d2), "l"(ab));
 }
 
-// Zero points of one output row in one chunk, a byte per group.
-template <int GROUPS>
-__device__ __forceinline__ uint32_t load_zeros(const uint8_t* zeros, int64_t tile, int g) {
-    const uint8_t* z = zeros + (tile * 8 + g) * GROUPS;
-    if (GROUPS == 4) return __ldg(reinterpret_cast<const uint32_t*>(z));
-    if (GROUPS == 2) return __ldg(reinterpret_cast<const uint16_t*>(z));
-    return __ldg(z);
-}
-
-// One warp's codes of a chunk: four 8-output tiles.
-struct Codes {
-    uint4 v[4];
-    uint32_t z[4];
-};
-
-template <int GROUPS>
-__device__ __forceinline__ void load_codes(const GemmParams& p, int tile8, int c, int lane, Codes& w) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t8 = tile8 + i;
-        w.v[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-        w.z[i] = 0x08080808u;
-        if (t8 < p.tiles8) {
-            const int64_t tile = static_cast<int64_t>(t8) * p.chunks + c;
-            w.v[i] = __ldg(p.codes + tile * 32 + lane);
-            if (p.zeros) w.z[i] = load_zeros<GROUPS>(p.zeros, tile, lane >> 2);
-        }
-    }
-}
-
 template <bool BF16>
-__device__ __forceinline__ uint4 dequant_word(uint32_t word, uint32_t zero) {
-    const uint32_t base = code_base<BF16>(zero);
+__device__ __forceinline__ uint4 dequant_word(uint32_t word, uint32_t base) {
     return make_uint4(code_pair<BF16>(word, 0, base), code_pair<BF16>(word, 1, base), code_pair<BF16>(word, 2, base),
                       code_pair<BF16>(word, 3, base));
 }
 
-template <bool BF16, int P, int BN, int CG, int GROUPS>
+// Every thread of the cluster, at its own time (cluster_sync wants whole warps).
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Arrives on a barrier of either CTA of the pair. What it announces is shared memory that the
+// arriving warp's own SM will read (each lane's fence.proxy.async comes first) or TMEM that it has
+// finished reading, so no release at cluster scope is needed; one cost a membar of about 1000 cycles
+// per step (prompt of 4096 rows, 4096 -> 8192: 452 us with it, 289 without).
+__device__ __forceinline__ void arrive_pair(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// A ring position and its phase.
+template <int N>
+struct Ring {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) {
+            at = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// Stores one output of up to 16 rows.
+template <typename T>
+__device__ __forceinline__ void store_rows(const GemmParams& p, float (&v)[16], int row, int n) {
+    T* out = static_cast<T*>(p.c) + static_cast<int64_t>(row) * p.ldc + n;
+    const int rows = min(16, p.m - row);
+    if (p.accumulate) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < rows) v[j] += static_cast<float>(out[j * p.ldc]);
+    }
+    if (rows == 16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            *out = static_cast<T>(v[j]);
+            out += p.ldc;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < rows) out[j * p.ldc] = static_cast<T>(v[j]);
+    }
+}
+
+// The epilogue of one output's sums over 16 rows (those below m).
+template <int P>
+__device__ __forceinline__ void finish_rows(const GemmParams& p, const uint32_t (&sum)[16], int row, int n, float bias) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(sum[j]);
+    if (P == 2) {
+        const float4* rs = reinterpret_cast<const float4*>(p.row_scale + row);  // padded to whole tiles
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 s = __ldg(rs + j);
+            v[4 * j] *= s.x;
+            v[4 * j + 1] *= s.y;
+            v[4 * j + 2] *= s.z;
+            v[4 * j + 3] *= s.w;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += bias;
+    if (p.act == kActRelu) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = fmaxf(v[j], 0.0f);
+    } else if (p.act == kActSilu) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = mul_sigmoid(v[j], v[j]);
+    }
+    if (p.scale != 1.0f) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] *= p.scale;
+    }
+    if (p.c_type == kQ4F32) store_rows<float>(p, v, row, n);
+    else if (p.c_type == kQ4BF16) store_rows<__nv_bfloat16>(p, v, row, n);
+    else store_rows<__half>(p, v, row, n);
+}
+
+// One dequantizing warp's whole work: 32 of the CTA's 128 outputs.
+template <bool BF16, int STAGES, int STAGE_BYTES, int CG, bool ZEROS>
+__device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem, const uint8_t* code_ring, uint64_t* full,
+                                             uint64_t* empty, uint64_t* code_full, uint64_t* code_empty, int first,
+                                             int stride, int c0, int c1) {
+    const int dw = (threadIdx.x / 32) & 3, lane = threadIdx.x % 32;
+    const int g = lane >> 2, t4 = lane & 3, odd = g & 1;
+    // Row r's 16-byte segment s lies at s ^ (r % 8) of its 128 bytes. Rows of odd g store their
+    // second word first, so the two rows that share a store's phase use different banks.
+    const uint32_t row = static_cast<uint32_t>((dw * 32 + g) * 128);
+    const uint32_t at_a = row + static_cast<uint32_t>((4 * odd + t4) ^ g) * 16;
+    const uint32_t at_b = row + static_cast<uint32_t>((4 * (odd ^ 1) + t4) ^ g) * 16;
+    const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : smem_u32(full);
+    const uint32_t stage0 = smem_u32(smem);
+    Ring<STAGES> st;
+    Ring<kCodeStages> cs;
+    for (int t = first; t < p.tiles; t += stride) {
+        for (int c = c0; c < c1; ++c) {
+            if (!mbar_wait(&code_full[cs.at], cs.phase)) return false;
+            const uint8_t* src = code_ring + cs.at * kCodeStage;
+            uint4 v[4];
+            uint32_t z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = reinterpret_cast<const uint4*>(src)[(dw * 4 + i) * 32 + lane];
+                if (ZEROS) {
+                    // One byte per word: a group spans 4 / per_chunk of a lane's four words.
+                    const uint8_t* zs = src + kCodeBytes + ((dw * 4 + i) * 8 + g) * p.per_chunk;
+                    z[i] = p.per_chunk == 4   ? *reinterpret_cast<const uint32_t*>(zs)
+                           : p.per_chunk == 2 ? __byte_perm(*reinterpret_cast<const uint16_t*>(zs), 0, 0x1100)
+                                              : *zs * 0x01010101u;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&code_empty[cs.at]);
+            cs.next();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && c * 128 + kStepK >= p.k) break;
+                if (!mbar_wait(&empty[st.at], st.phase ^ 1)) return false;
+                const uint32_t a = stage0 + st.at * STAGE_BYTES;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t w0 = h ? v[i].z : v[i].x, w1 = h ? v[i].w : v[i].y;
+                    uint32_t b0 = code_base<BF16>(8), b1 = b0;
+                    if (ZEROS) {
+                        b0 = code_base<BF16>((z[i] >> (16 * h)) & 0xffu);
+                        b1 = code_base<BF16>((z[i] >> (16 * h + 8)) & 0xffu);
+                    }
+                    st_shared_v4(a + at_a + i * 1024, dequant_word<BF16>(odd ? w1 : w0, ZEROS && odd ? b1 : b0));
+                    st_shared_v4(a + at_b + i * 1024, dequant_word<BF16>(odd ? w0 : w1, ZEROS && odd ? b0 : b1));
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 1) mbar_arrive(&full[st.at]);
+                    else arrive_pair(full0 + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
+                }
+                st.next();
+            }
+        }
+    }
+    return true;
+}
+
+template <bool BF16, int P, int BN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     using S = Shape<P, BN, CG>;
     constexpr int kCols = BN / 2;  // activation rows per adding thread
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes);
+    uint8_t* code_ring = smem + S::kStages * S::kStageBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(code_ring + kCodeStages * kCodeStage);
     uint64_t* empty = full + S::kStages;
-    uint64_t* acc_full = empty + S::kStages;
+    uint64_t* code_full = empty + S::kStages;
+    uint64_t* code_empty = code_full + kCodeStages;
+    uint64_t* acc_full = code_empty + kCodeStages;
     uint64_t* acc_empty = acc_full + S::kBufs;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kBufs);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-    const bool leader = rank == 0;
-    const int unit = blockIdx.x / CG, units = gridDim.x / CG;
-    const int num_n = (p.n + CG * 128 - 1) / (CG * 128);
-    const int64_t tiles = static_cast<int64_t>((p.m + BN - 1) / BN) * num_n;
-    const int steps = (p.k + kStepK - 1) / kStepK;
-    const int groups = (p.k + 128 / GROUPS - 1) / (128 / GROUPS);
+    // A cluster is a pair (CG = 2) or the CTAs that share a tile's inputs.
+    const int splits = CG == 2 ? 1 : p.splits;
+    const uint32_t rank = CG == 2 || splits > 1 ? cluster_rank() : 0;
+    const int pair = CG == 2 ? static_cast<int>(rank) : 0;  // this CTA's 128 of the tile's outputs
+    const bool leader = pair == 0;
+    const int split = splits > 1 ? static_cast<int>(rank) : 0;
+    const int first = blockIdx.x / (CG * splits), stride = gridDim.x / (CG * splits);
+    const int c0 = split * p.split_chunks, c1 = min(p.chunks, c0 + p.split_chunks);
+    const int s0 = 2 * c0, s1 = min((p.k + kStepK - 1) / kStepK, 2 * c1);  // steps of 64 inputs
+    const int per_chunk = p.per_chunk;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1 + CG * kDequantWarps);
             mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kCodeStages; ++s) {
+            mbar_init(&code_full[s], 1);
+            mbar_init(&code_empty[s], kDequantWarps);
         }
         for (int b = 0; b < S::kBufs; ++b) {
             mbar_init(&acc_full[b], 1);
@@ -177,228 +324,266 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp < 4) {
-        regs_dec<40>();
+        regs_dec<56>();
         if (warp == 0 && lane == 0) {
             // ---- activations by TMA ----------------------------------------------------------
-            int stage = 0;
-            uint32_t phase = 0;
-            for (int64_t t = unit; t < tiles && !*abort_flag; t += units) {
-                const int m0 = static_cast<int>(t / num_n) * BN + static_cast<int>(rank) * S::kBRows;
-                for (int s = 0; s < steps; ++s) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1)) {
-                        gave_up(p, abort_flag);
-                        break;
-                    }
-                    uint8_t* b = smem + stage * S::kStageBytes + kABytes;
+            Ring<S::kStages> st;
+            bool ok = true;
+            for (int t = first; t < p.tiles && ok; t += stride) {
+                const int m0 = t / p.num_n * BN + pair * S::kBRows;
+                for (int s = s0; s < s1; ++s) {
+                    if (!(ok = mbar_wait(&empty[st.at], st.phase ^ 1))) break;
+                    uint8_t* b = smem + st.at * S::kStageBytes + kABytes;
                     if (CG == 1) {
-                        mbar_arrive_expect_tx(&full[stage], P * S::kBPlane);
+                        mbar_arrive_expect_tx(&full[st.at], P * S::kBPlane);
                         for (int pl = 0; pl < P; ++pl)
-                            tma_load_2d(&map_a, &full[stage], b + pl * S::kBPlane, s * kStepK, m0 + pl * p.m);
+                            tma_load_2d(&map_a, &full[st.at], b + pl * S::kBPlane, s * kStepK, m0 + pl * p.m);
                     } else {
                         // Both CTAs' loads count on the first CTA's barrier, which expects them all.
-                        const uint32_t bar = cluster_addr(&full[stage], 0);
-                        if (leader) mbar_arrive_expect_tx(&full[stage], 2 * P * S::kBPlane);
+                        const uint32_t bar = cluster_addr(&full[st.at], 0);
+                        if (leader) mbar_arrive_expect_tx(&full[st.at], 2 * P * S::kBPlane);
                         for (int pl = 0; pl < P; ++pl)
                             tma_load_2d_pair(&map_a, bar, b + pl * S::kBPlane, s * kStepK, m0 + pl * p.m);
                     }
-                    if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+                    st.next();
                 }
             }
+            if (!ok) gave_up(p, abort_flag);
         } else if (warp == 1 && leader) {
             // ---- products (the pair's first CTA issues for both) -----------------------------
-            constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-            constexpr int kHalves = GROUPS == 4 ? 2 : 1;      // groups that start within a step
-            constexpr int kPerHalf = kStepK / 16 / kHalves;   // K = 16 instructions of each
-            int stage = 0, buf = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            const uint32_t peer_empty = CG == 2 ? cluster_addr(&empty[0], 1) : 0;
-            const uint32_t peer_acc_full = CG == 2 ? cluster_addr(&acc_full[0], 1) : 0;
-            for (int64_t t = unit; t < tiles && !*abort_flag; t += units) {
-                bool ok = true;
-                for (int s = 0; s < steps && ok; ++s) {
-                    if (!(ok = mbar_wait(&full[stage], phase))) break;
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(smem + stage * S::kStageBytes), b = a + kABytes;
+            if (elect_one()) {
+                constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+                Ring<S::kStages> st;
+                Ring<S::kBufs> acc;
+                const uint32_t peer_empty = CG == 2 ? cluster_addr(&empty[0], 1) : 0;
+                const uint32_t peer_acc_full = CG == 2 ? cluster_addr(&acc_full[0], 1) : 0;
+                const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + kABytes);
+                const auto product = [&](uint32_t d, int kk, bool start) {
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) {
-                        if (GROUPS == 4 && h == 1 && s * kStepK + 32 >= p.k) break;
-                        const bool first = GROUPS != 1 || s % 2 == 0;
-                        const bool last = GROUPS != 1 || s % 2 == 1 || s == steps - 1;
-                        if (first) {
-                            if (!(ok = mbar_wait(&acc_empty[buf], acc_phase ^ 1))) break;
+                    for (int pl = 0; pl < P; ++pl) {
+                        const uint64_t off = static_cast<uint64_t>((st.at * S::kStageBytes + kk * 32) >> 4);
+                        const uint64_t da = a0 + off, db = b0 + off + static_cast<uint64_t>(pl * S::kBPlane >> 4);
+                        const uint32_t add = start && pl == 0 ? 0u : 1u;
+                        if (CG == 1) mma_f16(d, da, db, idesc, add);
+                        else mma_f16_pair(d, da, db, idesc, add);
+                    }
+                };
+                const auto commit_acc = [&] {
+                    if (CG == 1) {
+                        mma_commit(&acc_full[acc.at]);
+                    } else {
+                        mma_commit_pair(smem_u32(&acc_full[acc.at]));
+                        mma_commit_pair(peer_acc_full + static_cast<uint32_t>(acc.at * sizeof(uint64_t)));
+                    }
+                    acc.next();
+                };
+                bool ok = true;
+                for (int t = first; t < p.tiles && ok; t += stride) {
+                    for (int s = s0; s < s1 && ok; ++s) {
+                        if (!(ok = mbar_wait(&full[st.at], st.phase))) break;
+                        tc_fence_after();
+                        // A group is two steps (128 inputs), one, or half of one.
+                        if (per_chunk != 1 || s % 2 == 0) {
+                            if (!(ok = mbar_wait(&acc_empty[acc.at], acc.phase ^ 1))) break;
                             tc_fence_after();
                         }
-                        if (lane == 0) {
-                            const uint32_t d = tmem_base + static_cast<uint32_t>(buf * BN);
-#pragma unroll
-                            for (int i = 0; i < kPerHalf; ++i) {
-                                const int kk = h * kPerHalf + i;
-#pragma unroll
-                                for (int pl = 0; pl < P; ++pl) {
-                                    const uint64_t da = sw128_desc(a + kk * 32);
-                                    const uint64_t db = sw128_desc(b + pl * S::kBPlane + kk * 32);
-                                    const uint32_t add = first && i == 0 && pl == 0 ? 0u : 1u;
-                                    if (CG == 1) mma_f16(d, da, db, idesc, add);
-                                    else mma_f16_pair(d, da, db, idesc, add);
-                                }
+                        uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * BN);
+                        product(d, 0, per_chunk != 1 || s % 2 == 0);
+                        product(d, 1, false);
+                        if (per_chunk == 4) {
+                            commit_acc();
+                            if (s * kStepK + 32 < p.k) {
+                                if (!(ok = mbar_wait(&acc_empty[acc.at], acc.phase ^ 1))) break;
+                                tc_fence_after();
+                                d = tmem_base + static_cast<uint32_t>(acc.at * BN);
+                                product(d, 2, true);
+                                product(d, 3, false);
+                                commit_acc();
                             }
-                            if (last) {
-                                if (CG == 1) {
-                                    mma_commit(&acc_full[buf]);
-                                } else {
-                                    mma_commit_pair(smem_u32(&acc_full[buf]));
-                                    mma_commit_pair(peer_acc_full + static_cast<uint32_t>(buf * sizeof(uint64_t)));
-                                }
-                            }
-                        }
-                        __syncwarp();
-                        if (last && ++buf == S::kBufs) { buf = 0; acc_phase ^= 1; }
-                    }
-                    if (!ok) break;
-                    if (lane == 0) {
-                        if (CG == 1) {
-                            mma_commit(&empty[stage]);
                         } else {
-                            mma_commit_pair(smem_u32(&empty[stage]));
-                            mma_commit_pair(peer_empty + static_cast<uint32_t>(stage * sizeof(uint64_t)));
+                            product(d, 2, false);
+                            product(d, 3, false);
+                            if (per_chunk == 2 || s % 2 == 1 || s == s1 - 1) commit_acc();
                         }
+                        if (CG == 1) {
+                            mma_commit(&empty[st.at]);
+                        } else {
+                            mma_commit_pair(smem_u32(&empty[st.at]));
+                            mma_commit_pair(peer_empty + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
+                        }
+                        st.next();
                     }
-                    __syncwarp();
-                    if (++stage == S::kStages) { stage = 0; phase ^= 1; }
                 }
-                if (!ok) {
-                    gave_up(p, abort_flag);
-                    break;
+                if (!ok) gave_up(p, abort_flag);
+            }
+        } else if (warp == 2 && lane == 0) {
+            // ---- codes and zero points: contiguous per 128 outputs and chunk ------------------
+            Ring<kCodeStages> cs;
+            bool ok = true;
+            const uint32_t zero_bytes = p.zeros ? 128u * static_cast<uint32_t>(per_chunk) : 0u;
+            for (int t = first; t < p.tiles && ok; t += stride) {
+                // A pair's second CTA may have no outputs of its own: it repeats the last ones.
+                const int block = min(t % p.num_n * CG + pair, (p.n + 127) / 128 - 1);
+                for (int c = c0; c < c1; ++c) {
+                    if (!(ok = mbar_wait(&code_empty[cs.at], cs.phase ^ 1))) break;
+                    uint8_t* dst = code_ring + cs.at * kCodeStage;
+                    const int64_t at = static_cast<int64_t>(block) * p.chunks + c;
+                    mbar_arrive_expect_tx(&code_full[cs.at], kCodeBytes + zero_bytes);
+                    bulk_load(dst, reinterpret_cast<const uint8_t*>(p.codes) + at * kCodeBytes, kCodeBytes, &code_full[cs.at]);
+                    if (zero_bytes) bulk_load(dst + kCodeBytes, p.zeros + at * zero_bytes, zero_bytes, &code_full[cs.at]);
+                    cs.next();
                 }
             }
+            if (!ok) gave_up(p, abort_flag);
         }
     } else if (warp < 8) {
-        regs_dec<104>();
-        // ---- weights: codes to operands ------------------------------------------------------
-        const int dw = warp - 4;
-        const int g = lane >> 2, t4 = lane & 3, odd = g & 1;
-        int stage = 0;
-        uint32_t phase = 0;
-        const uint32_t full0 = CG == 2 ? cluster_addr(&full[0], 0) : 0;
-        const auto first_tile = [&](int64_t t) {
-            return (static_cast<int>(t % num_n) * CG + static_cast<int>(rank)) * 16 + dw * 4;
-        };
-        Codes now, next;
-        int64_t t = unit;
-        int c = 0;
-        if (t < tiles) load_codes<GROUPS>(p, first_tile(t), 0, lane, now);
-        while (t < tiles && !*abort_flag) {
-            int64_t tn = t;
-            int cn = c + 1;
-            if (cn == p.chunks) {
-                cn = 0;
-                tn = t + units;
-            }
-            if (tn < tiles) load_codes<GROUPS>(p, first_tile(tn), cn, lane, next);
-            bool ok = true;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 1 && c * 128 + kStepK >= p.k) break;
-                if (!(ok = mbar_wait(&empty[stage], phase ^ 1))) break;
-                const uint32_t a = smem_u32(smem + stage * S::kStageBytes);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w0 = h ? now.v[i].z : now.v[i].x, w1 = h ? now.v[i].w : now.v[i].y;
-                    // Groups of the two words' inputs within the chunk.
-                    const int q0 = GROUPS == 4 ? 2 * h : GROUPS == 2 ? h : 0, q1 = GROUPS == 4 ? 2 * h + 1 : q0;
-                    const uint32_t z0 = (now.z[i] >> (8 * q0)) & 0xffu, z1 = (now.z[i] >> (8 * q1)) & 0xffu;
-                    // Row r's 16-byte segment s lies at s ^ (r % 8). Rows of odd g store their second
-                    // word first, so the two rows that share a store's phase use different banks.
-                    const uint32_t row = a + static_cast<uint32_t>(((dw * 4 + i) * 8 + g) * 128);
-                    const uint32_t sa = static_cast<uint32_t>((4 * odd + t4) ^ g), sb = static_cast<uint32_t>((4 * (odd ^ 1) + t4) ^ g);
-                    st_shared_v4(row + sa * 16, dequant_word<BF16>(odd ? w1 : w0, odd ? z1 : z0));
-                    st_shared_v4(row + sb * 16, dequant_word<BF16>(odd ? w0 : w1, odd ? z0 : z1));
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 1) mbar_arrive(&full[stage]);
-                    else mbar_arrive_cluster(full0 + static_cast<uint32_t>(stage * sizeof(uint64_t)));
-                }
-                if (++stage == S::kStages) { stage = 0; phase ^= 1; }
-            }
-            if (!ok) {
-                gave_up(p, abort_flag);
-                break;
-            }
-            now = next;
-            t = tn;
-            c = cn;
-        }
+        regs_dec<88>();
+        const bool ok =
+            p.zeros ? dequant_role<BF16, S::kStages, S::kStageBytes, CG, true>(p, smem, code_ring, full, empty, code_full,
+                                                                               code_empty, first, stride, c0, c1)
+                    : dequant_role<BF16, S::kStages, S::kStageBytes, CG, false>(p, smem, code_ring, full, empty, code_full,
+                                                                                code_empty, first, stride, c0, c1);
+        if (!ok) gave_up(p, abort_flag);
     } else {
         regs_inc<184>();
         // ---- sums and epilogue: thread = one output, kCols activation rows --------------------
         const int quad = warp & 3, half = (warp - 8) / 4;
-        int buf = 0;
-        uint32_t acc_phase = 0;
+        const int lane_row = quad * 32 + lane;
+        Ring<S::kBufs> ab;
         const uint32_t acc_empty0 = CG == 2 ? cluster_addr(&acc_empty[0], 0) : 0;
-        for (int64_t t = unit; t < tiles && !*abort_flag; t += units) {
-            const int m0 = static_cast<int>(t / num_n) * BN + half * kCols;
-            const int n = (static_cast<int>(t % num_n) * CG + static_cast<int>(rank)) * 128 + quad * 32 + lane;
+        for (int t = first; t < p.tiles; t += stride) {
+            const int m0 = t / p.num_n * BN + half * kCols;
+            const int n = (t % p.num_n * CG + pair) * 128 + lane_row;
             const bool n_ok = n < p.n;
-            // This output's scales: GROUPS per chunk, the next group's loaded a group ahead.
-            const __half* sc = p.scales + (static_cast<int64_t>(n / 8) * p.chunks * 8 + n % 8) * GROUPS;
-            float d = n_ok ? __half2float(__ldg(sc)) : 0.0f;
+            // This output's scales, 2 per_chunk bytes a chunk, loaded a chunk ahead.
+            const uint8_t* sc = reinterpret_cast<const uint8_t*>(p.scales) +
+                                ((static_cast<int64_t>(n / 128) * p.chunks + c0) * 128 + lane_row) * per_chunk * 2;
+            const auto load_scales = [&]() -> uint64_t {
+                uint64_t v = 0;
+                if (n_ok)
+                    v = per_chunk == 4   ? __ldg(reinterpret_cast<const unsigned long long*>(sc))
+                        : per_chunk == 2 ? __ldg(reinterpret_cast<const uint32_t*>(sc))
+                                         : __ldg(reinterpret_cast<const uint16_t*>(sc));
+                sc += 256 * per_chunk;
+                return v;
+            };
+            uint64_t next = c0 < c1 ? load_scales() : 0;
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int j = 0; j < kCols / 2; ++j) acc[j] = 0;
             bool ok = true;
-#pragma unroll 1
-            for (int gi = 0; gi < groups; ++gi) {
-                const float d_now = d;
-                if (gi + 1 < groups && n_ok)
-                    d = __half2float(__ldg(sc + static_cast<int64_t>((gi + 1) / GROUPS) * 8 * GROUPS + (gi + 1) % GROUPS));
-                ok = mbar_wait(&acc_full[buf], acc_phase);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                                       static_cast<uint32_t>(buf * BN + half * kCols);
-                const uint64_t d2 = pack_f2(make_float2(d_now, d_now));
-#pragma unroll
-                for (int q = 0; q < kCols / 32; ++q) {
-                    uint32_t r[32];
-                    tmem_ld32(taddr + q * 32, r);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) fma2(acc[q * 16 + j], d2, r[2 * j], r[2 * j + 1]);
-                }
+            const auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (CG == 1) mbar_arrive(&acc_empty[buf]);
-                    else mbar_arrive_cluster(acc_empty0 + static_cast<uint32_t>(buf * sizeof(uint64_t)));
+                    if (CG == 1) mbar_arrive(&acc_empty[ab.at]);
+                    else arrive_pair(acc_empty0 + static_cast<uint32_t>(ab.at * sizeof(uint64_t)));
                 }
-                if (++buf == S::kBufs) { buf = 0; acc_phase ^= 1; }
+                ab.next();
+            };
+#pragma unroll 1
+            for (int c = c0; c < c1 && ok; ++c) {
+                uint64_t now = next;
+                if (c + 1 < c1) next = load_scales();
+                const int left = p.k - c * 128, size = 128 / per_chunk;
+#pragma unroll 1
+                for (int i = 0; i < left && i < 128; i += size, now >>= 16) {
+                    const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(now & 0xffff)));
+                    ok = mbar_wait(&acc_full[ab.at], ab.phase);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                                           static_cast<uint32_t>(ab.at * BN + half * kCols);
+                    const uint64_t d2 = pack_f2(make_float2(d, d));
+                    // 16 columns are added while the next 16 are on their way.
+                    uint32_t r[2][16];
+                    tmem_ld16(taddr, r[0]);
+#pragma unroll
+                    for (int q = 0; q < kCols / 16; ++q) {
+                        tmem_ld_wait();
+                        if (q + 1 < kCols / 16) tmem_ld16(taddr + (q + 1) * 16, r[(q + 1) & 1]);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) fma2(acc[q * 8 + j], d2, r[q & 1][2 * j], r[q & 1][2 * j + 1]);
+                    }
+                    if (c == c1 - 1 && i + size >= left) break;  // the tile's last accumulator is kept
+                    release();
+                }
             }
             if (!ok) {
                 gave_up(p, abort_flag);
+                if (splits > 1) {
+                    cluster_meet();
+                    cluster_meet();
+                }
                 break;
             }
             const float bias = p.bias && n_ok ? __ldg(p.bias + n) : 0.0f;
+            if (CG == 2 || splits == 1) {
+                // The sums go back to the last accumulator's columns, from where a rolled loop can take
+                // them (registers cannot be indexed): the epilogue's code stays small. Unrolled over
+                // all columns it kept the instruction cache busy (1500 rows, 1024 -> 4096: 89 us).
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                                       static_cast<uint32_t>(ab.at * BN + half * kCols);
+#pragma unroll
+                for (int q = 0; q < kCols / 32; ++q) {
+                    uint32_t r[32];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        r[2 * j] = static_cast<uint32_t>(acc[q * 16 + j]);
+                        r[2 * j + 1] = static_cast<uint32_t>(acc[q * 16 + j] >> 32);
+                    }
+                    tmem_st32(taddr + q * 32, r);
+                }
+                tmem_st_wait();
+#pragma unroll 1
+                for (int q = 0; q < kCols / 16; ++q) {
+                    const int row = m0 + q * 16;
+                    if (row >= p.m) break;
+                    uint32_t r[16];
+                    tmem_ld16(taddr + q * 16, r);
+                    tmem_ld_wait();
+                    if (n_ok) finish_rows<P>(p, r, row, n, bias);
+                    __syncwarp();
+                }
+                release();
+                continue;
+            }
+            // The tile's CTAs each finish a slice of its rows: every CTA sends its sums of a slice to the
+            // slice's CTA, which adds them in rank order. The stages are free: all of a CTA's products
+            // have been added up, here and, after the barrier, in the others.
+            const int slice = kCols / splits, log = __ffs(slice) - 1;
+            cluster_meet();
 #pragma unroll
             for (int j = 0; j < kCols; ++j) {
-                const int row = m0 + j;
-                if (row >= p.m || !n_ok) continue;
-                const float2 pair = unpack_f2(acc[j / 2]);
-                float v = j % 2 ? pair.y : pair.x;
+                const float2 pair_v = unpack_f2(acc[j / 2]);
+                const uint32_t to = cluster_addr(smem, static_cast<uint32_t>(j >> log));
+                st_cluster_f32(to + static_cast<uint32_t>((((split * 2 + half) * slice + (j & (slice - 1))) * 128 + lane_row) * 4),
+                               j % 2 ? pair_v.y : pair_v.x);
+            }
+            cluster_meet();
+            const float* parts = reinterpret_cast<const float*>(smem);
+            for (int j = 0; j < slice; ++j) {
+                const int row = m0 + split * slice + j;
+                if (row >= p.m || !n_ok) break;
+                float v = 0.0f;
+                for (int q = 0; q < splits; ++q) v += parts[((q * 2 + half) * slice + j) * 128 + lane_row];
                 if (P == 2) v *= __ldg(p.row_scale + row);
                 v = q4_act(v + bias, p.act) * p.scale;
                 const int64_t at = static_cast<int64_t>(row) * p.ldc + n;
                 if (p.accumulate) v += q4_load(p.c, p.c_type, at);
                 q4_store(p.c, p.c_type, at, v);
             }
-            __syncwarp();
         }
     }
 
+    if (CG == 1 && splits > 1 && warp < 8) {
+        // The two meetings of the adding warps' exchange, which count every thread of the cluster.
+        cluster_meet();
+        cluster_meet();
+    }
     tc_fence_before();
     __syncthreads();
     // A pair's CTAs leave together: the first CTA's products read the second's shared memory and
@@ -450,16 +635,16 @@ __global__ void __launch_bounds__(kPrepThreads) q4_align_kernel(const uint16_t* 
     for (int i = threadIdx.x; i < ld; i += kPrepThreads) out[row * ld + i] = i < k ? __ldg(a + row * lda + i) : uint16_t(0);
 }
 
-template <bool BF16, int P, int BN, int CG, int GROUPS>
-cudaError_t launch_gemm(const void* a, int64_t lda, const GemmParams& p, int sms, cudaStream_t stream) {
+template <bool BF16, int P, int BN, int CG>
+cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, int sms, cudaStream_t stream) {
     using S = Shape<P, BN, CG>;
     static DeviceOnce once;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!once.done(dev)) {
-        if ((e = cudaFuncSetAttribute(q4_gemm_kernel<BF16, P, BN, CG, GROUPS>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes)) != cudaSuccess)
+        if ((e = cudaFuncSetAttribute(q4_gemm_kernel<BF16, P, BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      S::kSmemBytes)) != cudaSuccess)
             return e;
         once.mark(dev);
     }
@@ -468,38 +653,40 @@ cudaError_t launch_gemm(const void* a, int64_t lda, const GemmParams& p, int sms
                        static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m) * P, static_cast<uint64_t>(lda) * 2, kStepK,
                        S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
-    const int64_t tiles = static_cast<int64_t>((p.m + BN - 1) / BN) * ((p.n + CG * 128 - 1) / (CG * 128));
+    p.num_n = (p.n + CG * 128 - 1) / (CG * 128);
+    const int64_t tiles = static_cast<int64_t>((p.m + BN - 1) / BN) * p.num_n;
+    if (tiles > (1 << 28)) return cudaErrorInvalidValue;
+    p.tiles = static_cast<int>(tiles);
+    p.splits = splits;
+    p.split_chunks = (p.chunks + splits - 1) / splits;
+    const int cluster = CG * splits;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CG * static_cast<unsigned>(std::min<int64_t>(tiles, sms / CG)));
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster * std::min(p.tiles, splits > 1 ? p.tiles : sms / CG)));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = S::kSmemBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, q4_gemm_kernel<BF16, P, BN, CG, GROUPS>, map, p);
-}
-
-template <bool BF16, int P, int BN, int CG>
-cudaError_t launch_group(const void* a, int64_t lda, const GemmParams& p, int group, int sms, cudaStream_t stream) {
-    if (group == 32) return launch_gemm<BF16, P, BN, CG, 4>(a, lda, p, sms, stream);
-    if (group == 64) return launch_gemm<BF16, P, BN, CG, 2>(a, lda, p, sms, stream);
-    return launch_gemm<BF16, P, BN, CG, 1>(a, lda, p, sms, stream);
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, q4_gemm_kernel<BF16, P, BN, CG>, map, p);
 }
 
 template <bool BF16, int P>
-cudaError_t launch_shape(const void* a, int64_t lda, const GemmParams& p, int group, int sms, cudaStream_t stream) {
-    // Pairs on 256 x 256 tiles where they fill the GPU, else smaller tiles on single CTAs.
+cudaError_t launch_shape(const void* a, int64_t lda, const GemmParams& p, int sms, cudaStream_t stream) {
+    // Pairs on 256 x 256 tiles where they fill the GPU, else smaller tiles on single CTAs, and where
+    // those leave SMs idle clusters of up to eight CTAs that share a tile's inputs.
     const auto tiles = [&](int bn, int features) {
         return static_cast<int64_t>((p.m + bn - 1) / bn) * ((p.n + features - 1) / features);
     };
-    if (tiles(256, 256) * 2 >= sms) return launch_group<BF16, P, 256, 2>(a, lda, p, group, sms, stream);
-    if (tiles(128, 128) >= sms) return launch_group<BF16, P, 128, 1>(a, lda, p, group, sms, stream);
-    return launch_group<BF16, P, 64, 1>(a, lda, p, group, sms, stream);
+    if (tiles(256, 256) * 2 >= sms) return launch_gemm<BF16, P, 256, 2>(a, lda, p, 1, sms, stream);
+    if (tiles(128, 128) >= sms) return launch_gemm<BF16, P, 128, 1>(a, lda, p, 1, sms, stream);
+    int splits = 1;
+    while (splits < 8 && tiles(64, 128) * splits * 2 <= sms && splits * 4 <= p.chunks) splits *= 2;
+    return launch_gemm<BF16, P, 64, 1>(a, lda, p, splits, sms, stream);
 }
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -508,7 +695,7 @@ size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 size_t q4_gemm_workspace(const Q4Args& g) {
     const size_t m = static_cast<size_t>(g.m), ld = round_up(static_cast<size_t>(g.w->k), 8);
-    if (g.a_type == kQ4F32) return round_up(2 * m * ld * sizeof(__half), 256) + m * sizeof(float);
+    if (g.a_type == kQ4F32) return round_up(2 * m * ld * sizeof(__half), 256) + round_up(m, 256) * sizeof(float);
     const bool aligned = reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda % 8 == 0;
     return aligned ? 0 : m * ld * 2;
 }
@@ -521,7 +708,8 @@ cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream
     p.n = g.w->n;
     p.k = g.w->k;
     p.chunks = g.w->chunks;
-    p.tiles8 = (g.w->n + 15) / 16 * 2;
+    p.per_chunk = 128 / g.w->group;
+    p.tiles = p.num_n = p.splits = p.split_chunks = 0;
     p.m = g.m;
     p.row_scale = nullptr;
     p.bias = g.bias;
@@ -540,7 +728,7 @@ cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream
         q4_split_kernel<<<p.m, kPrepThreads, 0, stream>>>(static_cast<const float*>(g.a), g.lda, p.m, p.k, planes, ld, rs);
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
         p.row_scale = rs;
-        return launch_shape<false, 2>(planes, ld, p, g.w->group, g.sms, stream);
+        return launch_shape<false, 2>(planes, ld, p, g.sms, stream);
     }
     const void* a = g.a;
     int64_t lda = g.lda;
@@ -551,8 +739,8 @@ cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream
         a = workspace;
         lda = ld;
     }
-    return g.a_type == kQ4BF16 ? launch_shape<true, 1>(a, lda, p, g.w->group, g.sms, stream)
-                               : launch_shape<false, 1>(a, lda, p, g.w->group, g.sms, stream);
+    return g.a_type == kQ4BF16 ? launch_shape<true, 1>(a, lda, p, g.sms, stream)
+                               : launch_shape<false, 1>(a, lda, p, g.sms, stream);
 }
 
 }  // namespace telmo

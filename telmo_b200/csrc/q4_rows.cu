@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) q4_rows_kernel(const RowsParam
         RowScales<GROUPS> sc[2 * R];
 #pragma unroll
         for (int r = 0; r < 2 * R; ++r) {
-            const int64_t tile = (tile0 + r) * p.chunks + c;
+            const int64_t tile = q4_tile(tile0 + r, p.chunks, c);
             words[r] = __ldg(p.codes + tile * 32 + lane);
             sc[r] = load_scales<GROUPS, ZEROS>(p, tile, g);
         }
@@ -281,8 +281,9 @@ __global__ void q4_repack_kernel(const uint8_t* codes, const float* scales, cons
     const int64_t tile = word / 128;
     const int in = static_cast<int>(word % 128);
     const int lane = in / 4, wi = in % 4;
-    const int64_t o = tile / w.chunks * 8 + lane / 4;
-    const int c = static_cast<int>(tile % w.chunks);
+    const int64_t o0 = (tile / 16 / w.chunks * 16 + tile % 16) * 8;
+    const int64_t o = o0 + lane / 4;
+    const int c = static_cast<int>(tile / 16 % w.chunks);
     const int i0 = c * 128 + 32 * wi + 8 * (lane % 4);
     const int64_t row_bytes = (static_cast<int64_t>(w.k) + 1) / 2;
     uint32_t v = 0;
@@ -298,7 +299,7 @@ __global__ void q4_repack_kernel(const uint8_t* codes, const float* scales, cons
     // The first of a tile's threads write its scales and zero points.
     const int per = 128 / w.group;
     if (in < 8 * per) {
-        const int64_t so = tile / w.chunks * 8 + in / per;
+        const int64_t so = o0 + in / per;
         const int64_t groups = (static_cast<int64_t>(w.k) + w.group - 1) / w.group;
         const int64_t q = static_cast<int64_t>(c) * per + in % per;
         const bool ok = so < w.n && q < groups;
@@ -311,7 +312,7 @@ __global__ void q4_repack_kernel(const uint8_t* codes, const float* scales, cons
 
 cudaError_t q4_repack(const uint8_t* codes, const float* scales, const uint8_t* zeros, const Q4Weights& w,
                       cudaStream_t stream) {
-    const int64_t tiles = (static_cast<int64_t>(w.n) + 15) / 16 * 2 * w.chunks;
+    const int64_t tiles = (static_cast<int64_t>(w.n) + 127) / 128 * 16 * w.chunks;
     const int64_t blocks = (tiles * 128 + 255) / 256;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
     q4_repack_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(codes, scales, zeros, w, tiles);
