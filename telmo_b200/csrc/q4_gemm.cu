@@ -17,8 +17,8 @@
 // share of the L2 reads is halved.
 //
 // One CTA per SM, persistent, 16 warps:
-//   warp 0        TMA: 64 inputs of BN / CG activation rows (per plane) a stage
-//   warp 1        issues the products: four K = 16 instructions per stage and plane
+//   warp 0        TMA: 128 inputs of BN / CG activation rows (per plane) a stage
+//   warp 1        issues the products: eight K = 16 instructions per stage and plane
 //   warp 2        bulk copies of the codes (and zero points): 8 KB per 128 outputs and 128 inputs
 //   warps 4-7     take the codes apart and store them into the stage's swizzled A tile
 //   warps 8-15    add up: a group's sums from TMEM times its scale into registers (each thread one
@@ -34,14 +34,15 @@
 
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 namespace telmo {
 
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kStepK = 64;                    // inputs per stage: one 128-byte swizzled row of 16-bit values
-constexpr int kABytes = 128 * kStepK * 2;     // one CTA's A tile
+constexpr int kHalfK = 64;                    // inputs of one 128-byte swizzled row of 16-bit values
+constexpr int kAHalf = 128 * kHalfK * 2;      // one CTA's A tile of 64 inputs
 constexpr int kCodeBytes = 128 * 64;          // the codes of 128 outputs and one 128-input chunk
 constexpr int kCodeStage = kCodeBytes + 512;  // and their zero points
 constexpr int kCodeStages = 3;
@@ -52,9 +53,9 @@ constexpr int kStageBudget = 192 << 10;
 template <int P, int BN, int CG>
 struct Shape {
     static constexpr int kBRows = BN / CG;  // activation rows a CTA stages, per plane
-    static constexpr int kBPlane = kBRows * kStepK * 2;
-    static constexpr int kStageBytes = kABytes + P * kBPlane;
-    static constexpr int kStages = std::min(8, kStageBudget / kStageBytes);
+    static constexpr int kBHalf = kBRows * kHalfK * 2;  // of one plane and 64 inputs
+    static constexpr int kStageBytes = 2 * kAHalf + 2 * P * kBHalf;
+    static constexpr int kStages = std::min(4, kStageBudget / kStageBytes);
     static constexpr int kBufs = std::min(4, 512 / BN);  // accumulators in TMEM
     static constexpr int kTmemCols = kBufs * BN;
     static constexpr int kSmemBytes = kStages * kStageBytes + kCodeStages * kCodeStage + 1024 + 512;
@@ -124,6 +125,22 @@ __device__ __forceinline__ void cluster_meet() {
 // per step (prompt of 4096 rows, 4096 -> 8192: 452 us with it, 289 without).
 __device__ __forceinline__ void arrive_pair(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// mbar_wait with a longer run of polls before it sleeps: these waits are short and follow one another.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kWaitPolls; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (i > 4096) __nanosleep(256);
+    }
+    return false;
+}
+
+// Arrives on the same barrier of both CTAs of the pair once this thread's products are complete.
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
 // A ring position and its phase.
@@ -215,7 +232,7 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
     Ring<kCodeStages> cs;
     for (int t = first; t < p.tiles; t += stride) {
         for (int c = c0; c < c1; ++c) {
-            if (!mbar_wait(&code_full[cs.at], cs.phase)) return false;
+            if (!wait_for(&code_full[cs.at], cs.phase)) return false;
             const uint8_t* src = code_ring + cs.at * kCodeStage;
             uint4 v[4];
             uint32_t z[4];
@@ -230,33 +247,84 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
                                               : *zs * 0x01010101u;
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&code_empty[cs.at]);
-            cs.next();
+            if (!wait_for(&empty[st.at], st.phase ^ 1)) return false;
+            const uint32_t a = stage0 + st.at * STAGE_BYTES;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 1 && c * 128 + kStepK >= p.k) break;
-                if (!mbar_wait(&empty[st.at], st.phase ^ 1)) return false;
-                const uint32_t a = stage0 + st.at * STAGE_BYTES;
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int h = 0; h < 2; ++h) {
                     const uint32_t w0 = h ? v[i].z : v[i].x, w1 = h ? v[i].w : v[i].y;
                     uint32_t b0 = code_base<BF16>(8), b1 = b0;
                     if (ZEROS) {
                         b0 = code_base<BF16>((z[i] >> (16 * h)) & 0xffu);
                         b1 = code_base<BF16>((z[i] >> (16 * h + 8)) & 0xffu);
                     }
-                    st_shared_v4(a + at_a + i * 1024, dequant_word<BF16>(odd ? w1 : w0, ZEROS && odd ? b1 : b0));
-                    st_shared_v4(a + at_b + i * 1024, dequant_word<BF16>(odd ? w0 : w1, ZEROS && odd ? b0 : b1));
+                    const uint32_t at = a + h * kAHalf + i * 1024;
+                    st_shared_v4(at + at_a, dequant_word<BF16>(odd ? w1 : w0, ZEROS && odd ? b1 : b0));
+                    st_shared_v4(at + at_b, dequant_word<BF16>(odd ? w0 : w1, ZEROS && odd ? b0 : b1));
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 1) mbar_arrive(&full[st.at]);
-                    else arrive_pair(full0 + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
-                }
-                st.next();
             }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(&full[st.at]);
+                else arrive_pair(full0 + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
+                // Only now: the codes have reached registers, since their operands are stored.
+                mbar_arrive(&code_empty[cs.at]);
+            }
+            st.next();
+            cs.next();
+        }
+    }
+    return true;
+}
+
+// The issuing warp's whole work. All lanes walk the loops, so that addresses and descriptors stay in
+// uniform registers; the elected one issues. PER_CHUNK groups of 128 / PER_CHUNK inputs to a stage.
+template <bool BF16, int P, int BN, int CG, int PER_CHUNK>
+__device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, uint64_t* full, uint64_t* empty,
+                                           uint64_t* acc_full, uint64_t* acc_empty, uint32_t tmem_base, int first,
+                                           int stride, int c0, int c1) {
+    using S = Shape<P, BN, CG>;
+    constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+    constexpr int kSteps = 8 / PER_CHUNK;  // K = 16 instructions to a group
+    const bool issuer = elect_one();
+    Ring<S::kStages> st;
+    Ring<S::kBufs> acc;
+    const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + 2 * kAHalf);
+    for (int t = first; t < p.tiles; t += stride) {
+        for (int c = c0; c < c1; ++c) {
+            if (!wait_for(&full[st.at], st.phase)) return false;
+            tc_fence_after();
+            const uint64_t off = static_cast<uint64_t>(st.at * S::kStageBytes) >> 4;
+#pragma unroll
+            for (int q = 0; q < PER_CHUNK; ++q) {
+                if (q > 0 && c * 128 + q * (128 / PER_CHUNK) >= p.k) break;
+                if (!wait_for(&acc_empty[acc.at], acc.phase ^ 1)) return false;
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * BN);
+                if (issuer) {
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        const int kk = q * kSteps + i;  // of the stage's eight
+#pragma unroll
+                        for (int pl = 0; pl < P; ++pl) {
+                            const uint64_t da = a0 + off + static_cast<uint64_t>(((kk / 4) * kAHalf + (kk % 4) * 32) >> 4);
+                            const uint64_t db = b0 + off + static_cast<uint64_t>(((pl * 2 + kk / 4) * S::kBHalf + (kk % 4) * 32) >> 4);
+                            if (CG == 1) mma_f16(d, da, db, idesc, i + pl > 0);
+                            else mma_f16_pair(d, da, db, idesc, i + pl > 0);
+                        }
+                    }
+                    if (CG == 1) mma_commit(&acc_full[acc.at]);
+                    else commit_both(&acc_full[acc.at]);
+                }
+                acc.next();
+            }
+            if (issuer) {
+                if (CG == 1) mma_commit(&empty[st.at]);
+                else commit_both(&empty[st.at]);
+            }
+            st.next();
         }
     }
     return true;
@@ -288,7 +356,6 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     const int split = splits > 1 ? static_cast<int>(rank) : 0;
     const int first = blockIdx.x / (CG * splits), stride = gridDim.x / (CG * splits);
     const int c0 = split * p.split_chunks, c1 = min(p.chunks, c0 + p.split_chunks);
-    const int s0 = 2 * c0, s1 = min((p.k + kStepK - 1) / kStepK, 2 * c1);  // steps of 64 inputs
     const int per_chunk = p.per_chunk;
 
     if (threadIdx.x == 0) {
@@ -331,19 +398,17 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
             bool ok = true;
             for (int t = first; t < p.tiles && ok; t += stride) {
                 const int m0 = t / p.num_n * BN + pair * S::kBRows;
-                for (int s = s0; s < s1; ++s) {
-                    if (!(ok = mbar_wait(&empty[st.at], st.phase ^ 1))) break;
-                    uint8_t* b = smem + st.at * S::kStageBytes + kABytes;
-                    if (CG == 1) {
-                        mbar_arrive_expect_tx(&full[st.at], P * S::kBPlane);
-                        for (int pl = 0; pl < P; ++pl)
-                            tma_load_2d(&map_a, &full[st.at], b + pl * S::kBPlane, s * kStepK, m0 + pl * p.m);
-                    } else {
-                        // Both CTAs' loads count on the first CTA's barrier, which expects them all.
-                        const uint32_t bar = cluster_addr(&full[st.at], 0);
-                        if (leader) mbar_arrive_expect_tx(&full[st.at], 2 * P * S::kBPlane);
-                        for (int pl = 0; pl < P; ++pl)
-                            tma_load_2d_pair(&map_a, bar, b + pl * S::kBPlane, s * kStepK, m0 + pl * p.m);
+                for (int c = c0; c < c1; ++c) {
+                    if (!(ok = wait_for(&empty[st.at], st.phase ^ 1))) break;
+                    uint8_t* b = smem + st.at * S::kStageBytes + 2 * kAHalf;
+                    // Both CTAs' loads of a pair count on the first CTA's barrier, which expects them all.
+                    const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], 0) : 0;
+                    if (leader) mbar_arrive_expect_tx(&full[st.at], CG * P * 2 * S::kBHalf);
+#pragma unroll
+                    for (int i = 0; i < 2 * P; ++i) {  // plane i / 2, inputs 64 (i % 2) ..
+                        const int x = c * 128 + (i % 2) * kHalfK, y = m0 + (i / 2) * p.m;
+                        if (CG == 1) tma_load_2d(&map_a, &full[st.at], b + i * S::kBHalf, x, y);
+                        else tma_load_2d_pair(&map_a, bar, b + i * S::kBHalf, x, y);
                     }
                     st.next();
                 }
@@ -351,71 +416,14 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
             if (!ok) gave_up(p, abort_flag);
         } else if (warp == 1 && leader) {
             // ---- products (the pair's first CTA issues for both) -----------------------------
-            if (elect_one()) {
-                constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-                Ring<S::kStages> st;
-                Ring<S::kBufs> acc;
-                const uint32_t peer_empty = CG == 2 ? cluster_addr(&empty[0], 1) : 0;
-                const uint32_t peer_acc_full = CG == 2 ? cluster_addr(&acc_full[0], 1) : 0;
-                const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + kABytes);
-                const auto product = [&](uint32_t d, int kk, bool start) {
-#pragma unroll
-                    for (int pl = 0; pl < P; ++pl) {
-                        const uint64_t off = static_cast<uint64_t>((st.at * S::kStageBytes + kk * 32) >> 4);
-                        const uint64_t da = a0 + off, db = b0 + off + static_cast<uint64_t>(pl * S::kBPlane >> 4);
-                        const uint32_t add = start && pl == 0 ? 0u : 1u;
-                        if (CG == 1) mma_f16(d, da, db, idesc, add);
-                        else mma_f16_pair(d, da, db, idesc, add);
-                    }
-                };
-                const auto commit_acc = [&] {
-                    if (CG == 1) {
-                        mma_commit(&acc_full[acc.at]);
-                    } else {
-                        mma_commit_pair(smem_u32(&acc_full[acc.at]));
-                        mma_commit_pair(peer_acc_full + static_cast<uint32_t>(acc.at * sizeof(uint64_t)));
-                    }
-                    acc.next();
-                };
-                bool ok = true;
-                for (int t = first; t < p.tiles && ok; t += stride) {
-                    for (int s = s0; s < s1 && ok; ++s) {
-                        if (!(ok = mbar_wait(&full[st.at], st.phase))) break;
-                        tc_fence_after();
-                        // A group is two steps (128 inputs), one, or half of one.
-                        if (per_chunk != 1 || s % 2 == 0) {
-                            if (!(ok = mbar_wait(&acc_empty[acc.at], acc.phase ^ 1))) break;
-                            tc_fence_after();
-                        }
-                        uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * BN);
-                        product(d, 0, per_chunk != 1 || s % 2 == 0);
-                        product(d, 1, false);
-                        if (per_chunk == 4) {
-                            commit_acc();
-                            if (s * kStepK + 32 < p.k) {
-                                if (!(ok = mbar_wait(&acc_empty[acc.at], acc.phase ^ 1))) break;
-                                tc_fence_after();
-                                d = tmem_base + static_cast<uint32_t>(acc.at * BN);
-                                product(d, 2, true);
-                                product(d, 3, false);
-                                commit_acc();
-                            }
-                        } else {
-                            product(d, 2, false);
-                            product(d, 3, false);
-                            if (per_chunk == 2 || s % 2 == 1 || s == s1 - 1) commit_acc();
-                        }
-                        if (CG == 1) {
-                            mma_commit(&empty[st.at]);
-                        } else {
-                            mma_commit_pair(smem_u32(&empty[st.at]));
-                            mma_commit_pair(peer_empty + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
-                        }
-                        st.next();
-                    }
-                }
-                if (!ok) gave_up(p, abort_flag);
-            }
+            const auto role = [&](auto per) {
+                return issue_role<BF16, P, BN, CG, decltype(per)::value>(p, smem, full, empty, acc_full, acc_empty, tmem_base,
+                                                                         first, stride, c0, c1);
+            };
+            const bool ok = per_chunk == 4   ? role(std::integral_constant<int, 4>())
+                            : per_chunk == 2 ? role(std::integral_constant<int, 2>())
+                                             : role(std::integral_constant<int, 1>());
+            if (!ok) gave_up(p, abort_flag);
         } else if (warp == 2 && lane == 0) {
             // ---- codes and zero points: contiguous per 128 outputs and chunk ------------------
             Ring<kCodeStages> cs;
@@ -425,7 +433,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                 // A pair's second CTA may have no outputs of its own: it repeats the last ones.
                 const int block = min(t % p.num_n * CG + pair, (p.n + 127) / 128 - 1);
                 for (int c = c0; c < c1; ++c) {
-                    if (!(ok = mbar_wait(&code_empty[cs.at], cs.phase ^ 1))) break;
+                    if (!(ok = wait_for(&code_empty[cs.at], cs.phase ^ 1))) break;
                     uint8_t* dst = code_ring + cs.at * kCodeStage;
                     const int64_t at = static_cast<int64_t>(block) * p.chunks + c;
                     mbar_arrive_expect_tx(&code_full[cs.at], kCodeBytes + zero_bytes);
@@ -489,7 +497,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
 #pragma unroll 1
                 for (int i = 0; i < left && i < 128; i += size, now >>= 16) {
                     const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(now & 0xffff)));
-                    ok = mbar_wait(&acc_full[ab.at], ab.phase);
+                    ok = wait_for(&acc_full[ab.at], ab.phase);
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
                         break;
@@ -498,15 +506,14 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                                            static_cast<uint32_t>(ab.at * BN + half * kCols);
                     const uint64_t d2 = pack_f2(make_float2(d, d));
-                    // 16 columns are added while the next 16 are on their way.
-                    uint32_t r[2][16];
-                    tmem_ld16(taddr, r[0]);
+                    // Two warps of a scheduler take turns: one's loads are under way while the other adds.
 #pragma unroll
-                    for (int q = 0; q < kCols / 16; ++q) {
+                    for (int q = 0; q < kCols / 32; ++q) {
+                        uint32_t r[32];
+                        tmem_ld32(taddr + q * 32, r);
                         tmem_ld_wait();
-                        if (q + 1 < kCols / 16) tmem_ld16(taddr + (q + 1) * 16, r[(q + 1) & 1]);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) fma2(acc[q * 8 + j], d2, r[q & 1][2 * j], r[q & 1][2 * j + 1]);
+                        for (int j = 0; j < 16; ++j) fma2(acc[q * 16 + j], d2, r[2 * j], r[2 * j + 1]);
                     }
                     if (c == c1 - 1 && i + size >= left) break;  // the tile's last accumulator is kept
                     release();
@@ -650,7 +657,7 @@ cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, in
     }
     CUtensorMap map;
     if (!encode_map_2d(&map, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a,
-                       static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m) * P, static_cast<uint64_t>(lda) * 2, kStepK,
+                       static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m) * P, static_cast<uint64_t>(lda) * 2, kHalfK,
                        S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     p.num_n = (p.n + CG * 128 - 1) / (CG * 128);
