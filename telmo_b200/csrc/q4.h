@@ -57,12 +57,27 @@ struct Q4Args {
 cudaError_t q4_repack(const uint8_t* codes, const float* scales, const uint8_t* zeros, const Q4Weights& w,
                       cudaStream_t stream);
 
-// The product for few rows: every warp multiplies 16 or 32 outputs by up to 32 rows.
-cudaError_t q4_linear_rows(const Q4Args& g, cudaStream_t stream);
+// The activations as the kernels for more rows read them where they cannot read the caller's: f32 as
+// two fp16 planes (rows 0..m-1 hi, m..2m-1 lo, both times row_scale[r], a power of two), 16-bit
+// values copied to rows that start on 16-byte boundaries (row_scale null).
+struct Q4Planes {
+    const void* a = nullptr;
+    int64_t ld = 0;
+    const float* row_scale = nullptr;
+};
 
-// The product for many rows on tcgen05 tiles, and the bytes of workspace (16-byte aligned) it needs
-// for activations that it cannot read where they are: f32, or rows off 16-byte boundaries.
-size_t q4_gemm_workspace(const Q4Args& g);
-cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream);
+inline bool q4_rows_aligned(const Q4Args& g) {
+    return reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda * (g.a_type == kQ4F32 ? 4 : 2) % 16 == 0;
+}
+
+// Whether the product wants Q4Planes, their bytes, and their making.
+bool q4_rows_planes(const Q4Args& g);  // up to 32 rows
+inline bool q4_gemm_planes(const Q4Args& g) { return g.a_type == kQ4F32 || !q4_rows_aligned(g); }
+size_t q4_planes_bytes(const Q4Args& g);
+cudaError_t q4_make_planes(const Q4Args& g, void* workspace, Q4Planes* planes, cudaStream_t stream);
+
+// The product for up to 32 rows, and for any number of rows on tcgen05 tiles. `planes`: null where not wanted.
+cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream);
+cudaError_t q4_linear_gemm(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream);
 
 }  // namespace telmo

@@ -125,9 +125,12 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     g.ldc = static_cast<int64_t>(ldc);
     g.sms = ctx->sms;
     g.error = ctx->error_word;
-    if (m <= 32) return ctx->cuda(q4_linear_rows(g, stream), "telmo_linear_q4");
-    const size_t bytes = q4_gemm_workspace(g);
-    if (bytes == 0) return ctx->cuda(q4_linear_gemm(g, nullptr, stream), "telmo_linear_q4");
+    // Up to 32 rows stay on the row kernels; see q4_rows.cu and q4_gemm.cu for both sides' times.
+    const bool rows = m <= 32;
+    const auto product = [&](const Q4Planes* planes) {
+        return rows ? q4_linear_rows(g, planes, stream) : q4_linear_gemm(g, planes, stream);
+    };
+    if (!(rows ? q4_rows_planes(g) : q4_gemm_planes(g))) return ctx->cuda(product(nullptr), "telmo_linear_q4");
     // Workspace in stream order from the context's own pool: calls on several streams and captured
     // graphs each have their own, and a graph keeps its own while it lives.
     if (!ctx->pool) {
@@ -140,8 +143,12 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
         cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
     }
     void* ws = nullptr;
-    if (int rc = ctx->cuda(cudaMallocFromPoolAsync(&ws, bytes, ctx->pool, stream), "telmo_linear_q4: workspace")) return rc;
-    const cudaError_t e = q4_linear_gemm(g, ws, stream);
+    if (int rc = ctx->cuda(cudaMallocFromPoolAsync(&ws, q4_planes_bytes(g), ctx->pool, stream),
+                           "telmo_linear_q4: workspace"))
+        return rc;
+    Q4Planes planes;
+    cudaError_t e = q4_make_planes(g, ws, &planes, stream);
+    if (e == cudaSuccess) e = product(&planes);
     const cudaError_t f = cudaFreeAsync(ws, stream);
     return ctx->cuda(e != cudaSuccess ? e : f, "telmo_linear_q4");
 }

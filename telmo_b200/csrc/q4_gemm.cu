@@ -506,17 +506,19 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                                            static_cast<uint32_t>(ab.at * BN + half * kCols);
                     const uint64_t d2 = pack_f2(make_float2(d, d));
-                    // Two warps of a scheduler take turns: one's loads are under way while the other adds.
+                    // Two warps of a scheduler take turns: one's loads are under way while the other adds. The
+                    // accumulator is released with its last columns' additions still to come (prompt of
+                    // 4096 rows, 4096 -> 8192: 257 us with the release after them, 230 before).
+                    const bool last = c == c1 - 1 && i + size >= left;  // the tile's last accumulator is kept
 #pragma unroll
                     for (int q = 0; q < kCols / 32; ++q) {
                         uint32_t r[32];
                         tmem_ld32(taddr + q * 32, r);
                         tmem_ld_wait();
+                        if (q == kCols / 32 - 1 && !last) release();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) fma2(acc[q * 16 + j], d2, r[2 * j], r[2 * j + 1]);
                     }
-                    if (c == c1 - 1 && i + size >= left) break;  // the tile's last accumulator is kept
-                    release();
                 }
             }
             if (!ok) {
@@ -700,15 +702,31 @@ size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace
 
-size_t q4_gemm_workspace(const Q4Args& g) {
+size_t q4_planes_bytes(const Q4Args& g) {
     const size_t m = static_cast<size_t>(g.m), ld = round_up(static_cast<size_t>(g.w->k), 8);
-    if (g.a_type == kQ4F32) return round_up(2 * m * ld * sizeof(__half), 256) + round_up(m, 256) * sizeof(float);
-    const bool aligned = reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda % 8 == 0;
-    return aligned ? 0 : m * ld * 2;
+    if (g.a_type != kQ4F32) return m * ld * 2;
+    return round_up(2 * m * ld * sizeof(__half), 256) + round_up(m, 256) * sizeof(float);
 }
 
-cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream) {
-    GemmParams p;
+cudaError_t q4_make_planes(const Q4Args& g, void* workspace, Q4Planes* planes, cudaStream_t stream) {
+    const int64_t ld = static_cast<int64_t>(round_up(static_cast<size_t>(g.w->k), 8));
+    planes->a = workspace;
+    planes->ld = ld;
+    if (g.a_type == kQ4F32) {
+        float* rs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                             round_up(2 * static_cast<size_t>(g.m) * ld * sizeof(__half), 256));
+        planes->row_scale = rs;
+        q4_split_kernel<<<g.m, kPrepThreads, 0, stream>>>(static_cast<const float*>(g.a), g.lda, g.m, g.w->k,
+                                                          static_cast<__half*>(workspace), ld, rs);
+    } else {
+        q4_align_kernel<<<g.m, kPrepThreads, 0, stream>>>(static_cast<const uint16_t*>(g.a), g.lda, g.w->k,
+                                                          static_cast<uint16_t*>(workspace), ld);
+    }
+    return cudaGetLastError();
+}
+
+cudaError_t q4_linear_gemm(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream) {
+    GemmParams p = {};
     p.codes = g.w->codes;
     p.scales = g.w->scales;
     p.zeros = g.w->zeros;
@@ -716,9 +734,8 @@ cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream
     p.k = g.w->k;
     p.chunks = g.w->chunks;
     p.per_chunk = 128 / g.w->group;
-    p.tiles = p.num_n = p.splits = p.split_chunks = 0;
     p.m = g.m;
-    p.row_scale = nullptr;
+    p.row_scale = planes ? planes->row_scale : nullptr;
     p.bias = g.bias;
     p.act = g.act;
     p.scale = g.scale;
@@ -727,25 +744,9 @@ cudaError_t q4_linear_gemm(const Q4Args& g, void* workspace, cudaStream_t stream
     p.c_type = g.c_type;
     p.ldc = g.ldc;
     p.error = g.error;
-    const int64_t ld = static_cast<int64_t>(round_up(static_cast<size_t>(p.k), 8));
-    if (g.a_type == kQ4F32) {
-        __half* planes = static_cast<__half*>(workspace);
-        float* rs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                             round_up(2 * static_cast<size_t>(p.m) * ld * sizeof(__half), 256));
-        q4_split_kernel<<<p.m, kPrepThreads, 0, stream>>>(static_cast<const float*>(g.a), g.lda, p.m, p.k, planes, ld, rs);
-        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-        p.row_scale = rs;
-        return launch_shape<false, 2>(planes, ld, p, g.sms, stream);
-    }
-    const void* a = g.a;
-    int64_t lda = g.lda;
-    if (workspace) {
-        q4_align_kernel<<<p.m, kPrepThreads, 0, stream>>>(static_cast<const uint16_t*>(g.a), g.lda, p.k,
-                                                          static_cast<uint16_t*>(workspace), ld);
-        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-        a = workspace;
-        lda = ld;
-    }
+    const void* a = planes ? planes->a : g.a;
+    const int64_t lda = planes ? planes->ld : g.lda;
+    if (g.a_type == kQ4F32) return launch_shape<false, 2>(a, lda, p, g.sms, stream);
     return g.a_type == kQ4BF16 ? launch_shape<true, 1>(a, lda, p, g.sms, stream)
                                : launch_shape<false, 1>(a, lda, p, g.sms, stream);
 }
