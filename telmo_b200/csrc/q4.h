@@ -14,7 +14,8 @@ namespace telmo {
 // Codes are stored in tiles of 8 outputs by 128 inputs (a chunk), 512 bytes each; the 16 tiles of
 // 128 outputs and one chunk lie together (8 KB, one bulk copy), chunk after chunk. Lane l = 4 g + t
 // of a warp owns bytes 16 l .. 16 l + 15 of a tile: four 32-bit words of output row g, word w holding
-// inputs 32 w + 8 t + 0..7 of the chunk (input 2 p in nibble p, input 2 p + 1 in nibble p + 4). So a
+// inputs 32 w + 8 t + 0..7 of the chunk (input 2 p in nibble p, input 2 p + 1 in nibble p + 4), each code with
+// its top bit flipped (code - 8 in two's complement). So a
 // tile is one coalesced 16-byte load per lane; (word >> 4 p) & 0x000f000f leaves two neighbouring
 // inputs in the two halves of a register; and one word of the four lanes of a row spans 32 inputs, the
 // smallest group, so a 16-input matrix instruction never mixes two groups. Scales and zero points lie
@@ -75,6 +76,11 @@ bool q4_rows_planes(const Q4Args& g);  // up to 32 rows
 inline bool q4_gemm_planes(const Q4Args& g) { return g.a_type == kQ4F32 || !q4_rows_aligned(g); }
 size_t q4_planes_bytes(const Q4Args& g);
 cudaError_t q4_make_planes(const Q4Args& g, void* workspace, Q4Planes* planes, cudaStream_t stream);
+
+// The product for one or two rows whose digits fit shared memory (kQ4VecSmem bytes at most).
+constexpr size_t kQ4VecSmem = 222 << 10;
+bool q4_vec_fits(const Q4Args& g);
+cudaError_t q4_linear_vec(const Q4Args& g, cudaStream_t stream);
 
 // The product for up to 32 rows, and for any number of rows on tcgen05 tiles. `planes`: null where not wanted.
 cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream);

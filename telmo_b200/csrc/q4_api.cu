@@ -125,6 +125,7 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     g.ldc = static_cast<int64_t>(ldc);
     g.sms = ctx->sms;
     g.error = ctx->error_word;
+    if (q4_vec_fits(g)) return ctx->cuda(q4_linear_vec(g, stream), "telmo_linear_q4");
     // Up to 32 rows stay on the row kernels; see q4_rows.cu and q4_gemm.cu for both sides' times.
     const bool rows = m <= 32;
     const auto product = [&](const Q4Planes* planes) {

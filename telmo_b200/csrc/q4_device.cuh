@@ -17,7 +17,8 @@ __device__ __forceinline__ uint32_t code_base(uint32_t zero) {
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t base) {
-    const uint32_t v = ((word >> (4 * p)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+    // Codes are stored with their top bit flipped, which the exclusive or undoes.
+    const uint32_t v = ((word >> (4 * p)) & 0x000f000fu) ^ (BF16 ? 0x43084308u : 0x64086408u);
     if (BF16) {
         const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
                                          *reinterpret_cast<const __nv_bfloat162*>(&base));
@@ -28,7 +29,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t bas
 }
 
 __device__ __forceinline__ float q4_act(float v, int act) {
-    if (act == kActRelu) return fmaxf(v, 0.0f);
+    if (act == kActRelu) return v < 0.0f ? 0.0f : v;  // a NaN stays one
     if (act == kActSilu) return mul_sigmoid(v, v);
     return v;
 }

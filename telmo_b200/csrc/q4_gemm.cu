@@ -200,7 +200,7 @@ __device__ __forceinline__ void finish_rows(const GemmParams& p, const uint32_t 
     for (int j = 0; j < 16; ++j) v[j] += bias;
     if (p.act == kActRelu) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = fmaxf(v[j], 0.0f);
+        for (int j = 0; j < 16; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
     } else if (p.act == kActSilu) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = mul_sigmoid(v[j], v[j]);

@@ -26,7 +26,7 @@ __global__ void q4_repack_kernel(const uint8_t* codes, const float* scales, cons
             const uint8_t b = codes[o * row_bytes + (i0 + j) / 2];
             q = ((i0 + j) & 1) ? b >> 4 : b & 15;
         }
-        v |= q << (4 * (j / 2 + 4 * (j & 1)));
+        v |= (q ^ 8) << (4 * (j / 2 + 4 * (j & 1)));
     }
     reinterpret_cast<uint32_t*>(w.codes)[word] = v;
     // The first of a tile's threads write its scales and zero points.
@@ -58,13 +58,15 @@ namespace {
 
 template <int MODE>
 cudaError_t by_height(const RowsParams& p, int group, int r, cudaStream_t stream) {
-    return r == 2 ? launch_group<MODE, 2, 1>(p, group, stream) : launch_group<MODE, 1, 1>(p, group, stream);
+    return by_group(p, group, [&](auto groups, auto zeros) {
+        return r == 2 ? launch_direct<MODE, decltype(groups)::value, decltype(zeros)::value, 2>(p, stream)
+                      : launch_direct<MODE, decltype(groups)::value, decltype(zeros)::value, 1>(p, stream);
+    });
 }
 
 }  // namespace
 
 cudaError_t launch_small(const RowsParams& p, int mode, int group, int r, cudaStream_t stream) {
-    if (mode == kModeF32Packed) return by_height<kModeF32Packed>(p, group, r, stream);
     if (mode == kModeF32) return by_height<kModeF32>(p, group, r, stream);
     if (mode == kModeBF16) return by_height<kModeBF16>(p, group, r, stream);
     return by_height<kModeF16>(p, group, r, stream);
@@ -95,22 +97,22 @@ cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t
     p.c = g.c;
     p.c_type = g.c_type;
     p.ldc = g.ldc;
-    p.row_warps = 1;
     p.splits = 1;
     const int mode = g.a_type == kQ4BF16 ? kModeBF16 : g.a_type == kQ4F16 ? kModeF16 : kModeF32;
-    if (g.m <= 8) {
+    if (!p.vec || mode == kModeF32 ? g.m <= 8 : g.m <= 8 && p.chunks <= kWarps) {
         // Two 16-output slabs a warp share the activations' operands; one where that leaves SMs without work.
         const int r = (p.n + 31) / 32 >= 2 * g.sms ? 2 : 1;
         p.split_chunks = p.chunks;
-        return launch_small(p, mode == kModeF32 && g.m <= 2 ? kModeF32Packed : mode, g.w->group, r, stream);
+        return launch_small(p, mode, g.w->group, r, stream);
     }
-    // Four warps side by side read the same activations, 128 outputs a block; the chunks are split
-    // over clusters until there are two blocks per SM or a warp has two chunks left.
-    p.row_warps = 4;
-    const int blocks = (p.n + 127) / 128;
-    while (p.splits < 8 && blocks * p.splits < 2 * g.sms && p.chunks >= 8 * p.splits) p.splits *= 2;
+    // Warps side by side read the same activations; the chunks are split over clusters as long as the
+    // blocks all run at once and a share keeps two chunks.
+    const int row_warps = g.m <= 8 ? 2 : 4, shares = kWarps / row_warps;
+    const int blocks = (p.n + 32 * row_warps - 1) / (32 * row_warps);
+    const int resident = (g.m <= (mode == kModeF32 ? 8 : 16) ? 2 : 1) * g.sms;
+    while (p.splits < 8 && blocks * p.splits * 2 <= resident && p.chunks >= 4 * shares * p.splits) p.splits *= 2;
     p.split_chunks = (p.chunks + p.splits - 1) / p.splits;
-    return launch_mid(p, mode == kModeF32 ? kModePlanes : mode, g.w->group, stream);
+    return launch_aligned(p, mode == kModeF32 ? kModePlanes : mode, g.w->group, stream);
 }
 
 }  // namespace telmo

@@ -15,31 +15,32 @@
 //
 // Activations: bf16 and fp16 are operands as they are. An f32 activation becomes three bf16
 // parts of 8 significant bits by truncation, x = hi + mid + lo, which is exact (24 bits; parts
-// below 2^-126 vanish), and three products are summed: in three instructions, or for one and two
-// rows in one, the parts in columns of their own. More than eight f32 rows come as two fp16 planes
+// below 2^-126 vanish), and three products are summed. More than eight f32 rows come as two fp16 planes
 // (q4_split) and a power of two per row s_r, two instructions.
 //
-// A warp takes 16 R outputs and a share of the 128-input chunks, with the codes of its next chunk
-// under way while it works on one. Warps that share outputs add up in shared memory, in order.
+// A warp takes 16 R outputs and a share of the 128-input chunks, with its next chunks under way while
+// it works on one: in registers (q4_rows_kernel, rows of any alignment and f32), or in a ring in
+// shared memory together with the activations (q4_rows_staged_kernel). Warps that share outputs add up in shared memory, in order.
 // Where n gives too few blocks, the blocks of a cluster take a share of the chunks each and add up
 // through distributed shared memory, in rank order.
 #pragma once
 
 #include "ptx.cuh"
+#include "q4_async.cuh"
 #include "q4_device.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace telmo {
 
 namespace q4rows {
 
 enum RowsMode : int {
-    kModeF16 = 0,        // fp16 activations
-    kModeBF16 = 1,       // bf16 activations
-    kModeF32 = 2,        // f32 activations, three instructions
-    kModeF32Packed = 3,  // f32 activations of one or two rows: part p of row r in column 2 p + r
-    kModePlanes = 4,     // two fp16 planes, two instructions
+    kModeF16 = 0,     // fp16 activations
+    kModeBF16 = 1,    // bf16 activations
+    kModeF32 = 2,     // f32 activations, three instructions
+    kModePlanes = 3,  // two fp16 planes, two instructions
 };
 
 constexpr int kWarps = 8;
@@ -61,7 +62,6 @@ struct RowsParams {
     void* c;
     int c_type;
     int64_t ldc;
-    int row_warps;  // warps side by side on outputs; kWarps / row_warps share the chunks
     int splits;     // blocks of a cluster that share the chunks
     int split_chunks;
 };
@@ -131,9 +131,10 @@ __device__ __forceinline__ void split_parts(const float (&x)[N], uint32_t (&hi)[
     }
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -171,24 +172,116 @@ __device__ __forceinline__ void load_chunk(Chunk<GROUPS, ZEROS, R>& x, const uin
     }
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) {
-    return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w;
+// The loops over a chunk's four words stay rolled: unrolled, a warp runs through several KB of code a
+// few times only, and fetching it took longer than running it (32 rows, 4096 -> 8192: 36 us unrolled).
+// So scales and zero points are taken from the low end of their registers and shifted down.
+template <int GROUPS>
+__device__ __forceinline__ float next_scale(uint32_t (&d)[GROUPS == 4 ? 2 : 1]) {
+    const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(d[0] & 0xffffu)));
+    if (GROUPS == 4) {
+        d[0] = __funnelshift_r(d[0], d[GROUPS == 4 ? 1 : 0], 16);
+        d[GROUPS == 4 ? 1 : 0] >>= 16;
+    } else if (GROUPS == 2) {
+        d[0] >>= 16;
+    }
+    return v;
 }
 
-template <int MODE, int GROUPS, bool ZEROS, int R, int CB>
+// part times the group's scales onto acc, and part to zero.
+template <int GROUPS, int R, int CB>
+__device__ __forceinline__ void add_group(float (&acc)[R][CB][4], float (&part)[R][CB][4],
+                                          uint32_t (&d)[2 * R][GROUPS == 4 ? 2 : 1]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float d0 = next_scale<GROUPS>(d[2 * r]), d1 = next_scale<GROUPS>(d[2 * r + 1]);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            acc[r][cb][0] = fmaf(d0, part[r][cb][0], acc[r][cb][0]);
+            acc[r][cb][1] = fmaf(d0, part[r][cb][1], acc[r][cb][1]);
+            acc[r][cb][2] = fmaf(d1, part[r][cb][2], acc[r][cb][2]);
+            acc[r][cb][3] = fmaf(d1, part[r][cb][3], acc[r][cb][3]);
+            part[r][cb][0] = part[r][cb][1] = part[r][cb][2] = part[r][cb][3] = 0.0f;
+        }
+    }
+}
+
+// Two output rows' words as the A operands of two instructions.
+template <bool BF16>
+__device__ __forceinline__ void operands(uint32_t x0, uint32_t x1, uint32_t z0, uint32_t z1, uint32_t (&a)[2][4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        a[h][0] = code_pair<BF16>(x0, 2 * h, z0);
+        a[h][1] = code_pair<BF16>(x1, 2 * h, z1);
+        a[h][2] = code_pair<BF16>(x0, 2 * h + 1, z0);
+        a[h][3] = code_pair<BF16>(x1, 2 * h + 1, z1);
+    }
+}
+
+// The sums of a block's shares, and of a cluster's blocks, and the epilogue, four outputs a thread at a
+// time. `sums`: [share][column][output of the block] in shared memory, written and synchronised.
+template <bool SCALED, int SHARES, int OUTS, int COLS>
+__device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, int64_t out0, int m0, int split) {
+    constexpr int kAll = OUTS * COLS / 4;
+    float4* s4 = reinterpret_cast<float4*>(sums);
+    const auto add = [](float4& a, const float4& b) {
+        a.x += b.x;
+        a.y += b.y;
+        a.z += b.z;
+        a.w += b.w;
+    };
+    const auto finish = [&](int e, const float4& s) {
+        const int row = m0 + e / (OUTS / 4);
+        if (row >= p.m) return;
+        const float rs = SCALED ? __ldg(p.row_scale + row) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t out = out0 + e % (OUTS / 4) * 4 + j;
+            if (out >= p.n) return;
+            float v = (j == 0 ? s.x : j == 1 ? s.y : j == 2 ? s.z : s.w) * rs;
+            if (p.bias) v += __ldg(p.bias + out);
+            v = q4_act(v, p.act) * p.scale;
+            const int64_t at = static_cast<int64_t>(row) * p.ldc + out;
+            if (p.accumulate) v += q4_load(p.c, p.c_type, at);
+            q4_store(p.c, p.c_type, at, v);
+        }
+    };
+    for (int e = threadIdx.x; e < kAll; e += 32 * kWarps) {
+        float4 v = s4[e];
+#pragma unroll
+        for (int s = 1; s < SHARES; ++s) add(v, s4[s * kAll + e]);
+        if (p.splits == 1) finish(e, v);
+        else s4[e] = v;  // into the first share's place
+    }
+    if (p.splits == 1) return;
+    __syncwarp();
+    cluster_sync();
+    // Each block of the cluster finishes a part of the outputs. All blocks' sums are asked for at once.
+    for (int e = split * 32 * kWarps + threadIdx.x; e < kAll; e += p.splits * 32 * kWarps) {
+        float4 v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s < p.splits) v[s] = ld_cluster_v4(cluster_addr(s4 + e, static_cast<uint32_t>(s)));
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+            if (s < p.splits) add(v[0], v[s]);
+        finish(e, v[0]);
+    }
+    __syncwarp();
+    cluster_sync();  // the other blocks have read this one's sums
+}
+
+template <int MODE, int GROUPS, bool ZEROS, int R>
 __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p) {
-    constexpr bool BF16 = MODE != kModeF16 && MODE != kModePlanes;
-    constexpr bool kPacked = MODE == kModeF32Packed;
-    constexpr int kParts = MODE == kModeF32 ? 3 : MODE == kModePlanes ? 2 : 1;
+    constexpr bool BF16 = MODE != kModeF16;
+    constexpr int CB = 1;
+    constexpr int kParts = MODE == kModeF32 ? 3 : 1;
     constexpr int kWordsPerGroup = 4 / GROUPS;
-    constexpr int kCols = kPacked ? 2 : 8 * CB;  // activation rows of the block
-    constexpr int kPackedRow = 128 + 32;         // a part's 128 values, and what keeps rows off each other's banks
-    __shared__ float sums[kWarps * 16 * R * kCols];
-    __shared__ __align__(16) uint16_t packed[kPacked ? kWarps * 6 * kPackedRow : 8];
+    constexpr int kCols = 8;  // activation rows of the block
+    __shared__ __align__(16) float sums[kWarps * 16 * R * kCols];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int g = lane >> 2, t = lane & 3;
-    const int row_warps = p.row_warps, shares = kWarps / row_warps;
-    const int rw = warp % row_warps, share = warp / row_warps;
+    constexpr int row_warps = 1, shares = kWarps, rw = 0;
+    const int share = warp;
     const int split = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int block = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x;
     const int m0 = blockIdx.y * kCols;
@@ -197,7 +290,7 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
     const int c_end = min(p.chunks, (split + 1) * p.split_chunks);
     int c = split * p.split_chunks + share;
 
-    float acc[R][CB][4] = {};
+    float acc[R][CB][4] = {}, part[R][CB][4] = {};
     // Tiles past the last 128 outputs do not exist: such a warp has nothing to do.
     if (tile0 * 8 < p.n && c < c_end) {
         const int64_t first = q4_tile(tile0, p.chunks, c);
@@ -213,103 +306,47 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
             if (ZEROS) zeros += shares * (16 * 8 * GROUPS);
             if (c + shares < c_end) load_chunk(next, codes, scales, zeros);
 
-            if (kPacked) {
-                // Each lane splits four inputs of each row; lane (g, t) then reads row g % 2 of part g / 2.
-                uint16_t* mine = packed + warp * 6 * kPackedRow;
-                __syncwarp();
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x[4];
-                    const int i = c * 128 + lane * 4;
-                    load_a32<4>(static_cast<const float*>(p.a) + (m0 + r) * p.lda + i, m0 + r < p.m, p.vec, p.k - i, x);
-                    uint32_t parts[3][2];
-                    split_parts<4>(x, parts[0], parts[1], parts[2]);
-#pragma unroll
-                    for (int pl = 0; pl < 3; ++pl)
-                        *reinterpret_cast<uint2*>(mine + (pl * 2 + r) * kPackedRow + lane * 4) =
-                            make_uint2(parts[pl][0], parts[pl][1]);
-                }
-                __syncwarp();
-            }
-#pragma unroll
-            for (int q = 0; q < GROUPS; ++q) {
-                float part[R][CB][4] = {};
-#pragma unroll
-                for (int ww = 0; ww < kWordsPerGroup; ++ww) {
-                    const int w = q * kWordsPerGroup + ww;
-                    const int i = c * 128 + 32 * w + 8 * t;
-                    uint32_t b[kParts][CB][4];
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        const int row = m0 + 8 * cb + g;
-                        if (MODE == kModeF32) {
-                            float x[8];
-                            load_a32<8>(static_cast<const float*>(p.a) + row * p.lda + i, row < p.m, p.vec, p.k - i, x);
-                            split_parts<8>(x, b[0][cb], b[kParts > 1 ? 1 : 0][cb], b[kParts > 2 ? 2 : 0][cb]);
-                        } else if (kPacked) {
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (g < 6)
-                                v = *reinterpret_cast<const uint4*>(packed + (warp * 6 + g) * kPackedRow + 32 * w + 8 * t);
-                            b[0][cb][0] = v.x; b[0][cb][1] = v.y; b[0][cb][2] = v.z; b[0][cb][3] = v.w;
-                        } else {
-#pragma unroll
-                            for (int pl = 0; pl < kParts; ++pl) {
-                                const uint4 v = load_a16(static_cast<const uint16_t*>(p.a) +
-                                                             (row + static_cast<int64_t>(pl) * p.m) * p.lda + i,
-                                                         row < p.m, p.vec, p.k - i);
-                                b[pl][cb][0] = v.x; b[pl][cb][1] = v.y; b[pl][cb][2] = v.z; b[pl][cb][3] = v.w;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const uint32_t x0 = word_of(now.words[2 * r], w), x1 = word_of(now.words[2 * r + 1], w);
-                        const uint32_t z0 = code_base<BF16>(ZEROS ? (now.z[2 * r] >> (8 * q)) & 0xffu : 8u);
-                        const uint32_t z1 = code_base<BF16>(ZEROS ? (now.z[2 * r + 1] >> (8 * q)) & 0xffu : 8u);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t a[4] = {code_pair<BF16>(x0, 2 * h, z0), code_pair<BF16>(x1, 2 * h, z1),
-                                                   code_pair<BF16>(x0, 2 * h + 1, z0), code_pair<BF16>(x1, 2 * h + 1, z1)};
-#pragma unroll
-                            for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-                                for (int pl = 0; pl < kParts; ++pl)
-                                    mma_16816<BF16>(part[r][cb], a, b[pl][cb][2 * h], b[pl][cb][2 * h + 1]);
-                        }
-                    }
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+                const int i = c * 128 + 32 * w + 8 * t;
+                const int row = m0 + g;
+                uint32_t b[kParts][4];
+                if (MODE == kModeF32) {
+                    float x[8];
+                    load_a32<8>(static_cast<const float*>(p.a) + row * p.lda + i, row < p.m, p.vec, p.k - i, x);
+                    split_parts<8>(x, b[0], b[kParts > 1 ? 1 : 0], b[kParts > 2 ? 2 : 0]);
+                } else {
+                    const uint4 v = load_a16(static_cast<const uint16_t*>(p.a) + row * p.lda + i, row < p.m, p.vec, p.k - i);
+                    b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const auto scale_of = [&](int row) {
-                        const uint32_t pair = now.d[row][GROUPS == 4 ? q / 2 : 0];
-                        return __half2float(__ushort_as_half(static_cast<unsigned short>(q % 2 ? pair >> 16 : pair & 0xffff)));
-                    };
-                    const float d0 = scale_of(2 * r), d1 = scale_of(2 * r + 1);
+                    uint32_t a[2][4];
+                    operands<BF16>(now.words[2 * r].x, now.words[2 * r + 1].x, code_base<BF16>(ZEROS ? now.z[2 * r] & 0xffu : 8u),
+                                   code_base<BF16>(ZEROS ? now.z[2 * r + 1] & 0xffu : 8u), a);
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        acc[r][cb][0] = fmaf(d0, part[r][cb][0], acc[r][cb][0]);
-                        acc[r][cb][1] = fmaf(d0, part[r][cb][1], acc[r][cb][1]);
-                        acc[r][cb][2] = fmaf(d1, part[r][cb][2], acc[r][cb][2]);
-                        acc[r][cb][3] = fmaf(d1, part[r][cb][3], acc[r][cb][3]);
-                    }
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int pl = 0; pl < kParts; ++pl)
+                            mma_16816<BF16>(part[r][0], a[h], b[pl][2 * h], b[pl][2 * h + 1]);
+                }
+#pragma unroll
+                for (int r = 0; r < 2 * R; ++r) {
+                    now.words[r].x = now.words[r].y;
+                    now.words[r].y = now.words[r].z;
+                    now.words[r].z = now.words[r].w;
+                }
+                if ((w + 1) % kWordsPerGroup == 0) {
+                    add_group<GROUPS, R, CB>(acc, part, now.d);
+                    if (ZEROS)
+#pragma unroll
+                        for (int r = 0; r < 2 * R; ++r) now.z[r] >>= 8;
                 }
             }
             now = next;
         }
     }
 
-    if (kPacked) {
-        // Columns 2 p and 2 p + 1 hold part p of the two rows; 6 and 7 hold zeros.
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v = acc[r][0][j];
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                acc[r][0][j] = v;
-            }
-    }
     // sums[share][column][output of the block]
     const int outs = 16 * R * row_warps;
 #pragma unroll
@@ -319,54 +356,171 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int col = 8 * cb + 2 * t + (j & 1);
-                if (!kPacked || t == 0)
-                    sums[(share * kCols + col) * outs + rw * 16 * R + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
+                sums[(share * kCols + col) * outs + rw * 16 * R + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
             }
     __syncthreads();
-    const int all = outs * kCols;
-    const auto finish = [&](int e, float v) {
-        const int64_t out = out0 + e % outs;
-        const int row = m0 + e / outs;
-        if (out >= p.n || row >= p.m) return;
-        if (MODE == kModePlanes) v *= __ldg(p.row_scale + row);
-        if (p.bias) v += __ldg(p.bias + out);
-        v = q4_act(v, p.act) * p.scale;
-        const int64_t at = static_cast<int64_t>(row) * p.ldc + out;
-        if (p.accumulate) v += q4_load(p.c, p.c_type, at);
-        q4_store(p.c, p.c_type, at, v);
-    };
-    if (p.splits == 1) {
-        for (int e = threadIdx.x; e < all; e += 32 * kWarps) {
-            float v = 0.0f;
-            for (int s = 0; s < shares; ++s) v += sums[s * all + e];
-            finish(e, v);
-        }
-        return;
-    }
-    // The block's own sums into its first share's place, then each block finishes a part of the outputs.
-    for (int e = threadIdx.x; e < all; e += 32 * kWarps) {
-        float v = 0.0f;
-        for (int s = 0; s < shares; ++s) v += sums[s * all + e];
-        sums[e] = v;
-    }
-    __syncwarp();
-    cluster_sync();
-    for (int e = split * 32 * kWarps + threadIdx.x; e < all; e += p.splits * 32 * kWarps) {
-        float v = 0.0f;
-        for (int s = 0; s < p.splits; ++s) v += ld_cluster_f32(cluster_addr(sums + e, static_cast<uint32_t>(s)));
-        finish(e, v);
-    }
-    __syncwarp();
-    cluster_sync();  // the other blocks have read this one's sums
+    finish_block<false, kWarps, 16 * R, kCols>(p, sums, out0, m0, split);
 }
 
+// Rows that start on 16-byte boundaries (16-bit activations, or planes): activations and codes come
+// through a ring of chunks in shared memory (cp.async), filled by the warps of a share together.
+// The rows' pitch of 320 bytes puts the two rows of an 8-lane phase on different banks.
+constexpr int kRing = 3;
+constexpr int kPitch = 320;
+
+template <int MODE, int R, int CB>
+struct Staged {
+    static constexpr int kParts = MODE == kModePlanes ? 2 : 1;
+    static constexpr int kActBytes = kParts * 8 * CB * kPitch;
+    static constexpr int kCodeBytes = 2 * R * 512;  // of one warp
+    // Warps side by side on outputs: they share the activations; the others share the chunks.
+    static constexpr int kRowWarps = CB == 1 ? 2 : 4;
+    static constexpr int kShares = kWarps / kRowWarps;
+    static constexpr int kStageBytes = kActBytes + kRowWarps * kCodeBytes;
+    static constexpr int kSmem = std::max(kShares * kRing * kStageBytes, kWarps * 16 * R * 8 * CB * 4);
+    static constexpr int kBlocks = CB * kParts <= 2 ? 2 : 1;  // per SM, which bounds the registers
+};
+
 template <int MODE, int GROUPS, bool ZEROS, int R, int CB>
-cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
-    constexpr int kCols = MODE == kModeF32Packed ? 2 : 8 * CB;
-    const int outs = 16 * R * p.row_warps;
+__global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_rows_staged_kernel(const RowsParams p) {
+    using S = Staged<MODE, R, CB>;
+    constexpr bool BF16 = MODE == kModeBF16;
+    constexpr int kParts = S::kParts, kWordsPerGroup = 4 / GROUPS, kCols = 8 * CB;
+    extern __shared__ __align__(128) uint8_t ring[];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int row_warps = S::kRowWarps, shares = S::kShares;
+    const int rw = warp % row_warps, share = warp / row_warps;
+    const int split = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int block = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x;
+    const int64_t out0 = static_cast<int64_t>(block) * (16 * R * row_warps);
+    const int64_t tile0 = out0 / 8 + rw * 2 * R;
+    const bool live = tile0 * 8 < p.n;  // tiles past the last 128 outputs do not exist
+    const int c_end = min(p.chunks, (split + 1) * p.split_chunks);
+    const int c0 = split * p.split_chunks + share;
+
+    constexpr int stage_bytes = S::kStageBytes;
+    const uint32_t mine = smem_u32(ring) + static_cast<uint32_t>(share * kRing * stage_bytes);
+    const int64_t first = q4_tile(live ? tile0 : 0, p.chunks, 0);
+    const uint4* codes = p.codes + first * 32 + lane;
+    const uint8_t* scales = reinterpret_cast<const uint8_t*>(p.scales) + (first * 8 + g) * GROUPS * 2;
+    const uint8_t* zeros = ZEROS ? p.zeros + (first * 8 + g) * GROUPS : nullptr;
+
+    // Starts the copies of chunk c into a ring place: 16 pieces of 16 bytes to each row of activations.
+    const auto fetch = [&](int c, int place) {
+        if (c < c_end) {
+            const uint32_t at = mine + static_cast<uint32_t>(place * stage_bytes);
+            for (int e = rw * 32 + lane; e < kParts * kCols * 16; e += row_warps * 32) {
+                const int row = e / 16, piece = e % 16, m = row % kCols;
+                const int left = m < p.m ? max(0, min(8, p.k - c * 128 - piece * 8)) : 0;
+                const uint16_t* src = static_cast<const uint16_t*>(p.a);
+                if (left) src += (static_cast<int64_t>(row / kCols) * p.m + m) * p.lda + c * 128 + piece * 8;
+                cp_async16(at + row * kPitch + piece * 16, src, left * 2);
+            }
+            if (live) {
+                const uint32_t to = at + S::kActBytes + rw * S::kCodeBytes + lane * 16;
+#pragma unroll
+                for (int r = 0; r < 2 * R; ++r)
+                    cp_async16(to + r * 512, codes + static_cast<int64_t>(c) * 512 + r * 32, 16);
+            }
+        }
+        cp_commit();  // an empty group where there is no such chunk, so that the counts stay even
+    };
+    const auto load_scales = [&](int c, uint32_t (&d)[2 * R][GROUPS == 4 ? 2 : 1], uint32_t (&z)[2 * R]) {
+#pragma unroll
+        for (int r = 0; r < 2 * R; ++r) {
+            const uint8_t* s = scales + static_cast<int64_t>(c) * (16 * 8 * GROUPS * 2) + r * (8 * GROUPS * 2);
+            if (GROUPS == 4) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+                d[r][0] = v.x;
+                d[r][GROUPS == 4 ? 1 : 0] = v.y;
+            } else if (GROUPS == 2) {
+                d[r][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+            } else {
+                d[r][0] = __ldg(reinterpret_cast<const uint16_t*>(s));
+            }
+            if (ZEROS) {
+                const uint8_t* y = zeros + static_cast<int64_t>(c) * (16 * 8 * GROUPS) + r * (8 * GROUPS);
+                z[r] = GROUPS == 4   ? __ldg(reinterpret_cast<const uint32_t*>(y))
+                       : GROUPS == 2 ? __ldg(reinterpret_cast<const uint16_t*>(y))
+                                     : __ldg(y);
+            }
+        }
+    };
+
+    float acc[R][CB][4] = {}, part[R][CB][4] = {};
+    uint32_t d_next[2 * R][GROUPS == 4 ? 2 : 1], z_next[2 * R] = {};
+    for (int i = 0; i < kRing - 1; ++i) fetch(c0 + i * shares, i);
+    if (c0 < c_end) load_scales(c0, d_next, z_next);
+    int place = 0;
+    for (int c = c0; c < c_end; c += shares) {
+        uint32_t d[2 * R][GROUPS == 4 ? 2 : 1], z[2 * R];
+#pragma unroll
+        for (int r = 0; r < 2 * R; ++r) {
+            d[r][0] = d_next[r][0];
+            if (GROUPS == 4) d[r][GROUPS == 4 ? 1 : 0] = d_next[r][GROUPS == 4 ? 1 : 0];
+            z[r] = z_next[r];
+        }
+        cp_wait<kRing - 2>();
+        // The share's copies are complete, and its warps are done with the place that is filled next.
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
+        fetch(c + (kRing - 1) * shares, place == 0 ? kRing - 1 : place - 1);
+        if (c + shares < c_end) load_scales(c + shares, d_next, z_next);
+        const uint32_t at = mine + static_cast<uint32_t>(place * stage_bytes);
+        const uint32_t acts = at + static_cast<uint32_t>(g * kPitch + t * 16);
+        const uint32_t mine_codes = at + S::kActBytes + rw * S::kCodeBytes + lane * 16;
+        if (++place == kRing) place = 0;
+        if (!live) continue;
+#pragma unroll 1
+        for (int w = 0; w < 4; ++w) {
+            uint32_t a[R][2][4];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                operands<BF16>(ld_shared_u32(mine_codes + (2 * r) * 512 + w * 4), ld_shared_u32(mine_codes + (2 * r + 1) * 512 + w * 4),
+                               code_base<BF16>(ZEROS ? z[2 * r] & 0xffu : 8u), code_base<BF16>(ZEROS ? z[2 * r + 1] & 0xffu : 8u), a[r]);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int pl = 0; pl < kParts; ++pl) {
+                    const uint4 b = ld_shared_v4(acts + (pl * kCols + cb * 8) * kPitch + w * 64);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        mma_16816<BF16>(part[r][cb], a[r][0], b.x, b.y);
+                        mma_16816<BF16>(part[r][cb], a[r][1], b.z, b.w);
+                    }
+                }
+            if ((w + 1) % kWordsPerGroup == 0) {
+                add_group<GROUPS, R, CB>(acc, part, d);
+                if (ZEROS)
+#pragma unroll
+                    for (int r = 0; r < 2 * R; ++r) z[r] >>= 8;
+            }
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();  // the ring's bytes now hold the sums
+    float* sums = reinterpret_cast<float*>(ring);
+    const int outs = 16 * R * row_warps;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                sums[(share * kCols + 8 * cb + 2 * t + (j & 1)) * outs + rw * 16 * R + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
+    __syncthreads();
+    finish_block<MODE == kModePlanes, S::kShares, 16 * R * S::kRowWarps, kCols>(p, sums, out0, 0, split);
+}
+
+inline dim3 rows_grid(const RowsParams& p, int outs, int cols) {
+    return dim3(static_cast<unsigned>((p.n + outs - 1) / outs) * p.splits, (p.m + cols - 1) / cols);
+}
+
+inline cudaError_t rows_launch(void (*kernel)(RowsParams), const RowsParams& p, dim3 grid, size_t smem, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((p.n + outs - 1) / outs) * p.splits, (p.m + kCols - 1) / kCols);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -375,24 +529,49 @@ cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, q4_rows_kernel<MODE, GROUPS, ZEROS, R, CB>, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <int MODE, int R, int CB>
-cudaError_t launch_group(const RowsParams& p, int group, cudaStream_t stream) {
-    if (p.zeros) {
-        if (group == 32) return launch<MODE, 4, true, R, CB>(p, stream);
-        if (group == 64) return launch<MODE, 2, true, R, CB>(p, stream);
-        return launch<MODE, 1, true, R, CB>(p, stream);
+template <int MODE, int GROUPS, bool ZEROS, int R, int CB>
+cudaError_t launch_staged(const RowsParams& p, cudaStream_t stream) {
+    using S = Staged<MODE, R, CB>;
+    static DeviceOnce once;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (!once.done(dev)) {
+        e = cudaFuncSetAttribute(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 S::kSmem);
+        if (e != cudaSuccess) return e;
+        once.mark(dev);
     }
-    if (group == 32) return launch<MODE, 4, false, R, CB>(p, stream);
-    if (group == 64) return launch<MODE, 2, false, R, CB>(p, stream);
-    return launch<MODE, 1, false, R, CB>(p, stream);
+    return rows_launch(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, p, rows_grid(p, 16 * R * S::kRowWarps, 8 * CB), S::kSmem,
+                       stream);
 }
 
-// Up to 8 rows (q4_rows.cu), 9 to 32 rows (q4_rows_mid.cu).
+template <int MODE, int GROUPS, bool ZEROS, int R>
+cudaError_t launch_direct(const RowsParams& p, cudaStream_t stream) {
+    return rows_launch(q4_rows_kernel<MODE, GROUPS, ZEROS, R>, p,
+                       rows_grid(p, 16 * R, 8), 0, stream);
+}
+
+// Calls f with the group's and the zero points' constants.
+template <typename F>
+cudaError_t by_group(const RowsParams& p, int group, F f) {
+    using std::integral_constant;
+    if (p.zeros) {
+        if (group == 32) return f(integral_constant<int, 4>(), std::true_type());
+        if (group == 64) return f(integral_constant<int, 2>(), std::true_type());
+        return f(integral_constant<int, 1>(), std::true_type());
+    }
+    if (group == 32) return f(integral_constant<int, 4>(), std::false_type());
+    if (group == 64) return f(integral_constant<int, 2>(), std::false_type());
+    return f(integral_constant<int, 1>(), std::false_type());
+}
+
+// Up to 8 rows as they are (q4_rows.cu); up to 32 aligned rows (q4_rows_staged.cu).
 cudaError_t launch_small(const RowsParams& p, int mode, int group, int r, cudaStream_t stream);
-cudaError_t launch_mid(const RowsParams& p, int mode, int group, cudaStream_t stream);
+cudaError_t launch_aligned(const RowsParams& p, int mode, int group, cudaStream_t stream);
 
 }  // namespace q4rows
 
