@@ -14,10 +14,17 @@
 // tiles of 8192 tokens: it loads its logits, counts the row's tokens so far that fall into the tile
 // in shared memory (integer atomics: the counts do not depend on their order), adds the listed
 // biases (one warp, in list order, so that sums do not depend on timing), and sets a bit for
-// every token so touched; eight tokens whose bits are clear skip the rules. Every block of a row
-// reads the whole list of tokens (from L2), which is what a larger tile would save and shared
-// memory limits. For `choose` the blocks of a row form a cluster of up to eight and meet through
-// distributed shared memory: no workspace, no counters, one launch.
+// every token so touched; eight tokens whose bits are clear skip the rules. Only the touched places of
+// the counts and biases are cleared, and a block keeps the lists in registers from tile to tile.
+//
+// The k best are found by a bound: a token's key is its value's order and then its place, so no two are
+// equal; tokens whose key is below the block's bound are passed over, others go to a buffer in
+// shared memory. The bound starts as the k-th largest of the threads' best keys of the first tile (k
+// threads have a key that large) and rises when the buffer has to be emptied. So nearly all tokens cost
+// one comparison of a group's maximum; per-thread lists of the k best, of which some lane of a
+// warp always has a new entry, took 250 us where this takes 60 (256 rows of 131072 f32 values, k = 8).
+// The blocks of a row form a cluster of up to eight and meet through distributed shared memory: no
+// workspace, no counters, one launch.
 #include "../../include/telmo_b200.h"
 #include "api_internal.h"
 #include "kernels.h"
@@ -28,6 +35,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace telmo {
 
@@ -38,6 +46,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                        // tokens per tile
 constexpr int kPerThread = kTile / 8 / kThreads;   // groups of eight tokens a thread has in a tile
 constexpr int kMaxK = 8;
+constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
 constexpr float kLowest = -3.402823466e38f;
 
 struct RuleParams {
@@ -88,71 +97,42 @@ struct alignas(16) Eight {
     T v[8];
 };
 
-// A row's k best values so far, best first. Values arrive in the order of their tokens, so an
-// equal value stays behind.
-template <int K>
-struct Best {
-    float x[K];
-    int id[K];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < K; ++i) {
-            x[i] = -INFINITY;
-            id[i] = INT_MAX;
-        }
-    }
-    // (v, token) goes before entry i where v is larger, or equal with a lower token.
-    __device__ __forceinline__ void insert(float v, int token) {
-#pragma unroll
-        for (int i = K - 1; i >= 0; --i) {
-            const bool here = v > x[i] || (v == x[i] && token < id[i]);
-            const bool above = i > 0 && (v > x[i - 1] || (v == x[i - 1] && token < id[i - 1]));
-            if (above) {
-                x[i] = x[i - 1];
-                id[i] = id[i - 1];
-            } else if (here) {
-                x[i] = v;
-                id[i] = token;
-            }
-        }
-    }
-    __device__ __forceinline__ void drop_first() {
-#pragma unroll
-        for (int i = 0; i + 1 < K; ++i) {
-            x[i] = x[i + 1];
-            id[i] = id[i + 1];
-        }
-        x[K - 1] = -INFINITY;
-        id[K - 1] = INT_MAX;
-    }
-};
+// A token's place in the order of choice: the larger value first (-0 counts as 0), then the lower
+// token. 0 for what is never chosen: a NaN, or -infinity.
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    const uint32_t order = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return x > -INFINITY ? (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~token) : 0;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t order = static_cast<uint32_t>(key >> 32);
+    return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ int token_of(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 
-// An unsigned number in the order of the floats (no NaN; -0 counts as 0).
-__device__ __forceinline__ uint32_t ordered(float v) {
-    const uint32_t u = __float_as_uint(v + 0.0f);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+__device__ __forceinline__ uint64_t warp_max(uint64_t key) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u);
+    return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-// The k best of the warp's lanes' lists: lane i ends with the i-th.
-template <int K>
-__device__ __forceinline__ void warp_best(Best<K>& mine, float& x, int& id) {
+// The k largest of `count` keys in shared memory, lane i of the warp (which all calls it) getting the
+// i-th, 0 where there are fewer: k rounds, each lane offering the largest of its own that is below
+// the last round's.
+__device__ __forceinline__ uint64_t warp_best(const uint64_t* keys, int count, int k) {
     const int lane = threadIdx.x % 32;
-    x = -INFINITY;
-    id = INT_MAX;
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const uint32_t key = ordered(mine.x[0]);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, key);
-        const int first = __reduce_min_sync(0xffffffffu, key == top ? mine.id[0] : INT_MAX);
-        const bool owner = key == top && mine.id[0] == first;
-        const unsigned owners = __ballot_sync(0xffffffffu, owner);
-        const float v = __shfl_sync(0xffffffffu, mine.x[0], __ffs(owners) - 1);
-        if (lane == i) {
-            x = v;
-            id = first;
+    uint64_t last = ~0ull, mine = 0;
+    for (int i = 0; i < k; ++i) {
+        uint64_t top = 0;
+        for (int c = lane; c < count; c += 32) {
+            const uint64_t v = keys[c];
+            if (v < last && v > top) top = v;
         }
-        if (owner) mine.drop_first();  // several own it only where nothing is left
+        last = warp_max(top);
+        if (lane == i) mine = last;
+        if (last == 0) break;
     }
+    return mine;
 }
 
 __device__ __forceinline__ float exp_of(float d) { return ex2_approx(d * 1.44269504f); }
@@ -172,38 +152,128 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const void* p, uint32_t rank)
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
+__device__ __forceinline__ uint64_t ld_cluster_u64(const void* p, uint32_t rank) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
 
-// T: the logits' type. K: 0 stores every value (constrain), else the tokens kept per row. Blocks
-// (x: slice of the row, y: row) take the row's tiles in turn.
-template <typename T, int K>
+// One step of the rules on a touched token's value.
+__device__ __forceinline__ float penalised(float x, uint32_t n, float theta, float freq, float pres) {
+    if (n == 0) return x;
+    x = x > 0.0f ? __fdiv_rn(x, theta) : __fmul_rn(x, theta);
+    return __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(n))), pres);
+}
+
+// The choosing side of a block.
+struct Choice {
+    uint64_t buffer[kBuffer];
+    uint64_t firsts[kWarps * kMaxK];
+    uint64_t bound, best[kMaxK];
+    int buffered;
+    float warp_m[kWarps], warp_s[kWarps], m, s;
+};
+
+// Puts the buffer's k best at its start; every thread calls it. The k-th is then a bound.
+__device__ void empty_buffer(Choice& ch, int k) {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        const uint64_t key = warp_best(ch.buffer, ch.buffered, k);
+        const int found = __popc(__ballot_sync(0xffffffffu, key != 0));
+        const uint64_t kth = __shfl_sync(0xffffffffu, key, k - 1);
+        __syncwarp();
+        if (lane < found) ch.buffer[lane] = key;
+        if (lane == 0) {
+            ch.buffered = found;
+            if (kth > ch.bound) ch.bound = kth;
+        }
+    }
+    __syncthreads();
+}
+
+// Raises the bound to the k-th largest of the threads' best keys; every thread calls it.
+__device__ void bound_by_threads(Choice& ch, uint64_t key, int k) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int i = 0; i < k; ++i) {
+        const uint64_t top = warp_max(key);
+        if (lane == 0) ch.firsts[warp * k + i] = top;
+        if (key == top) key = 0;  // a key that is not 0 is one thread's alone
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint64_t kth = __shfl_sync(0xffffffffu, warp_best(ch.firsts, kWarps * k, k), k - 1);
+        if (lane == 0 && kth > ch.bound) ch.bound = kth;
+    }
+    __syncthreads();
+}
+
+// T: the logits' type. CHOOSE: the k best of each row, else every value. Blocks (x: slice of the
+// row, y: row) take the row's tiles in turn.
+template <typename T, bool CHOOSE>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
-    constexpr int kBest = K ? K : 1;
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint32_t touched[kTile / 32];  // one bit per token of the tile
+    __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const bool counting = p.history != nullptr, biasing = p.n_bias > 0;
-    uint32_t* touched = reinterpret_cast<uint32_t*>(smem);  // one bit per token of the tile
-    uint32_t* count = touched + kTile / 32;
+    const bool counting = p.history != nullptr, biasing = p.n_bias > 0, listing = counting || biasing;
+    uint32_t* count = reinterpret_cast<uint32_t*>(smem);
     float* bias = reinterpret_cast<float*>(count + (counting ? kTile : 0));
 
     const T* in = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.ld;
-    T* out = K ? nullptr : static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_ld;
+    T* out = CHOOSE ? nullptr : static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_ld;
     // Tiles are cut where the row's addresses are multiples of 16 bytes: place e of the cut row is
     // token e - shift.
     const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
-    const bool same_cut = !K && static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T)) == shift;
+    const bool same_cut = !CHOOSE && static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T)) == shift;
     const int places = p.vocab + shift;
     const int tiles = (places + kTile - 1) / kTile;
 
-    int said = 0;
+    // The row's lists: the first of the tokens so far in every thread's registers, the first of the
+    // biases in those of the last warp.
+    constexpr int kKept = 4;
+    int said = 0, kept[kKept], bias_kept_id[kKept];
+    float bias_kept[kKept];
     float theta = 1.0f, freq = 0.0f, pres = 0.0f;
+    const int32_t* history = counting ? p.history + static_cast<int64_t>(row) * p.history_ld : nullptr;
+    const int32_t* bias_ids = biasing ? p.bias_ids + static_cast<int64_t>(row) * p.bias_ld : nullptr;
+    const float* bias_values = biasing ? p.bias + static_cast<int64_t>(row) * p.bias_ld : nullptr;
     if (counting) {
-        said = __ldg(p.history_len + row);
-        said = max(0, min(said, p.n_history));
+        said = max(0, min(__ldg(p.history_len + row), p.n_history));
         if (p.repetition) theta = __ldg(p.repetition + row);
         if (p.frequency) freq = __ldg(p.frequency + row);
         if (p.presence) pres = __ldg(p.presence + row);
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) kept[i] = tid + i * kThreads < said ? __ldg(history + tid + i * kThreads) : -1;
     }
+    const bool bias_warp = biasing && warp == kWarps - 1;
+    if (bias_warp) {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) {
+            const bool there = lane + 32 * i < p.n_bias;
+            bias_kept_id[i] = there ? __ldg(bias_ids + lane + 32 * i) : -1;
+            bias_kept[i] = there ? __ldg(bias_values + lane + 32 * i) : 0.0f;
+        }
+    }
+    // Calls f(token) for each of this thread's tokens so far, g(token, bias) for a lane's biases in list order.
+    const auto each_said = [&](auto f) {
+        if (!counting) return;
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) f(kept[i]);
+        for (int i = tid + kKept * kThreads; i < said; i += kThreads) f(__ldg(history + i));
+    };
+    const auto each_bias = [&](auto f) {
+        if (!bias_warp) return;
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (32 * i < p.n_bias) f(bias_kept_id[i], bias_kept[i]);
+        for (int base = 32 * kKept; base < p.n_bias; base += 32) {
+            const bool there = base + lane < p.n_bias;
+            f(there ? __ldg(bias_ids + base + lane) : -1, there ? __ldg(bias_values + base + lane) : 0.0f);
+        }
+    };
+
     const uint32_t* mask = nullptr;
     bool none = false;
     if (p.allowed) {
@@ -212,9 +282,13 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
         if (st >= 0 && !none) mask = p.allowed + static_cast<int64_t>(st) * p.allowed_ld;
     }
 
-    Best<kBest> best;
-    best.clear();
     MaxSum total;
+    if constexpr (CHOOSE) {
+        if (tid == 0) {
+            choice.bound = 0x007fffffffffffffull;  // the value -infinity: below what can be chosen
+            choice.buffered = 0;
+        }
+    }
 
     for (int tile = slice; tile < tiles; tile += p.slices) {
         const int e0 = tile * kTile;
@@ -233,58 +307,58 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
                     raw[i].v[j] = e + j >= shift && e + j < places ? in[e + j - shift] : from_f32<T>(0.0f);
             }
         }
-        if (counting || biasing) {
+        const int v0 = e0 - shift;  // the token at the tile's first place (negative before the row)
+        const auto in_tile = [&](int v) { return v >= 0 && v < p.vocab && v >= v0 && v - v0 < kTile; };
+        if (listing) {
             __syncthreads();  // the previous tile has been read
-            const int words = kTile / 32 + (counting ? kTile : 0) + (biasing ? kTile : 0);
-            for (int i = tid; i < words / 4; i += kThreads)
-                reinterpret_cast<uint4*>(touched)[i] = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < kTile / 32; i += kThreads) touched[i] = 0;
+            const auto clear = [&](int v) {
+                if (!in_tile(v)) return;
+                if (counting) count[v - v0] = 0;
+                if (biasing) bias[v - v0] = 0.0f;
+            };
+            each_said(clear);
+            each_bias([&](int v, float) { clear(v); });
             __syncthreads();
-            const int v0 = e0 - shift;  // the token at the tile's first place (negative before the row)
-            if (counting) {
-                const int32_t* h = p.history + static_cast<int64_t>(row) * p.history_ld;
-                for (int i = tid; i < said; i += kThreads) {
-                    const int v = __ldg(h + i);
-                    if (v >= 0 && v < p.vocab && v >= v0 && v - v0 < kTile) {
-                        atomicAdd(count + (v - v0), 1u);
-                        atomicOr(touched + (v - v0) / 32, 1u << ((v - v0) % 32));
-                    }
+            const auto touch = [&](int v) { atomicOr(touched + (v - v0) / 32, 1u << ((v - v0) % 32)); };
+            each_said([&](int v) {
+                if (!in_tile(v)) return;
+                atomicAdd(count + (v - v0), 1u);
+                touch(v);
+            });
+            each_bias([&](int v, float b) {
+                // The lowest lane of each token adds its lanes' values in lane order.
+                const bool here = in_tile(v);
+                if (!__any_sync(0xffffffffu, here)) return;
+                unsigned same = __match_any_sync(0xffffffffu, here ? v : -1);
+                const bool leader = here && __ffs(same) - 1 == lane;
+                float sum = leader ? bias[v - v0] : 0.0f;
+                while (__any_sync(0xffffffffu, leader && same)) {
+                    const int from = same ? __ffs(same) - 1 : lane;
+                    const float add = __shfl_sync(0xffffffffu, b, from);
+                    if (leader && same) sum += add;
+                    same &= same - 1;
                 }
-            }
-            if (biasing && warp == kWarps - 1) {
-                const int32_t* ids = p.bias_ids + static_cast<int64_t>(row) * p.bias_ld;
-                const float* values = p.bias + static_cast<int64_t>(row) * p.bias_ld;
-                for (int base = 0; base < p.n_bias; base += 32) {
-                    int v = -1;
-                    float b = 0.0f;
-                    if (base + lane < p.n_bias) {
-                        v = __ldg(ids + base + lane);
-                        b = __ldg(values + base + lane);
-                    }
-                    const bool here = v >= 0 && v < p.vocab && v >= v0 && v - v0 < kTile;
-                    // The lowest lane of each token adds its lanes' values in lane order.
-                    unsigned same = __match_any_sync(0xffffffffu, here ? v : -1);
-                    const bool leader = here && __ffs(same) - 1 == lane;
-                    float sum = leader ? bias[v - v0] : 0.0f;
-                    while (__any_sync(0xffffffffu, leader && same)) {
-                        const int from = same ? __ffs(same) - 1 : lane;
-                        const float add = __shfl_sync(0xffffffffu, b, from);
-                        if (leader && same) sum += add;
-                        same &= same - 1;
-                    }
-                    if (leader) {
-                        bias[v - v0] = sum;
-                        atomicOr(touched + (v - v0) / 32, 1u << ((v - v0) % 32));
-                    }
-                    __syncwarp();
+                if (leader) {
+                    bias[v - v0] = sum;
+                    touch(v);
                 }
-            }
+                __syncwarp();
+            });
             __syncthreads();
         }
+        float x[kPerThread][8];
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
             const int at = (i * kThreads + tid) * 8;  // place within the tile
             const int e = e0 + at, v = e - shift;     // place in the row, token
-            if (e >= places) continue;
+            if (e >= places) {
+                if (CHOOSE) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
+                }
+                continue;
+            }
             // Bit j: token v + j exists and is allowed.
             uint32_t ok = 0xffu;
             if (v < 0) ok = (0xffu << -v) & 0xffu;
@@ -303,34 +377,28 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
                 }
                 ok &= bits;
             }
-            float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = to_f32(raw[i].v[j]);
-            if (counting || biasing) {
+            for (int j = 0; j < 8; ++j) x[i][j] = to_f32(raw[i].v[j]);
+            if (listing) {
                 const uint32_t hit = (touched[at / 32] >> (at % 32)) & 0xffu;
                 if (hit) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (!((hit >> j) & 1)) continue;
-                        if (counting) {
-                            const uint32_t c = count[at + j];
-                            if (c) {
-                                x[j] = x[j] > 0.0f ? __fdiv_rn(x[j], theta) : __fmul_rn(x[j], theta);
-                                x[j] = __fsub_rn(x[j], __fmul_rn(freq, static_cast<float>(c)));
-                                x[j] = __fsub_rn(x[j], pres);
-                            }
-                        }
-                        if (biasing) x[j] = __fadd_rn(x[j], bias[at + j]);
+                        if (counting) x[i][j] = penalised(x[i][j], count[at + j], theta, freq, pres);
+                        if (biasing) x[i][j] = __fadd_rn(x[i][j], bias[at + j]);
                     }
                 }
             }
+            if (ok != 0xffu) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!((ok >> j) & 1)) x[j] = -INFINITY;
-            if (K == 0) {
+                for (int j = 0; j < 8; ++j)
+                    if (!((ok >> j) & 1)) x[i][j] = -INFINITY;
+            }
+            if (!CHOOSE) {
                 Eight<T> y;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y.v[j] = from_f32<T>(x[j]);
+                for (int j = 0; j < 8; ++j) y.v[j] = from_f32<T>(x[i][j]);
                 if (same_cut && inside == 0xffu) {
                     int4* dst = reinterpret_cast<int4*>(out + v);
                     const int4* src = reinterpret_cast<const int4*>(&y);
@@ -341,56 +409,78 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
                     for (int j = 0; j < 8; ++j)
                         if ((inside >> j) & 1) out[v + j] = y.v[j];
                 }
-            } else {
-                float top = x[0];
+            }
+        }
+        if constexpr (CHOOSE) {
+            float top = x[0][0];
 #pragma unroll
-                for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-                if (top > total.m) {
-                    total.s *= exp_of(total.m - top);
-                    total.m = top;
+            for (int j = 1; j < 8 * kPerThread; ++j) top = fmaxf(top, x[j / 8][j % 8]);
+            if (top > total.m) {
+                total.s *= exp_of(total.m - top);
+                total.m = top;
+            }
+#pragma unroll
+            for (int j = 0; j < 8 * kPerThread; ++j) total.s += exp_of(x[j / 8][j % 8] - total.m);
+            // Keys that reach the bound go to the buffer; it is emptied, and the bound raised, where the
+            // tile might not fit.
+            const int first = e0 - shift + tid * 8;  // the token of x[0][0]
+            const auto best_key = [&] {
+                uint64_t key = 0;
+#pragma unroll
+                for (int j = 0; j < 8 * kPerThread; ++j) {
+                    const uint64_t one = key_of(x[j / 8][j % 8], first + j / 8 * (kThreads * 8) + j % 8);
+                    if (one > key) key = one;
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) total.s += exp_of(x[j] - total.m);
-                if (top > best.x[kBest - 1]) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (x[j] > best.x[kBest - 1]) best.insert(x[j], v + j);
+                return key;
+            };
+            if (tile == slice) __syncthreads();  // the bound has been set
+            int have = 0;  // read before the meeting: behind it some thread may be adding already
+            const auto hot_threads = [&] {
+                const uint64_t bound = choice.bound;
+                have = choice.buffered;
+                const bool hot = top > -INFINITY && top >= value_of(bound | 0xffffffffu) && best_key() >= bound;
+                return __syncthreads_count(hot);
+            };
+            int hot = hot_threads();
+            if (hot > 0) {
+                if (have + hot * 8 * kPerThread > kBuffer) {
+                    empty_buffer(choice, p.k);
+                    hot = hot_threads();
+                    if (have + hot * 8 * kPerThread > kBuffer) {
+                        bound_by_threads(choice, best_key(), p.k);
+                    }
                 }
+                const uint64_t bound = choice.bound;
+                if (top > -INFINITY && top >= value_of(bound | 0xffffffffu)) {
+#pragma unroll
+                    for (int j = 0; j < 8 * kPerThread; ++j) {
+                        const uint64_t key = key_of(x[j / 8][j % 8], first + j / 8 * (kThreads * 8) + j % 8);
+                        if (key >= bound) choice.buffer[atomicAdd(&choice.buffered, 1)] = key;
+                    }
+                }
+                __syncthreads();  // the buffer's count is settled before it is read again
             }
         }
     }
 
-    if (K) {
-        __shared__ float warp_x[kWarps][kBest];
-        __shared__ int warp_id[kWarps][kBest];
-        __shared__ float warp_m[kWarps], warp_s[kWarps];
-        __shared__ float block_x[kBest], block_ms[2];
-        __shared__ int block_id[kBest];
-        float x;
-        int id;
-        warp_best<kBest>(best, x, id);
+    if constexpr (CHOOSE) {
+        if (slice >= tiles) __syncthreads();  // a block without a tile: its buffer has been set
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) {
             const float m2 = __shfl_xor_sync(0xffffffffu, total.m, d), s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
             total.merge(m2, s2);
         }
-        if (lane < kBest) {
-            warp_x[warp][lane] = x;
-            warp_id[warp][lane] = id;
-        }
         if (lane == 0) {
-            warp_m[warp] = total.m;
-            warp_s[warp] = total.s;
+            choice.warp_m[warp] = total.m;
+            choice.warp_s[warp] = total.s;
         }
         __syncthreads();
-        if (warp == 0) {
-            best.clear();
-            for (int c = lane; c < kWarps * kBest; c += 32) best.insert(warp_x[c / kBest][c % kBest], warp_id[c / kBest][c % kBest]);
-            warp_best<kBest>(best, x, id);
+        uint64_t key = 0;
+        const auto across = [&](bool there, float m, float s) {  // over the warp's lanes
             total = MaxSum();
-            if (lane < kWarps) {
-                total.m = warp_m[lane];
-                total.s = warp_s[lane];
+            if (there) {
+                total.m = m;
+                total.s = s;
             }
 #pragma unroll
             for (int d = 16; d > 0; d /= 2) {
@@ -398,59 +488,50 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
                 const float s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
                 total.merge(m2, s2);
             }
-            if (p.slices > 1) {
-                if (lane < kBest) {
-                    block_x[lane] = x;
-                    block_id[lane] = id;
-                }
-                if (lane == 0) {
-                    block_ms[0] = total.m;
-                    block_ms[1] = total.s;
-                }
+        };
+        if (warp == 0) {
+            key = warp_best(choice.buffer, choice.buffered, p.k);
+            across(lane < kWarps, choice.warp_m[lane % kWarps], choice.warp_s[lane % kWarps]);
+            if (lane < p.k) choice.best[lane] = key;
+            if (lane == 0) {
+                choice.m = total.m;
+                choice.s = total.s;
             }
         }
         if (p.slices > 1) {
+            __syncwarp();
             cluster_sync();
             if (slice == 0 && warp == 0) {
-                best.clear();
-                for (int c = lane; c < p.slices * kBest; c += 32)
-                    best.insert(__uint_as_float(ld_cluster_u32(block_x + c % kBest, c / kBest)),
-                                static_cast<int>(ld_cluster_u32(block_id + c % kBest, c / kBest)));
-                warp_best<kBest>(best, x, id);
-                total = MaxSum();
-                if (lane < p.slices) {
-                    total.m = __uint_as_float(ld_cluster_u32(block_ms, lane));
-                    total.s = __uint_as_float(ld_cluster_u32(block_ms + 1, lane));
-                }
-#pragma unroll
-                for (int d = 16; d > 0; d /= 2) {
-                    const float m2 = __shfl_xor_sync(0xffffffffu, total.m, d);
-                    const float s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
-                    total.merge(m2, s2);
-                }
+                // At most 8 blocks of 8 keys: two a lane.
+                for (int c = lane; c < p.slices * p.k; c += 32)
+                    choice.firsts[c] = ld_cluster_u64(&choice.best[c % p.k], c / p.k);
+                __syncwarp();
+                key = warp_best(choice.firsts, p.slices * p.k, p.k);
+                const uint32_t from = lane < p.slices ? lane : 0;
+                across(lane < p.slices, __uint_as_float(ld_cluster_u32(&choice.m, from)),
+                       __uint_as_float(ld_cluster_u32(&choice.s, from)));
             }
+            __syncwarp();
             cluster_sync();  // the other blocks' shared memory has been read
         }
         if (slice == 0 && warp == 0 && lane < p.k) {
-            const bool found = id != INT_MAX;
             const int64_t at = static_cast<int64_t>(row) * p.k + lane;
-            p.ids[at] = found ? id : -1;
-            if (p.logprobs) p.logprobs[at] = found ? (x - total.m) - logf(total.s) : -INFINITY;
+            p.ids[at] = key ? token_of(key) : -1;
+            if (p.logprobs) p.logprobs[at] = key ? (value_of(key) - total.m) - logf(total.s) : -INFINITY;
         }
     }
 }
 
-template <typename T, int K>
+template <typename T, bool CHOOSE>
 cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
     static DeviceOnce once;
-    const size_t rules = (p.history ? kTile * 4 : 0) + (p.n_bias > 0 ? kTile * 4 : 0);
-    const size_t bytes = rules ? rules + kTile / 8 : 0;
+    const size_t bytes = (p.history ? kTile * 4 : 0) + (p.n_bias > 0 ? kTile * 4 : 0);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!once.done(dev)) {
-        if ((e = cudaFuncSetAttribute(logits_kernel<T, K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kTile * 8 + kTile / 8)) != cudaSuccess)
+        if ((e = cudaFuncSetAttribute(logits_kernel<T, CHOOSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kTile * 8)) != cudaSuccess)
             return e;
         once.mark(dev);
     }
@@ -489,17 +570,17 @@ cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = K && p.slices > 1 ? 1 : 0;
-        if ((e = cudaLaunchKernelEx(&cfg, logits_kernel<T, K>, q)) != cudaSuccess) return e;
+        cfg.numAttrs = CHOOSE && p.slices > 1 ? 1 : 0;
+        if ((e = cudaLaunchKernelEx(&cfg, logits_kernel<T, CHOOSE>, q)) != cudaSuccess) return e;
     }
     return cudaSuccess;
 }
 
-template <int K>
+template <bool CHOOSE>
 cudaError_t launch_type(const RuleParams& p, int dtype, cudaStream_t stream) {
-    if (dtype == TELMO_DTYPE_F32) return launch<float, K>(p, stream);
-    if (dtype == TELMO_DTYPE_BF16) return launch<__nv_bfloat16, K>(p, stream);
-    return launch<__half, K>(p, stream);
+    if (dtype == TELMO_DTYPE_F32) return launch<float, CHOOSE>(p, stream);
+    if (dtype == TELMO_DTYPE_BF16) return launch<__nv_bfloat16, CHOOSE>(p, stream);
+    return launch<__half, CHOOSE>(p, stream);
 }
 
 // Checks what both entry points share and fills `p`.
@@ -579,8 +660,11 @@ extern "C" int telmo_logits_constrain(telmo_ctx* c, const void* logits, int dtyp
     if (int rc = scope.enter(ctx)) return rc;
     p.out = out;
     p.out_ld = static_cast<int64_t>(out_ld);
-    p.slices = (p.vocab + 7 + kTile - 1) / kTile;
-    return ctx->cuda(launch_type<0>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_constrain");
+    // As many blocks as tiles, or several tiles a block (whose lists are read once) where six blocks per
+    // SM stay.
+    const int tiles = (p.vocab + 7 + kTile - 1) / kTile;
+    p.slices = std::min<int64_t>(tiles, std::max<int64_t>(1, (6ll * ctx->sms + p.rows - 1) / p.rows));
+    return ctx->cuda(launch_type<false>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_constrain");
 }
 
 extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, size_t ld, size_t rows, size_t vocab,
@@ -600,12 +684,9 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    // Enough blocks for two per SM, and no block without a tile.
+    // Clusters of up to eight blocks a row until there are six blocks per SM or a tile for each.
     const int tiles = (p.vocab + 7 + kTile - 1) / kTile;
     p.slices = 1;
-    while (p.slices < 8 && p.slices < tiles && static_cast<int64_t>(p.slices) * p.rows < 2 * ctx->sms) p.slices *= 2;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = k == 1 ? launch_type<1>(p, dtype, s) : k == 2 ? launch_type<2>(p, dtype, s)
-                        : k <= 4 ? launch_type<4>(p, dtype, s) : launch_type<8>(p, dtype, s);
-    return ctx->cuda(e, "telmo_logits_choose");
+    while (p.slices < 8 && p.slices < tiles && static_cast<int64_t>(p.slices) * p.rows < 6 * ctx->sms) p.slices *= 2;
+    return ctx->cuda(launch_type<true>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_choose");
 }
