@@ -10,21 +10,29 @@
 // `constrain` stores x in the logits' type; `choose` keeps the k best x of a row, ties to the lowest
 // token, and their log-probabilities x - log sum_v e^x, and stores nothing else.
 //
-// Both read the logits once and are bound by that (constrain writes them once more). A block takes
-// tiles of 8192 tokens: it loads its logits, counts the row's tokens so far that fall into the tile
-// in shared memory (integer atomics: the counts do not depend on their order), adds the listed
-// biases (one warp, in list order, so that sums do not depend on timing), and sets a bit for
-// every token so touched; eight tokens whose bits are clear skip the rules. Only the touched places of
-// the counts and biases are cleared, and a block keeps the lists in registers from tile to tile.
+// Both read the logits once and are bound by that (constrain writes them once more), if few
+// instructions go to each value: 6.5 TB/s leave an SM about ten a value of 16 bits. So the pass over the
+// logits knows masks alone, and the listed tokens, few against the vocabulary, come after it, a token
+// a thread:
+//   constrain  copies allowed values and writes -infinity elsewhere, in the logits' own type; then
+//              each listed token that is allowed is read again (in place or not, it is still the
+//              logit), goes through the rules and is written.
+//   choose     leaves listed tokens out by a bit map of the window; then they go through the rules and
+//              join the others.
+// A block walks over windows of 16384 tokens: it collects the window's tokens so far from the row's list
+// (again for each window), gives each listed token a number, and counts by number in shared
+// memory with integer atomics (the counts do not depend on their order); the listed biases are added
+// by one warp in list order, so that sums do not depend on timing. A window with more listed tokens than
+// there are numbers goes in sections of as many places. With the rules inside the pass over the logits
+// some lane of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16
+// values with 2000 tokens each.
 //
 // The k best are found by a bound: a token's key is its value's order and then its place, so no two are
 // equal; tokens whose key is below the block's bound are passed over, others go to a buffer in
-// shared memory. The bound starts as the k-th largest of the threads' best keys of the first tile (k
-// threads have a key that large) and rises when the buffer has to be emptied. So nearly all tokens cost
-// one comparison of a group's maximum; per-thread lists of the k best, of which some lane of a
-// warp always has a new entry, took 250 us where this takes 60 (256 rows of 131072 f32 values, k = 8).
-// The blocks of a row form a cluster of up to eight and meet through distributed shared memory: no
-// workspace, no counters, one launch.
+// shared memory. The bound starts as the k-th largest of the warps' largest values of the first tile (k
+// warps have a value that large) and rises when the buffer has to be emptied, so nearly all tokens cost
+// one comparison of a thread's maximum. The blocks of a row form a cluster of up to eight and meet
+// through distributed shared memory: no workspace, no counters, one launch.
 #include "../../include/telmo_b200.h"
 #include "api_internal.h"
 #include "kernels.h"
@@ -45,6 +53,8 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                        // tokens per tile
 constexpr int kPerThread = kTile / 8 / kThreads;   // groups of eight tokens a thread has in a tile
+constexpr int kWindow = 2 * kTile;                 // tokens per window
+constexpr int kNumbers = 2048;                     // listed tokens with a number, and tokens so far collected
 constexpr int kMaxK = 8;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
 constexpr float kLowest = -3.402823466e38f;
@@ -99,10 +109,12 @@ struct alignas(16) Eight {
 
 // A token's place in the order of choice: the larger value first (-0 counts as 0), then the lower
 // token. 0 for what is never chosen: a NaN, or -infinity.
-__device__ __forceinline__ uint64_t key_of(float x, int token) {
+__device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
-    const uint32_t order = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return x > -INFINITY ? (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~token) : 0;
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+    return x > -INFINITY ? (static_cast<uint64_t>(order_of(x)) << 32) | static_cast<uint32_t>(~token) : 0;
 }
 __device__ __forceinline__ float value_of(uint64_t key) {
     const uint32_t order = static_cast<uint32_t>(key >> 32);
@@ -116,30 +128,30 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t key) {
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-// The k largest of `count` keys in shared memory, lane i of the warp (which all calls it) getting the
-// i-th, 0 where there are fewer: k rounds, each lane offering the largest of its own that is below
-// the last round's.
-__device__ __forceinline__ uint64_t warp_best(const uint64_t* keys, int count, int k) {
-    const int lane = threadIdx.x % 32;
-    uint64_t last = ~0ull, mine = 0;
-    for (int i = 0; i < k; ++i) {
-        uint64_t top = 0;
-        for (int c = lane; c < count; c += 32) {
-            const uint64_t v = keys[c];
-            if (v < last && v > top) top = v;
-        }
-        last = warp_max(top);
-        if (lane == i) mine = last;
-        if (last == 0) break;
+// The k largest of `count` keys in shared memory, in order, into best (0 where there are fewer). Every
+// thread calls it, with the keys written and synchronised; best is written behind the next meeting.
+__device__ __forceinline__ void find_best(const uint64_t* keys, int count, int k, uint64_t* best) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const uint64_t mine = keys[i];
+        int larger = 0;
+        for (int j = 0; j < count; ++j) larger += keys[j] > mine;
+        if (larger < k) best[larger] = mine;
     }
-    return mine;
 }
 
 __device__ __forceinline__ float exp_of(float d) { return ex2_approx(d * 1.44269504f); }
 
-// Running maximum and sum of e^(x - maximum).
+// The sum of e^x as e^m s with the running maximum m. (One fused multiply-add for x log2 e - m log2 e would
+// save an instruction a value, but overflow at a type's lowest value.)
 struct MaxSum {
     float m = kLowest, s = 0.0f;
+    __device__ __forceinline__ void reach(float top) {
+        if (top > m) {
+            s *= exp_of(m - top);
+            m = top;
+        }
+    }
+    __device__ __forceinline__ void add(float x) { s += exp_of(x - m); }
     __device__ __forceinline__ void merge(float m2, float s2) {
         const float top = fmaxf(m, m2);
         s = s * exp_of(m - top) + s2 * exp_of(m2 - top);
@@ -171,23 +183,20 @@ struct Choice {
     uint64_t firsts[kWarps * kMaxK];
     uint64_t bound, best[kMaxK];
     int buffered;
+    uint32_t warp_top[kWarps];
     float warp_m[kWarps], warp_s[kWarps], m, s;
 };
 
-// Puts the buffer's k best at its start; every thread calls it. The k-th is then a bound.
+// Keeps the buffer's k best alone and makes the k-th the bound; every thread calls it.
 __device__ void empty_buffer(Choice& ch, int k) {
+    if (threadIdx.x < kMaxK) ch.best[threadIdx.x] = 0;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        const uint64_t key = warp_best(ch.buffer, ch.buffered, k);
-        const int found = __popc(__ballot_sync(0xffffffffu, key != 0));
-        const uint64_t kth = __shfl_sync(0xffffffffu, key, k - 1);
-        __syncwarp();
-        if (lane < found) ch.buffer[lane] = key;
-        if (lane == 0) {
-            ch.buffered = found;
-            if (kth > ch.bound) ch.bound = kth;
-        }
+    find_best(ch.buffer, ch.buffered, k, ch.best);
+    __syncthreads();
+    if (threadIdx.x < k) ch.buffer[threadIdx.x] = ch.best[threadIdx.x];
+    if (threadIdx.x == 0) {
+        ch.buffered = min(ch.buffered, k);
+        if (ch.best[k - 1] > ch.bound) ch.bound = ch.best[k - 1];
     }
     __syncthreads();
 }
@@ -195,31 +204,70 @@ __device__ void empty_buffer(Choice& ch, int k) {
 // Raises the bound to the k-th largest of the threads' best keys; every thread calls it.
 __device__ void bound_by_threads(Choice& ch, uint64_t key, int k) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x < kMaxK) ch.best[threadIdx.x] = 0;
     for (int i = 0; i < k; ++i) {
         const uint64_t top = warp_max(key);
         if (lane == 0) ch.firsts[warp * k + i] = top;
         if (key == top) key = 0;  // a key that is not 0 is one thread's alone
     }
     __syncthreads();
-    if (warp == 0) {
-        const uint64_t kth = __shfl_sync(0xffffffffu, warp_best(ch.firsts, kWarps * k, k), k - 1);
-        if (lane == 0 && kth > ch.bound) ch.bound = kth;
+    // Keys of 0 have as many larger ones as there are others: at most the last of them is one of the k best.
+    find_best(ch.firsts, kWarps * k, k, ch.best);
+    __syncthreads();
+    if (threadIdx.x == 0 && ch.best[k - 1] > ch.bound) ch.bound = ch.best[k - 1];
+    __syncthreads();
+}
+
+// The first bound: the k-th largest of the warps' largest values. top: the thread's.
+__device__ void bound_by_warps(Choice& ch, float top, int k) {
+    const uint32_t order = __reduce_max_sync(0xffffffffu, order_of(top > -INFINITY ? top : -INFINITY));
+    if (threadIdx.x % 32 == 0) ch.warp_top[threadIdx.x / 32] = order;
+    __syncthreads();
+    if (threadIdx.x < kWarps) {
+        const uint32_t mine = ch.warp_top[threadIdx.x];
+        int before = 0;  // larger ones, and equal ones of earlier warps
+        for (int w = 0; w < kWarps; ++w)
+            before += ch.warp_top[w] > mine || (ch.warp_top[w] == mine && w < static_cast<int>(threadIdx.x));
+        const uint64_t bound = static_cast<uint64_t>(mine) << 32;
+        if (before == k - 1 && bound > ch.bound) ch.bound = bound;
     }
     __syncthreads();
 }
 
+// Eight values of which those with a bit of `ok` clear become -infinity.
+__device__ __forceinline__ void keep_allowed(Eight<float>& y, uint32_t ok) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (!((ok >> j) & 1)) y.v[j] = -INFINITY;
+}
+template <typename T>
+__device__ __forceinline__ void keep_allowed(Eight<T>& y, uint32_t ok) {
+    constexpr uint32_t kNone = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t two = (ok >> (2 * j)) & 3u, keep = ((two | (two << 15)) & 0x00010001u) * 0xffffu;
+        w[j] = (w[j] & keep) | (kNone & ~keep);
+    }
+}
+
 // T: the logits' type. CHOOSE: the k best of each row, else every value. Blocks (x: slice of the
-// row, y: row) take the row's tiles in turn.
+// row, y: row) take the row's windows in turn.
 template <typename T, bool CHOOSE>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint32_t touched[kTile / 32];  // one bit per token of the tile
+    __shared__ uint32_t left_out[CHOOSE ? kWindow / 32 : 1];  // a bit per place of the window: it is listed
+    __shared__ uint32_t numbered[kWindow / 32];               // a bit per place of the section: it has a number
+    __shared__ uint16_t window_said[kNumbers];
+    __shared__ int n_said, n_listed, numbers;
     __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const bool counting = p.history != nullptr, biasing = p.n_bias > 0, listing = counting || biasing;
-    uint32_t* count = reinterpret_cast<uint32_t*>(smem);
-    float* bias = reinterpret_cast<float*>(count + (counting ? kTile : 0));
+    uint16_t* number = reinterpret_cast<uint16_t*>(smem);  // by place
+    uint16_t* list = number + kWindow;                     // places by number
+    uint32_t* count = reinterpret_cast<uint32_t*>(list + kNumbers);
+    float* bias = reinterpret_cast<float*>(count + kNumbers);
 
     const T* in = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.ld;
     T* out = CHOOSE ? nullptr : static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_ld;
@@ -228,49 +276,36 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
     const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
     const bool same_cut = !CHOOSE && static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T)) == shift;
     const int places = p.vocab + shift;
-    const int tiles = (places + kTile - 1) / kTile;
 
-    // The row's lists: the first of the tokens so far in every thread's registers, the first of the
-    // biases in those of the last warp.
-    constexpr int kKept = 4;
-    int said = 0, kept[kKept], bias_kept_id[kKept];
-    float bias_kept[kKept];
+    // The row's lists. What lies outside the vocabulary becomes kNowhere. (They are read again for each
+    // window, from L1 or L2: keeping them in registers cost the pass over the logits spills.)
+    constexpr int kNowhere = INT_MIN;
+    int said = 0;
     float theta = 1.0f, freq = 0.0f, pres = 0.0f;
     const int32_t* history = counting ? p.history + static_cast<int64_t>(row) * p.history_ld : nullptr;
     const int32_t* bias_ids = biasing ? p.bias_ids + static_cast<int64_t>(row) * p.bias_ld : nullptr;
     const float* bias_values = biasing ? p.bias + static_cast<int64_t>(row) * p.bias_ld : nullptr;
+    const auto token = [&](const int32_t* list_at) {
+        const int v = __ldg(list_at);
+        return v >= 0 && v < p.vocab ? v : kNowhere;
+    };
     if (counting) {
         said = max(0, min(__ldg(p.history_len + row), p.n_history));
         if (p.repetition) theta = __ldg(p.repetition + row);
         if (p.frequency) freq = __ldg(p.frequency + row);
         if (p.presence) pres = __ldg(p.presence + row);
-#pragma unroll
-        for (int i = 0; i < kKept; ++i) kept[i] = tid + i * kThreads < said ? __ldg(history + tid + i * kThreads) : -1;
     }
-    const bool bias_warp = biasing && warp == kWarps - 1;
-    if (bias_warp) {
-#pragma unroll
-        for (int i = 0; i < kKept; ++i) {
-            const bool there = lane + 32 * i < p.n_bias;
-            bias_kept_id[i] = there ? __ldg(bias_ids + lane + 32 * i) : -1;
-            bias_kept[i] = there ? __ldg(bias_values + lane + 32 * i) : 0.0f;
-        }
-    }
-    // Calls f(token) for each of this thread's tokens so far, g(token, bias) for a lane's biases in list order.
+    // Calls f(token) for each of this thread's tokens so far, f(token, bias) for the last warp's lanes in list
+    // order.
     const auto each_said = [&](auto f) {
-        if (!counting) return;
-#pragma unroll
-        for (int i = 0; i < kKept; ++i) f(kept[i]);
-        for (int i = tid + kKept * kThreads; i < said; i += kThreads) f(__ldg(history + i));
+#pragma unroll 4
+        for (int i = tid; i < said; i += kThreads) f(token(history + i));
     };
     const auto each_bias = [&](auto f) {
-        if (!bias_warp) return;
-#pragma unroll
-        for (int i = 0; i < kKept; ++i)
-            if (32 * i < p.n_bias) f(bias_kept_id[i], bias_kept[i]);
-        for (int base = 32 * kKept; base < p.n_bias; base += 32) {
+        if (!biasing || warp != kWarps - 1) return;
+        for (int base = 0; base < p.n_bias; base += 32) {
             const bool there = base + lane < p.n_bias;
-            f(there ? __ldg(bias_ids + base + lane) : -1, there ? __ldg(bias_values + base + lane) : 0.0f);
+            f(there ? token(bias_ids + base + lane) : kNowhere, there ? __ldg(bias_values + base + lane) : 0.0f);
         }
     };
 
@@ -283,188 +318,251 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
     }
 
     MaxSum total;
+    bool bounded = false;  // the bound comes from a tile
+    int used = 0;          // no fewer than the buffer's keys
     if constexpr (CHOOSE) {
         if (tid == 0) {
             choice.bound = 0x007fffffffffffffull;  // the value -infinity: below what can be chosen
             choice.buffered = 0;
         }
     }
+    // Up to kMost tokens of every thread: those that reach the bound go to the buffer, which is emptied, and
+    // the bound raised, where they might not fit. top: the thread's largest value; each_token(f) calls
+    // f(value, token). Every thread calls this.
+    const auto offer = [&](float top, auto each_token, auto most) {
+        if constexpr (CHOOSE) {
+            constexpr int kMost = decltype(most)::value;
+            if (!bounded) {
+                bound_by_warps(choice, top, p.k);
+                bounded = true;
+            }
+            const auto hot = [&] { return top > -INFINITY && top >= value_of(choice.bound); };
+            int n = __syncthreads_count(hot());
+            if (n == 0) return;
+            if (used + n * kMost > kBuffer) {
+                empty_buffer(choice, p.k);
+                used = p.k;
+                n = __syncthreads_count(hot());
+                if (used + n * kMost > kBuffer) {
+                    uint64_t best = 0;
+                    each_token([&](float x, int v) {
+                        const uint64_t key = key_of(x, v);
+                        if (key > best) best = key;
+                    });
+                    bound_by_threads(choice, best, p.k);
+                    n = p.k;  // threads with a key that large
+                }
+            }
+            used += n * kMost;
+            const uint64_t bound = choice.bound;
+            if (hot())
+                each_token([&](float x, int v) {
+                    if (!(x >= value_of(bound))) return;
+                    const uint64_t key = key_of(x, v);
+                    if (key >= bound) choice.buffer[atomicAdd(&choice.buffered, 1)] = key;
+                });
+        }
+    };
 
-    for (int tile = slice; tile < tiles; tile += p.slices) {
-        const int e0 = tile * kTile;
-        Eight<T> raw[kPerThread];
+    for (int w_begin = slice * kWindow; w_begin < places; w_begin += p.slices * kWindow) {
+        const int w0 = w_begin - shift;  // the token at the window's first place (negative before the row)
+        const auto in_window = [&](int v) { return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u; };
+        if (listing) {
+            __syncthreads();  // the previous window is done with
+            if (tid == 0) n_said = n_listed = 0;
+            if (CHOOSE)
+                for (int i = tid; i < kWindow / 32; i += kThreads) left_out[i] = 0;
+            __syncthreads();
+            each_said([&](int v) {
+                const unsigned at = in_window(v);
+                if (at >= kWindow) return;
+                if (CHOOSE) atomicOr(left_out + at / 32, 1u << (at % 32));
+                const int i = atomicAdd(&n_said, 1);
+                if (i < kNumbers) window_said[i] = static_cast<uint16_t>(at);
+            });
+            each_bias([&](int v, float) {
+                const unsigned at = in_window(v);
+                if (at >= kWindow) return;
+                if (CHOOSE) atomicOr(left_out + at / 32, 1u << (at % 32));
+                atomicAdd(&n_listed, 1);
+            });
+            __syncthreads();
+        } else if (CHOOSE && !bounded) {
+            __syncthreads();  // the bound has been set
+        }
+
+        // ---- the logits ----------------------------------------------------------------------------
+        for (int e0 = w_begin; e0 < min(places, w_begin + kWindow); e0 += kTile) {
+            const int v0 = e0 - shift;
+            Eight<T> raw[kPerThread];
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const int e = e0 + (i * kThreads + tid) * 8;
-            if (e >= shift && e + 8 <= places) {
-                const int4* src = reinterpret_cast<const int4*>(in + (e - shift));
-                int4* dst = reinterpret_cast<int4*>(&raw[i]);
+            for (int i = 0; i < kPerThread; ++i) {
+                const int e = e0 + (i * kThreads + tid) * 8;
+                if (e >= shift && e + 8 <= places) {
+                    const int4* src = reinterpret_cast<const int4*>(in + (e - shift));
+                    int4* dst = reinterpret_cast<int4*>(&raw[i]);
 #pragma unroll
-                for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) dst[j] = src[j];
-            } else {
+                    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) dst[j] = src[j];
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    raw[i].v[j] = e + j >= shift && e + j < places ? in[e + j - shift] : from_f32<T>(0.0f);
+                    for (int j = 0; j < 8; ++j)
+                        raw[i].v[j] = e + j >= shift && e + j < places ? in[e + j - shift] : from_f32<T>(0.0f);
+                }
+            }
+            float x[CHOOSE ? kPerThread : 1][8];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int e = e0 + (i * kThreads + tid) * 8, v = e - shift;  // place in the row, token
+                // Bit j: token v + j exists and is allowed.
+                uint32_t inside = 0xffu;
+                if (v < 0) inside = (0xffu << -v) & 0xffu;
+                if (v + 8 > p.vocab) inside = e < places ? inside & (0xffu >> (v + 8 - p.vocab)) : 0u;
+                uint32_t ok = none ? 0u : inside;
+                if (mask && inside) {
+                    uint32_t bits;
+                    if (v < 0) {
+                        bits = __ldg(mask) << -v;
+                    } else {
+                        const uint32_t m0 = __ldg(mask + v / 32);
+                        const bool next = v % 32 > 24 && (v / 32 + 1) * 32 < p.vocab;
+                        const uint32_t m1 = next ? __ldg(mask + v / 32 + 1) : 0u;
+                        bits = __funnelshift_r(m0, m1, v % 32);
+                    }
+                    ok &= bits;
+                }
+                if (CHOOSE) {
+                    if (listing) ok &= ~(left_out[(e - w_begin) / 32] >> (e % 32));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[CHOOSE ? i : 0][j] = (ok >> j) & 1 ? to_f32(raw[i].v[j]) : -INFINITY;
+                } else if (inside) {
+                    if (ok != 0xffu) keep_allowed(raw[i], ok);
+                    if (same_cut && inside == 0xffu) {
+                        int4* dst = reinterpret_cast<int4*>(out + v);
+                        const int4* src = reinterpret_cast<const int4*>(&raw[i]);
+#pragma unroll
+                        for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) dst[j] = src[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if ((inside >> j) & 1) out[v + j] = raw[i].v[j];
+                    }
+                }
+            }
+            if constexpr (CHOOSE) {
+                float top = x[0][0];
+#pragma unroll
+                for (int j = 1; j < 8 * kPerThread; ++j) top = fmaxf(top, x[j / 8][j % 8]);
+                total.reach(top);
+#pragma unroll
+                for (int j = 0; j < 8 * kPerThread; ++j) total.add(x[j / 8][j % 8]);
+                offer(
+                    top,
+                    [&](auto f) {
+#pragma unroll
+                        for (int j = 0; j < 8 * kPerThread; ++j)
+                            f(x[j / 8][j % 8], v0 + (j / 8 * kThreads + tid) * 8 + j % 8);
+                    },
+                    std::integral_constant<int, 8 * kPerThread>());
             }
         }
-        const int v0 = e0 - shift;  // the token at the tile's first place (negative before the row)
-        const auto in_tile = [&](int v) { return v >= 0 && v < p.vocab && v >= v0 && v - v0 < kTile; };
-        if (listing) {
-            __syncthreads();  // the previous tile has been read
-            for (int i = tid; i < kTile / 32; i += kThreads) touched[i] = 0;
-            const auto clear = [&](int v) {
-                if (!in_tile(v)) return;
-                if (counting) count[v - v0] = 0;
-                if (biasing) bias[v - v0] = 0.0f;
+        if (!listing || n_said + n_listed == 0) continue;
+
+        // ---- the listed tokens: all at once, or in sections of as many places as there are numbers ----
+        const int section = n_said + n_listed <= kNumbers ? kWindow : kNumbers;
+        for (int s0 = 0; s0 < kWindow; s0 += section) {
+            const auto place = [&](int v) {  // within the window, if in the section
+                const unsigned at = in_window(v);
+                return at - static_cast<unsigned>(s0) < static_cast<unsigned>(section) ? at : ~0u;
             };
-            each_said(clear);
-            each_bias([&](int v, float) { clear(v); });
+            const auto each_place = [&](auto f) {  // of the tokens so far in this section
+                if (n_said <= kNumbers) {
+                    for (int i = tid; i < n_said; i += kThreads) {
+                        const unsigned at = window_said[i];
+                        if (at - static_cast<unsigned>(s0) < static_cast<unsigned>(section)) f(at);
+                    }
+                } else {
+                    each_said([&](int v) {
+                        const unsigned at = place(v);
+                        if (at != ~0u) f(at);
+                    });
+                }
+            };
+            __syncthreads();  // the logits have been written (constrain), the previous section is done with
+            for (int i = tid; i < kWindow / 32; i += kThreads) numbered[i] = 0;
+            if (tid == 0) numbers = 0;
             __syncthreads();
-            const auto touch = [&](int v) { atomicOr(touched + (v - v0) / 32, 1u << ((v - v0) % 32)); };
-            each_said([&](int v) {
-                if (!in_tile(v)) return;
-                atomicAdd(count + (v - v0), 1u);
-                touch(v);
+            const auto give_number = [&](unsigned at) {
+                const uint32_t bit = 1u << (at % 32);
+                if (atomicOr(numbered + at / 32, bit) & bit) return;
+                const int i = atomicAdd(&numbers, 1);
+                number[at] = static_cast<uint16_t>(i);
+                list[i] = static_cast<uint16_t>(at);
+                count[i] = 0;
+                bias[i] = 0.0f;
+            };
+            each_place(give_number);
+            each_bias([&](int v, float) {
+                const unsigned at = place(v);
+                if (at != ~0u) give_number(at);
             });
+            __syncthreads();
+            each_place([&](unsigned at) { atomicAdd(count + number[at], 1u); });
             each_bias([&](int v, float b) {
                 // The lowest lane of each token adds its lanes' values in lane order.
-                const bool here = in_tile(v);
+                const unsigned at = place(v);
+                const bool here = at != ~0u;
                 if (!__any_sync(0xffffffffu, here)) return;
-                unsigned same = __match_any_sync(0xffffffffu, here ? v : -1);
+                unsigned same = __match_any_sync(0xffffffffu, at);
                 const bool leader = here && __ffs(same) - 1 == lane;
-                float sum = leader ? bias[v - v0] : 0.0f;
+                float sum = leader ? bias[number[at]] : 0.0f;
                 while (__any_sync(0xffffffffu, leader && same)) {
                     const int from = same ? __ffs(same) - 1 : lane;
                     const float add = __shfl_sync(0xffffffffu, b, from);
                     if (leader && same) sum += add;
                     same &= same - 1;
                 }
-                if (leader) {
-                    bias[v - v0] = sum;
-                    touch(v);
-                }
+                if (leader) bias[number[at]] = sum;
                 __syncwarp();
             });
             __syncthreads();
-        }
-        float x[kPerThread][8];
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const int at = (i * kThreads + tid) * 8;  // place within the tile
-            const int e = e0 + at, v = e - shift;     // place in the row, token
-            if (e >= places) {
+            const int n = numbers;
+            float top = -INFINITY;
+            for (int i = tid; i < n; i += kThreads) {
+                const int v = w0 + list[i];
+                const uint32_t bits = mask ? __ldg(mask + v / 32) : ~0u;
+                float x = to_f32(in[v]);
+                x = penalised(x, count[i], theta, freq, pres);
+                if (biasing) x = __fadd_rn(x, bias[i]);
+                const bool ok = !none && ((bits >> (v % 32)) & 1);
                 if (CHOOSE) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
-                }
-                continue;
-            }
-            // Bit j: token v + j exists and is allowed.
-            uint32_t ok = 0xffu;
-            if (v < 0) ok = (0xffu << -v) & 0xffu;
-            if (v + 8 > p.vocab) ok &= 0xffu >> (v + 8 - p.vocab);
-            const uint32_t inside = ok;
-            if (none) ok = 0;
-            if (mask) {
-                uint32_t bits;
-                if (v < 0) {
-                    bits = __ldg(mask) << -v;
-                } else {
-                    const uint32_t w0 = __ldg(mask + v / 32);
-                    const bool next = v % 32 > 24 && (v / 32 + 1) * 32 < p.vocab;
-                    const uint32_t w1 = next ? __ldg(mask + v / 32 + 1) : 0u;
-                    bits = __funnelshift_r(w0, w1, v % 32);
-                }
-                ok &= bits;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] = to_f32(raw[i].v[j]);
-            if (listing) {
-                const uint32_t hit = (touched[at / 32] >> (at % 32)) & 0xffu;
-                if (hit) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (!((hit >> j) & 1)) continue;
-                        if (counting) x[i][j] = penalised(x[i][j], count[at + j], theta, freq, pres);
-                        if (biasing) x[i][j] = __fadd_rn(x[i][j], bias[at + j]);
-                    }
+                    x = ok ? x : -INFINITY;
+                    bias[i] = x;
+                    top = fmaxf(top, x);
+                } else if (ok) {
+                    out[v] = from_f32<T>(x);
                 }
             }
-            if (ok != 0xffu) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!((ok >> j) & 1)) x[i][j] = -INFINITY;
-            }
-            if (!CHOOSE) {
-                Eight<T> y;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y.v[j] = from_f32<T>(x[i][j]);
-                if (same_cut && inside == 0xffu) {
-                    int4* dst = reinterpret_cast<int4*>(out + v);
-                    const int4* src = reinterpret_cast<const int4*>(&y);
-#pragma unroll
-                    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) dst[j] = src[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if ((inside >> j) & 1) out[v + j] = y.v[j];
+            if constexpr (CHOOSE) {
+                offer(
+                    top,
+                    [&](auto f) {
+                        for (int i = tid; i < n; i += kThreads) f(bias[i], w0 + list[i]);
+                    },
+                    std::integral_constant<int, kNumbers / kThreads>());
+                // Numbers go by who came first; the sum goes by place, so that it does not depend on that.
+                for (int w = tid; w < kWindow / 32; w += kThreads) {
+                    float most = -INFINITY;
+                    for (uint32_t b = numbered[w]; b; b &= b - 1) most = fmaxf(most, bias[number[w * 32 + __ffs(b) - 1]]);
+                    total.reach(most);
+                    for (uint32_t b = numbered[w]; b; b &= b - 1) total.add(bias[number[w * 32 + __ffs(b) - 1]]);
                 }
-            }
-        }
-        if constexpr (CHOOSE) {
-            float top = x[0][0];
-#pragma unroll
-            for (int j = 1; j < 8 * kPerThread; ++j) top = fmaxf(top, x[j / 8][j % 8]);
-            if (top > total.m) {
-                total.s *= exp_of(total.m - top);
-                total.m = top;
-            }
-#pragma unroll
-            for (int j = 0; j < 8 * kPerThread; ++j) total.s += exp_of(x[j / 8][j % 8] - total.m);
-            // Keys that reach the bound go to the buffer; it is emptied, and the bound raised, where the
-            // tile might not fit.
-            const int first = e0 - shift + tid * 8;  // the token of x[0][0]
-            const auto best_key = [&] {
-                uint64_t key = 0;
-#pragma unroll
-                for (int j = 0; j < 8 * kPerThread; ++j) {
-                    const uint64_t one = key_of(x[j / 8][j % 8], first + j / 8 * (kThreads * 8) + j % 8);
-                    if (one > key) key = one;
-                }
-                return key;
-            };
-            if (tile == slice) __syncthreads();  // the bound has been set
-            int have = 0;  // read before the meeting: behind it some thread may be adding already
-            const auto hot_threads = [&] {
-                const uint64_t bound = choice.bound;
-                have = choice.buffered;
-                const bool hot = top > -INFINITY && top >= value_of(bound | 0xffffffffu) && best_key() >= bound;
-                return __syncthreads_count(hot);
-            };
-            int hot = hot_threads();
-            if (hot > 0) {
-                if (have + hot * 8 * kPerThread > kBuffer) {
-                    empty_buffer(choice, p.k);
-                    hot = hot_threads();
-                    if (have + hot * 8 * kPerThread > kBuffer) {
-                        bound_by_threads(choice, best_key(), p.k);
-                    }
-                }
-                const uint64_t bound = choice.bound;
-                if (top > -INFINITY && top >= value_of(bound | 0xffffffffu)) {
-#pragma unroll
-                    for (int j = 0; j < 8 * kPerThread; ++j) {
-                        const uint64_t key = key_of(x[j / 8][j % 8], first + j / 8 * (kThreads * 8) + j % 8);
-                        if (key >= bound) choice.buffer[atomicAdd(&choice.buffered, 1)] = key;
-                    }
-                }
-                __syncthreads();  // the buffer's count is settled before it is read again
             }
         }
     }
 
     if constexpr (CHOOSE) {
-        if (slice >= tiles) __syncthreads();  // a block without a tile: its buffer has been set
+        if (tid < kMaxK) choice.best[tid] = 0;
+        __syncthreads();  // the buffer is complete; a block without a window has set it
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) {
             const float m2 = __shfl_xor_sync(0xffffffffu, total.m, d), s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
@@ -475,7 +573,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
             choice.warp_s[warp] = total.s;
         }
         __syncthreads();
-        uint64_t key = 0;
+        find_best(choice.buffer, choice.buffered, p.k, choice.best);
         const auto across = [&](bool there, float m, float s) {  // over the warp's lanes
             total = MaxSum();
             if (there) {
@@ -490,23 +588,31 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
             }
         };
         if (warp == 0) {
-            key = warp_best(choice.buffer, choice.buffered, p.k);
             across(lane < kWarps, choice.warp_m[lane % kWarps], choice.warp_s[lane % kWarps]);
-            if (lane < p.k) choice.best[lane] = key;
             if (lane == 0) {
                 choice.m = total.m;
                 choice.s = total.s;
             }
         }
+        __syncthreads();
+        uint64_t key = lane < p.k ? choice.best[lane] : 0;
         if (p.slices > 1) {
             __syncwarp();
             cluster_sync();
             if (slice == 0 && warp == 0) {
-                // At most 8 blocks of 8 keys: two a lane.
-                for (int c = lane; c < p.slices * p.k; c += 32)
-                    choice.firsts[c] = ld_cluster_u64(&choice.best[c % p.k], c / p.k);
+                // At most 8 blocks of 8 keys, two a lane: each key's place is the number of larger ones.
+                const int all = p.slices * p.k;
+                for (int c = lane; c < all; c += 32) choice.firsts[c] = ld_cluster_u64(&choice.best[c % p.k], c / p.k);
                 __syncwarp();
-                key = warp_best(choice.firsts, p.slices * p.k, p.k);
+                if (lane < p.k) choice.buffer[lane] = 0;
+                __syncwarp();
+                for (int c = lane; c < all; c += 32) {
+                    int larger = 0;
+                    for (int j = 0; j < all; ++j) larger += choice.firsts[j] > choice.firsts[c];
+                    if (larger < p.k) choice.buffer[larger] = choice.firsts[c];
+                }
+                __syncwarp();
+                key = lane < p.k ? choice.buffer[lane] : 0;
                 const uint32_t from = lane < p.slices ? lane : 0;
                 across(lane < p.slices, __uint_as_float(ld_cluster_u32(&choice.m, from)),
                        __uint_as_float(ld_cluster_u32(&choice.s, from)));
@@ -525,13 +631,14 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const RuleParams p) {
 template <typename T, bool CHOOSE>
 cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
     static DeviceOnce once;
-    const size_t bytes = (p.history ? kTile * 4 : 0) + (p.n_bias > 0 ? kTile * 4 : 0);
+    constexpr size_t kLists = kWindow * 2 + kNumbers * 10;
+    const size_t bytes = p.history || p.n_bias > 0 ? kLists : 0;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!once.done(dev)) {
         if ((e = cudaFuncSetAttribute(logits_kernel<T, CHOOSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kTile * 8)) != cudaSuccess)
+                                      static_cast<int>(kLists))) != cudaSuccess)
             return e;
         once.mark(dev);
     }
@@ -581,6 +688,12 @@ cudaError_t launch_type(const RuleParams& p, int dtype, cudaStream_t stream) {
     if (dtype == TELMO_DTYPE_F32) return launch<float, CHOOSE>(p, stream);
     if (dtype == TELMO_DTYPE_BF16) return launch<__nv_bfloat16, CHOOSE>(p, stream);
     return launch<__half, CHOOSE>(p, stream);
+}
+
+// Windows of a row, some of whose rows may start up to seven values behind a 16-byte boundary.
+int windows(const RuleParams& p, size_t size) {
+    const bool aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * size % 16 == 0;
+    return (p.vocab + (aligned ? 0 : 7) + kWindow - 1) / kWindow;
 }
 
 // Checks what both entry points share and fills `p`.
@@ -660,10 +773,7 @@ extern "C" int telmo_logits_constrain(telmo_ctx* c, const void* logits, int dtyp
     if (int rc = scope.enter(ctx)) return rc;
     p.out = out;
     p.out_ld = static_cast<int64_t>(out_ld);
-    // As many blocks as tiles, or several tiles a block (whose lists are read once) where six blocks per
-    // SM stay.
-    const int tiles = (p.vocab + 7 + kTile - 1) / kTile;
-    p.slices = std::min<int64_t>(tiles, std::max<int64_t>(1, (6ll * ctx->sms + p.rows - 1) / p.rows));
+    p.slices = windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
     return ctx->cuda(launch_type<false>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_constrain");
 }
 
@@ -684,9 +794,8 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    // Clusters of up to eight blocks a row until there are six blocks per SM or a tile for each.
-    const int tiles = (p.vocab + 7 + kTile - 1) / kTile;
+    // A block for each window, up to a cluster of eight.
     p.slices = 1;
-    while (p.slices < 8 && p.slices < tiles && static_cast<int64_t>(p.slices) * p.rows < 6 * ctx->sms) p.slices *= 2;
+    while (p.slices < 8 && p.slices < windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2)) p.slices *= 2;
     return ctx->cuda(launch_type<true>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_choose");
 }
