@@ -21,8 +21,8 @@
 //              join the others.
 // A block walks over windows of 16384 tokens: it collects the window's tokens so far from the row's list
 // (again for each window), gives each listed token a number, and counts by number in shared
-// memory with integer atomics (the counts do not depend on their order); the listed biases are added
-// by one warp in list order, so that sums do not depend on timing. A window with more listed tokens than
+// memory with integer atomics (the counts do not depend on their order); a token's first entry among the
+// biases adds the others in list order, so that sums do not depend on timing. A window with more listed tokens than
 // there are numbers goes in sections of as many places. With the rules inside the pass over the logits
 // some lane of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16
 // values with 2000 tokens each.
@@ -256,10 +256,10 @@ __device__ __forceinline__ void keep_allowed(Eight<T>& y, uint32_t ok) {
 template <typename T, bool CHOOSE>
 __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint32_t left_out[CHOOSE ? kWindow / 32 : 1];  // a bit per place of the window: it is listed
-    __shared__ uint32_t numbered[kWindow / 32];               // a bit per place of the section: it has a number
+    __shared__ uint32_t listed[kWindow / 32];                 // a bit per place of the window
+    __shared__ uint32_t numbered_also[CHOOSE ? kWindow / 32 : 1];  // and per place of a section
     __shared__ uint16_t window_said[kNumbers];
-    __shared__ int n_said, n_listed, numbers;
+    __shared__ int n_said, numbers, twice;  // twice: a token stands twice among the biases
     __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
     uint16_t* list = number + kWindow;                     // places by number
     uint32_t* count = reinterpret_cast<uint32_t*>(list + kNumbers);
     float* bias = reinterpret_cast<float*>(count + kNumbers);
+    uint32_t* entry = reinterpret_cast<uint32_t*>(bias + kNumbers);  // a bias of the token
 
     const T* in = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.ld;
     T* out = CHOOSE ? nullptr : static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_ld;
@@ -295,18 +296,14 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
         if (p.frequency) freq = __ldg(p.frequency + row);
         if (p.presence) pres = __ldg(p.presence + row);
     }
-    // Calls f(token) for each of this thread's tokens so far, f(token, bias) for the last warp's lanes in list
-    // order.
+    // Calls f(token) for each of this thread's tokens so far, f(token, bias, entry) for its biases.
     const auto each_said = [&](auto f) {
 #pragma unroll 4
         for (int i = tid; i < said; i += kThreads) f(token(history + i));
     };
     const auto each_bias = [&](auto f) {
-        if (!biasing || warp != kWarps - 1) return;
-        for (int base = 0; base < p.n_bias; base += 32) {
-            const bool there = base + lane < p.n_bias;
-            f(there ? token(bias_ids + base + lane) : kNowhere, there ? __ldg(bias_values + base + lane) : 0.0f);
-        }
+        if (biasing)
+            for (int i = tid; i < p.n_bias; i += kThreads) f(token(bias_ids + i), __ldg(bias_values + i), i);
     };
 
     const uint32_t* mask = nullptr;
@@ -367,29 +364,76 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
     for (int w_begin = slice * kWindow; w_begin < places; w_begin += p.slices * kWindow) {
         const int w0 = w_begin - shift;  // the token at the window's first place (negative before the row)
         const auto in_window = [&](int v) { return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u; };
-        if (listing) {
-            __syncthreads();  // the previous window is done with
-            if (tid == 0) n_said = n_listed = 0;
-            if (CHOOSE)
-                for (int i = tid; i < kWindow / 32; i += kThreads) left_out[i] = 0;
+        // The listed tokens of places s0 .. s0 + section of the window get numbers, if there are enough;
+        // `bits` gets a bit for each. The tokens so far come from the row's list and, where `collect`,
+        // are collected.
+        const auto give_numbers = [&](uint32_t* bits, unsigned s0, unsigned section, bool collect) {
+            for (int i = tid; i < kWindow / 32; i += kThreads) bits[i] = 0;
+            if (tid == 0) {
+                numbers = 0;
+                twice = 0;
+                if (collect) n_said = 0;
+            }
             __syncthreads();
+            const auto give = [&](unsigned at) {
+                const uint32_t bit = 1u << (at % 32);
+                if (atomicOr(bits + at / 32, bit) & bit) return;
+                const int i = atomicAdd(&numbers, 1);
+                if (i >= kNumbers) return;
+                number[at] = static_cast<uint16_t>(i);
+                list[i] = static_cast<uint16_t>(at);
+                count[i] = 0;
+                bias[i] = 0.0f;
+                entry[i] = ~0u;
+            };
             each_said([&](int v) {
                 const unsigned at = in_window(v);
-                if (at >= kWindow) return;
-                if (CHOOSE) atomicOr(left_out + at / 32, 1u << (at % 32));
+                if (at - s0 >= section) return;
+                give(at);
+                if (!collect) return;
                 const int i = atomicAdd(&n_said, 1);
                 if (i < kNumbers) window_said[i] = static_cast<uint16_t>(at);
             });
-            each_bias([&](int v, float) {
-                const unsigned at = in_window(v);
-                if (at >= kWindow) return;
-                if (CHOOSE) atomicOr(left_out + at / 32, 1u << (at % 32));
-                atomicAdd(&n_listed, 1);
+            each_bias([&](int v, float, int) {
+                if (in_window(v) - s0 < section) give(in_window(v));
             });
             __syncthreads();
+        };
+        // The numbered tokens' counts and biases. A token's biases add up in list order.
+        const auto add_up = [&](unsigned s0, unsigned section) {
+            if (n_said <= kNumbers) {
+                for (int i = tid; i < n_said; i += kThreads) {
+                    const unsigned at = window_said[i];
+                    if (at - s0 < section) atomicAdd(count + number[at], 1u);
+                }
+            } else {
+                each_said([&](int v) {
+                    if (in_window(v) - s0 < section) atomicAdd(count + number[in_window(v)], 1u);
+                });
+            }
+            if (!biasing) return;
+            each_bias([&](int v, float, int i) {
+                if (in_window(v) - s0 < section && atomicMin(entry + number[in_window(v)], static_cast<uint32_t>(i)) != ~0u) twice = 1;
+            });
+            __syncthreads();
+            const bool search = twice != 0;
+            each_bias([&](int v, float b, int i) {
+                if (in_window(v) - s0 >= section) return;
+                const int n = number[in_window(v)];
+                if (entry[n] != static_cast<uint32_t>(i)) return;  // the token's first entry adds the others
+                if (search)
+                    for (int j = i + 1; j < p.n_bias; ++j)
+                        if (__ldg(bias_ids + j) == v) b += __ldg(bias_values + j);
+                bias[n] = b;
+            });
+        };
+        if (listing) {
+            __syncthreads();  // the previous window is done with
+            give_numbers(listed, 0, kWindow, true);
         } else if (CHOOSE && !bounded) {
             __syncthreads();  // the bound has been set
         }
+        const int window_numbers = listing ? numbers : 0;  // the same for every thread until the list's turn
 
         // ---- the logits ----------------------------------------------------------------------------
         for (int e0 = w_begin; e0 < min(places, w_begin + kWindow); e0 += kTile) {
@@ -431,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
                     ok &= bits;
                 }
                 if (CHOOSE) {
-                    if (listing) ok &= ~(left_out[(e - w_begin) / 32] >> (e % 32));
+                    if (listing) ok &= ~(listed[(e - w_begin) / 32] >> (e % 32));
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[CHOOSE ? i : 0][j] = (ok >> j) & 1 ? to_f32(raw[i].v[j]) : -INFINITY;
                 } else if (inside) {
@@ -465,65 +509,17 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
                     std::integral_constant<int, 8 * kPerThread>());
             }
         }
-        if (!listing || n_said + n_listed == 0) continue;
+        if (window_numbers == 0) continue;
 
         // ---- the listed tokens: all at once, or in sections of as many places as there are numbers ----
-        const int section = n_said + n_listed <= kNumbers ? kWindow : kNumbers;
-        for (int s0 = 0; s0 < kWindow; s0 += section) {
-            const auto place = [&](int v) {  // within the window, if in the section
-                const unsigned at = in_window(v);
-                return at - static_cast<unsigned>(s0) < static_cast<unsigned>(section) ? at : ~0u;
-            };
-            const auto each_place = [&](auto f) {  // of the tokens so far in this section
-                if (n_said <= kNumbers) {
-                    for (int i = tid; i < n_said; i += kThreads) {
-                        const unsigned at = window_said[i];
-                        if (at - static_cast<unsigned>(s0) < static_cast<unsigned>(section)) f(at);
-                    }
-                } else {
-                    each_said([&](int v) {
-                        const unsigned at = place(v);
-                        if (at != ~0u) f(at);
-                    });
-                }
-            };
+        const bool fits = window_numbers <= kNumbers;
+        const unsigned section = fits ? kWindow : kNumbers;
+        uint32_t* numbered = CHOOSE ? numbered_also : listed;
+        if (fits) numbered = listed;
+        for (unsigned s0 = 0; s0 < kWindow; s0 += section) {
             __syncthreads();  // the logits have been written (constrain), the previous section is done with
-            for (int i = tid; i < kWindow / 32; i += kThreads) numbered[i] = 0;
-            if (tid == 0) numbers = 0;
-            __syncthreads();
-            const auto give_number = [&](unsigned at) {
-                const uint32_t bit = 1u << (at % 32);
-                if (atomicOr(numbered + at / 32, bit) & bit) return;
-                const int i = atomicAdd(&numbers, 1);
-                number[at] = static_cast<uint16_t>(i);
-                list[i] = static_cast<uint16_t>(at);
-                count[i] = 0;
-                bias[i] = 0.0f;
-            };
-            each_place(give_number);
-            each_bias([&](int v, float) {
-                const unsigned at = place(v);
-                if (at != ~0u) give_number(at);
-            });
-            __syncthreads();
-            each_place([&](unsigned at) { atomicAdd(count + number[at], 1u); });
-            each_bias([&](int v, float b) {
-                // The lowest lane of each token adds its lanes' values in lane order.
-                const unsigned at = place(v);
-                const bool here = at != ~0u;
-                if (!__any_sync(0xffffffffu, here)) return;
-                unsigned same = __match_any_sync(0xffffffffu, at);
-                const bool leader = here && __ffs(same) - 1 == lane;
-                float sum = leader ? bias[number[at]] : 0.0f;
-                while (__any_sync(0xffffffffu, leader && same)) {
-                    const int from = same ? __ffs(same) - 1 : lane;
-                    const float add = __shfl_sync(0xffffffffu, b, from);
-                    if (leader && same) sum += add;
-                    same &= same - 1;
-                }
-                if (leader) bias[number[at]] = sum;
-                __syncwarp();
-            });
+            if (!fits) give_numbers(numbered, s0, section, false);
+            add_up(s0, section);
             __syncthreads();
             const int n = numbers;
             float top = -INFINITY;
@@ -631,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
 template <typename T, bool CHOOSE>
 cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
     static DeviceOnce once;
-    constexpr size_t kLists = kWindow * 2 + kNumbers * 10;
+    constexpr size_t kLists = kWindow * 2 + kNumbers * 14;
     const size_t bytes = p.history || p.n_bias > 0 ? kLists : 0;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -794,8 +790,9 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    // A block for each window, up to a cluster of eight.
+    // A block for each window, up to a cluster of eight; several windows a block where six blocks per SM stay.
     p.slices = 1;
-    while (p.slices < 8 && p.slices < windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2)) p.slices *= 2;
+    const int most = windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    while (p.slices < 8 && p.slices < most && static_cast<int64_t>(p.slices) * p.rows < 6 * ctx->sms) p.slices *= 2;
     return ctx->cuda(launch_type<true>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_choose");
 }
