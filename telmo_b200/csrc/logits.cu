@@ -19,13 +19,13 @@
 //              logit), goes through the rules and is written.
 //   choose     leaves listed tokens out by a bit map of the window; then they go through the rules and
 //              join the others.
-// A block walks over windows of 16384 tokens: it collects the window's tokens so far from the row's list
-// (again for each window), gives each listed token a number, and counts by number in shared
-// memory with integer atomics (the counts do not depend on their order); a token's first entry among the
-// biases adds the others in list order, so that sums do not depend on timing. A window with more listed tokens than
-// there are numbers goes in sections of as many places. With the rules inside the pass over the logits
-// some lane of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16
-// values with 2000 tokens each.
+// A block walks over windows of 16384 tokens: it sets a bit for each listed token's place, numbers the
+// bits in order (a prefix sum over the words' counts), and counts by number in shared memory with
+// integer atomics (the counts do not depend on their order); a token's first entry among the biases adds
+// the others in list order. Tokens go to threads by number, so no sum depends on timing. A window with
+// more listed tokens than there are numbers goes in sections of as many places. With the rules inside
+// the pass over the logits some lane of a warp nearly always had a listed token and all paid: 92 us for 256
+// rows of 131072 bf16 values with 2000 tokens each.
 //
 // The k best are found by a bound: a token's key is its value's order and then its place, so no two are
 // equal; tokens whose key is below the block's bound are passed over, others go to a buffer in
@@ -54,7 +54,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                        // tokens per tile
 constexpr int kPerThread = kTile / 8 / kThreads;   // groups of eight tokens a thread has in a tile
 constexpr int kWindow = 2 * kTile;                 // tokens per window
-constexpr int kNumbers = 2048;                     // listed tokens with a number, and tokens so far collected
+constexpr int kNumbers = 2048;                     // listed tokens with a number
 constexpr int kMaxK = 8;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
 constexpr float kLowest = -3.402823466e38f;
@@ -256,16 +256,15 @@ __device__ __forceinline__ void keep_allowed(Eight<T>& y, uint32_t ok) {
 template <typename T, bool CHOOSE>
 __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint32_t listed[kWindow / 32];                 // a bit per place of the window
-    __shared__ uint32_t numbered_also[CHOOSE ? kWindow / 32 : 1];  // and per place of a section
-    __shared__ uint16_t window_said[kNumbers];
-    __shared__ int n_said, numbers, twice;  // twice: a token stands twice among the biases
+    __shared__ uint32_t listed[kWindow / 32];          // a bit per place of the window
+    __shared__ uint32_t in_section[kWindow / 32];      // and per place of a section of it
+    __shared__ uint16_t before[kWindow / 32];          // bits in the words before
+    __shared__ int warp_bits[kWarps], twice;           // twice: a token stands twice among the biases
     __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const bool counting = p.history != nullptr, biasing = p.n_bias > 0, listing = counting || biasing;
-    uint16_t* number = reinterpret_cast<uint16_t*>(smem);  // by place
-    uint16_t* list = number + kWindow;                     // places by number
+    uint16_t* list = reinterpret_cast<uint16_t*>(smem);  // places by number
     uint32_t* count = reinterpret_cast<uint32_t*>(list + kNumbers);
     float* bias = reinterpret_cast<float*>(count + kNumbers);
     uint32_t* entry = reinterpret_cast<uint32_t*>(bias + kNumbers);  // a bias of the token
@@ -364,62 +363,64 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
     for (int w_begin = slice * kWindow; w_begin < places; w_begin += p.slices * kWindow) {
         const int w0 = w_begin - shift;  // the token at the window's first place (negative before the row)
         const auto in_window = [&](int v) { return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u; };
-        // The listed tokens of places s0 .. s0 + section of the window get numbers, if there are enough;
-        // `bits` gets a bit for each. The tokens so far come from the row's list and, where `collect`,
-        // are collected.
-        const auto give_numbers = [&](uint32_t* bits, unsigned s0, unsigned section, bool collect) {
+        // Sets the bits of the listed tokens at places s0 .. s0 + section of the window and numbers them, if
+        // there are numbers enough. Returns how many there are.
+        const auto give_numbers = [&](uint32_t* bits, unsigned s0, unsigned section) -> int {
             for (int i = tid; i < kWindow / 32; i += kThreads) bits[i] = 0;
-            if (tid == 0) {
-                numbers = 0;
-                twice = 0;
-                if (collect) n_said = 0;
-            }
+            if (tid == 0) twice = 0;
             __syncthreads();
-            const auto give = [&](unsigned at) {
-                const uint32_t bit = 1u << (at % 32);
-                if (atomicOr(bits + at / 32, bit) & bit) return;
-                const int i = atomicAdd(&numbers, 1);
-                if (i >= kNumbers) return;
-                number[at] = static_cast<uint16_t>(i);
-                list[i] = static_cast<uint16_t>(at);
-                count[i] = 0;
-                bias[i] = 0.0f;
-                entry[i] = ~0u;
-            };
-            each_said([&](int v) {
+            const auto give = [&](int v) {
                 const unsigned at = in_window(v);
-                if (at - s0 >= section) return;
-                give(at);
-                if (!collect) return;
-                const int i = atomicAdd(&n_said, 1);
-                if (i < kNumbers) window_said[i] = static_cast<uint16_t>(at);
-            });
-            each_bias([&](int v, float, int) {
-                if (in_window(v) - s0 < section) give(in_window(v));
-            });
+                if (at - s0 < section) atomicOr(bits + at / 32, 1u << (at % 32));
+            };
+            each_said(give);
+            each_bias([&](int v, float, int) { give(v); });
             __syncthreads();
+            static_assert(kWindow / 32 == kThreads, "a word of bits a thread");
+            const uint32_t word = bits[tid];
+            int upto = __popc(word);
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += up;
+            }
+            if (lane == 31) warp_bits[warp] = upto;
+            __syncthreads();
+            int all = 0;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) upto += all;
+                all += warp_bits[w];
+            }
+            int i = upto - __popc(word);
+            before[tid] = static_cast<uint16_t>(i);
+            if (all <= kNumbers)
+                for (uint32_t b = word; b; b &= b - 1, ++i) {
+                    list[i] = static_cast<uint16_t>(tid * 32 + __ffs(b) - 1);
+                    count[i] = 0;
+                    bias[i] = 0.0f;
+                    entry[i] = ~0u;
+                }
+            __syncthreads();
+            return all;
         };
         // The numbered tokens' counts and biases. A token's biases add up in list order.
-        const auto add_up = [&](unsigned s0, unsigned section) {
-            if (n_said <= kNumbers) {
-                for (int i = tid; i < n_said; i += kThreads) {
-                    const unsigned at = window_said[i];
-                    if (at - s0 < section) atomicAdd(count + number[at], 1u);
-                }
-            } else {
-                each_said([&](int v) {
-                    if (in_window(v) - s0 < section) atomicAdd(count + number[in_window(v)], 1u);
-                });
-            }
+        const auto add_up = [&](const uint32_t* bits, unsigned s0, unsigned section) {
+            const auto number = [&](unsigned at) { return before[at / 32] + __popc(bits[at / 32] & ((1u << (at % 32)) - 1)); };
+            each_said([&](int v) {
+                const unsigned at = in_window(v);
+                if (at - s0 < section) atomicAdd(count + number(at), 1u);
+            });
             if (!biasing) return;
             each_bias([&](int v, float, int i) {
-                if (in_window(v) - s0 < section && atomicMin(entry + number[in_window(v)], static_cast<uint32_t>(i)) != ~0u) twice = 1;
+                const unsigned at = in_window(v);
+                if (at - s0 < section && atomicMin(entry + number(at), static_cast<uint32_t>(i)) != ~0u) twice = 1;
             });
             __syncthreads();
             const bool search = twice != 0;
             each_bias([&](int v, float b, int i) {
-                if (in_window(v) - s0 >= section) return;
-                const int n = number[in_window(v)];
+                const unsigned at = in_window(v);
+                if (at - s0 >= section) return;
+                const int n = number(at);
                 if (entry[n] != static_cast<uint32_t>(i)) return;  // the token's first entry adds the others
                 if (search)
                     for (int j = i + 1; j < p.n_bias; ++j)
@@ -427,13 +428,13 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
                 bias[n] = b;
             });
         };
+        int numbers = 0;
         if (listing) {
             __syncthreads();  // the previous window is done with
-            give_numbers(listed, 0, kWindow, true);
+            numbers = give_numbers(listed, 0, kWindow);
         } else if (CHOOSE && !bounded) {
             __syncthreads();  // the bound has been set
         }
-        const int window_numbers = listing ? numbers : 0;  // the same for every thread until the list's turn
 
         // ---- the logits ----------------------------------------------------------------------------
         for (int e0 = w_begin; e0 < min(places, w_begin + kWindow); e0 += kTile) {
@@ -509,17 +510,15 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
                     std::integral_constant<int, 8 * kPerThread>());
             }
         }
-        if (window_numbers == 0) continue;
+        if (numbers == 0) continue;
 
         // ---- the listed tokens: all at once, or in sections of as many places as there are numbers ----
-        const bool fits = window_numbers <= kNumbers;
+        const bool fits = numbers <= kNumbers;
         const unsigned section = fits ? kWindow : kNumbers;
-        uint32_t* numbered = CHOOSE ? numbered_also : listed;
-        if (fits) numbered = listed;
         for (unsigned s0 = 0; s0 < kWindow; s0 += section) {
             __syncthreads();  // the logits have been written (constrain), the previous section is done with
-            if (!fits) give_numbers(numbered, s0, section, false);
-            add_up(s0, section);
+            if (!fits) numbers = give_numbers(in_section, s0, section);
+            add_up(fits ? listed : in_section, s0, section);
             __syncthreads();
             const int n = numbers;
             float top = -INFINITY;
@@ -539,19 +538,14 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
                 }
             }
             if constexpr (CHOOSE) {
+                total.reach(top);
+                for (int i = tid; i < n; i += kThreads) total.add(bias[i]);
                 offer(
                     top,
                     [&](auto f) {
                         for (int i = tid; i < n; i += kThreads) f(bias[i], w0 + list[i]);
                     },
                     std::integral_constant<int, kNumbers / kThreads>());
-                // Numbers go by who came first; the sum goes by place, so that it does not depend on that.
-                for (int w = tid; w < kWindow / 32; w += kThreads) {
-                    float most = -INFINITY;
-                    for (uint32_t b = numbered[w]; b; b &= b - 1) most = fmaxf(most, bias[number[w * 32 + __ffs(b) - 1]]);
-                    total.reach(most);
-                    for (uint32_t b = numbered[w]; b; b &= b - 1) total.add(bias[number[w * 32 + __ffs(b) - 1]]);
-                }
             }
         }
     }
@@ -627,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p)
 template <typename T, bool CHOOSE>
 cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
     static DeviceOnce once;
-    constexpr size_t kLists = kWindow * 2 + kNumbers * 14;
+    constexpr size_t kLists = kNumbers * 14;
     const size_t bytes = p.history || p.n_bias > 0 ? kLists : 0;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
