@@ -254,7 +254,7 @@ __device__ __forceinline__ void keep_allowed(Eight<T>& y, uint32_t ok) {
 // T: the logits' type. CHOOSE: the k best of each row, else every value. Blocks (x: slice of the
 // row, y: row) take the row's windows in turn.
 template <typename T, bool CHOOSE>
-__global__ void __launch_bounds__(kThreads, 2) logits_kernel(const RuleParams p) {
+__global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const RuleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t listed[kWindow / 32];          // a bit per place of the window
     __shared__ uint32_t in_section[kWindow / 32];      // and per place of a section of it
@@ -784,9 +784,11 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    // A block for each window, up to a cluster of eight; several windows a block where six blocks per SM stay.
+    // A block for each window, up to a cluster of eight, until all SMs have the two blocks they can hold: a
+    // block's first bound and its end cost as much as a window (256 rows of 131072: 103 us on two blocks a row,
+    // 114 on four).
     p.slices = 1;
     const int most = windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
-    while (p.slices < 8 && p.slices < most && static_cast<int64_t>(p.slices) * p.rows < 6 * ctx->sms) p.slices *= 2;
+    while (p.slices < 8 && p.slices < most && static_cast<int64_t>(p.slices) * p.rows < 2 * ctx->sms) p.slices *= 2;
     return ctx->cuda(launch_type<true>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_choose");
 }
