@@ -89,7 +89,7 @@ def _refuse(message: str):
 def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
     """The address of a [rows, cols] matrix with rows `ld` elements apart that starts at tensor `t`,
     which must lie on the context's device, be of one of `dtypes` and reach to the last element."""
-    if not t.is_cuda or t.get_device() != ctx.device:
+    if t.get_device() != ctx.device:  # -1 in host memory
         _refuse(f"{name}: a tensor on {t.device}, the context is on cuda:{ctx.device}")
     if t.dtype not in dtypes:
         _refuse(f"{name}: {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
@@ -125,9 +125,16 @@ def _i32_only() -> tuple:
 def _stream_on(ctx, stream) -> Optional[int]:
     """The given stream, or torch's current stream on the context's device."""
     if stream is None:
-        import torch
-        return torch.cuda.current_stream(ctx.device).cuda_stream
+        return _current_stream()(ctx.device)
     return getattr(stream, "cuda_stream", stream)
+
+
+@functools.lru_cache(maxsize=None)
+def _current_stream():
+    """A function from a device to torch's current stream there, as an address."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object in between
+    return raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class Context:
@@ -285,7 +292,29 @@ class LogitRules:
     allowed: Optional[object] = None      # int32 (or uint32) [states, ceil(vocab / 32)] bit masks
     state: Optional[object] = None        # int32 [rows], negative: no mask; None: row r has mask r
 
+    def __post_init__(self):
+        self._checked = None  # the last structure, and what it was made of
+
     def _struct(self, ctx, rows: int, vocab: int) -> "_lib.LogitRules":
+        """The checked C structure. It is made again unless the call's sizes, the tensors and their
+        addresses and element counts are those of the last call."""
+        tensors = (self.history, self.history_len, self.repetition, self.frequency, self.presence,
+                   self.bias_ids, self.bias, self.allowed, self.state)
+        if self._checked is not None:
+            device, r, v, known, s = self._checked
+            if device == ctx.device and r == rows and v == vocab:
+                for t, (u, address, count) in zip(tensors, known):
+                    if t is not u or (t is not None and (t.data_ptr() != address or t.numel() != count)):
+                        break
+                else:
+                    return s
+        s = self._check(ctx, rows, vocab)
+        known = tuple((t, None if t is None else t.data_ptr(), None if t is None else t.numel())
+                      for t in tensors)
+        self._checked = (ctx.device, rows, vocab, known, s)
+        return s
+
+    def _check(self, ctx, rows: int, vocab: int) -> "_lib.LogitRules":
         import torch
         i32, f32 = (torch.int32,), (torch.float32,)
 
