@@ -33,6 +33,8 @@
 #include "tma.h"
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -77,7 +79,7 @@ struct GemmParams {
     int c_type;
     int64_t ldc;
     int tiles, num_n;
-    int splits;        // CTAs (one cluster) that share a tile's inputs; 1 with pairs
+    int splits;        // CTAs or pairs of one cluster that share a tile's inputs
     int split_chunks;  // chunks of each
     uint32_t* error;
 };
@@ -136,11 +138,12 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
-// Arrives on the same barrier of both CTAs of the pair once this thread's products are complete.
-__device__ __forceinline__ void commit_both(uint64_t* bar) {
+// Arrives on the same barrier of both CTAs of the pair (the bits of their ranks: `both`) once this thread's
+// products are complete.
+__device__ __forceinline__ void commit_both(uint64_t* bar, uint16_t both) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+        ::"r"(smem_u32(bar)), "h"(both) : "memory");
 }
 
 // A ring position and its phase.
@@ -156,39 +159,36 @@ struct Ring {
     }
 };
 
-// Stores one output of up to 16 rows.
-template <typename T>
-__device__ __forceinline__ void store_rows(const GemmParams& p, float (&v)[16], int row, int n) {
+// Stores one output of N rows (those below m).
+template <typename T, int N>
+__device__ __forceinline__ void store_rows(const GemmParams& p, float (&v)[N], int row, int n) {
     T* out = static_cast<T*>(p.c) + static_cast<int64_t>(row) * p.ldc + n;
-    const int rows = min(16, p.m - row);
+    const int rows = min(N, p.m - row);
     if (p.accumulate) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < N; ++j)
             if (j < rows) v[j] += static_cast<float>(out[j * p.ldc]);
     }
-    if (rows == 16) {
+    if (rows == N) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < N; ++j) {
             *out = static_cast<T>(v[j]);
             out += p.ldc;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < N; ++j)
             if (j < rows) out[j * p.ldc] = static_cast<T>(v[j]);
     }
 }
 
-// The epilogue of one output's sums over 16 rows (those below m).
-template <int P>
-__device__ __forceinline__ void finish_rows(const GemmParams& p, const uint32_t (&sum)[16], int row, int n, float bias) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(sum[j]);
+// The epilogue of one output's sums over N rows, a multiple of four (those below m).
+template <int P, int N>
+__device__ __forceinline__ void finish_rows(const GemmParams& p, float (&v)[N], int row, int n, float bias) {
     if (P == 2) {
         const float4* rs = reinterpret_cast<const float4*>(p.row_scale + row);  // padded to whole tiles
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < N / 4; ++j) {
             const float4 s = __ldg(rs + j);
             v[4 * j] *= s.x;
             v[4 * j + 1] *= s.y;
@@ -197,21 +197,21 @@ __device__ __forceinline__ void finish_rows(const GemmParams& p, const uint32_t 
         }
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += bias;
+    for (int j = 0; j < N; ++j) v[j] += bias;
     if (p.act == kActRelu) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
+        for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
     } else if (p.act == kActSilu) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = mul_sigmoid(v[j], v[j]);
+        for (int j = 0; j < N; ++j) v[j] = mul_sigmoid(v[j], v[j]);
     }
     if (p.scale != 1.0f) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] *= p.scale;
+        for (int j = 0; j < N; ++j) v[j] *= p.scale;
     }
-    if (p.c_type == kQ4F32) store_rows<float>(p, v, row, n);
-    else if (p.c_type == kQ4BF16) store_rows<__nv_bfloat16>(p, v, row, n);
-    else store_rows<__half>(p, v, row, n);
+    if (p.c_type == kQ4F32) store_rows<float, N>(p, v, row, n);
+    else if (p.c_type == kQ4BF16) store_rows<__nv_bfloat16, N>(p, v, row, n);
+    else store_rows<__half, N>(p, v, row, n);
 }
 
 // One dequantizing warp's whole work: 32 of the CTA's 128 outputs.
@@ -226,7 +226,7 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
     const uint32_t row = static_cast<uint32_t>((dw * 32 + g) * 128);
     const uint32_t at_a = row + static_cast<uint32_t>((4 * odd + t4) ^ g) * 16;
     const uint32_t at_b = row + static_cast<uint32_t>((4 * (odd ^ 1) + t4) ^ g) * 16;
-    const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : smem_u32(full);
+    const uint32_t full0 = CG == 2 ? cluster_addr(full, cluster_rank() & ~1u) : smem_u32(full);
     const uint32_t stage0 = smem_u32(smem);
     Ring<STAGES> st;
     Ring<kCodeStages> cs;
@@ -289,6 +289,7 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
     constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
     constexpr int kSteps = 8 / PER_CHUNK;  // K = 16 instructions to a group
     const bool issuer = elect_one();
+    const uint16_t both = CG == 2 ? static_cast<uint16_t>(3u << cluster_rank()) : 0;  // this rank is the pair's first
     Ring<S::kStages> st;
     Ring<S::kBufs> acc;
     const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + 2 * kAHalf);
@@ -316,13 +317,13 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
                         }
                     }
                     if (CG == 1) mma_commit(&acc_full[acc.at]);
-                    else commit_both(&acc_full[acc.at]);
+                    else commit_both(&acc_full[acc.at], both);
                 }
                 acc.next();
             }
             if (issuer) {
                 if (CG == 1) mma_commit(&empty[st.at]);
-                else commit_both(&empty[st.at]);
+                else commit_both(&empty[st.at], both);
             }
             st.next();
         }
@@ -330,7 +331,9 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
     return true;
 }
 
-template <bool BF16, int P, int BN, int CG>
+// SPLIT: the CTAs or pairs of a cluster share a tile's inputs (apart, since the exchange's code costs the
+// adding warps registers: prompt of 4096 rows, groups of 32, 588 us with it, 470 without).
+template <bool BF16, int P, int BN, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     using S = Shape<P, BN, CG>;
@@ -348,12 +351,12 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    // A cluster is a pair (CG = 2) or the CTAs that share a tile's inputs.
-    const int splits = CG == 2 ? 1 : p.splits;
-    const uint32_t rank = CG == 2 || splits > 1 ? cluster_rank() : 0;
-    const int pair = CG == 2 ? static_cast<int>(rank) : 0;  // this CTA's 128 of the tile's outputs
+    // A cluster is the CTAs, or pairs of neighbouring ranks (CG = 2), that share a tile's inputs.
+    const int splits = SPLIT ? p.splits : 1;
+    const uint32_t rank = CG == 2 || SPLIT ? cluster_rank() : 0, first_rank = CG == 2 ? rank & ~1u : rank;
+    const int pair = static_cast<int>(rank - first_rank);  // this CTA's 128 of the tile's outputs
     const bool leader = pair == 0;
-    const int split = splits > 1 ? static_cast<int>(rank) : 0;
+    const int split = static_cast<int>(rank) / CG;
     const int first = blockIdx.x / (CG * splits), stride = gridDim.x / (CG * splits);
     const int c0 = split * p.split_chunks, c1 = min(p.chunks, c0 + p.split_chunks);
     const int per_chunk = p.per_chunk;
@@ -402,7 +405,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                     if (!(ok = wait_for(&empty[st.at], st.phase ^ 1))) break;
                     uint8_t* b = smem + st.at * S::kStageBytes + 2 * kAHalf;
                     // Both CTAs' loads of a pair count on the first CTA's barrier, which expects them all.
-                    const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], 0) : 0;
+                    const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], first_rank) : 0;
                     if (leader) mbar_arrive_expect_tx(&full[st.at], CG * P * 2 * S::kBHalf);
 #pragma unroll
                     for (int i = 0; i < 2 * P; ++i) {  // plane i / 2, inputs 64 (i % 2) ..
@@ -458,7 +461,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
         const int quad = warp & 3, half = (warp - 8) / 4;
         const int lane_row = quad * 32 + lane;
         Ring<S::kBufs> ab;
-        const uint32_t acc_empty0 = CG == 2 ? cluster_addr(&acc_empty[0], 0) : 0;
+        const uint32_t acc_empty0 = CG == 2 ? cluster_addr(&acc_empty[0], first_rank) : 0;
         for (int t = first; t < p.tiles; t += stride) {
             const int m0 = t / p.num_n * BN + half * kCols;
             const int n = (t % p.num_n * CG + pair) * 128 + lane_row;
@@ -523,72 +526,78 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
             }
             if (!ok) {
                 gave_up(p, abort_flag);
-                if (splits > 1) {
+                if (SPLIT) {
                     cluster_meet();
                     cluster_meet();
                 }
                 break;
             }
             const float bias = p.bias && n_ok ? __ldg(p.bias + n) : 0.0f;
-            if (CG == 2 || splits == 1) {
-                // The sums go back to the last accumulator's columns, from where a rolled loop can take
-                // them (registers cannot be indexed): the epilogue's code stays small. Unrolled over
-                // all columns it kept the instruction cache busy (1500 rows, 1024 -> 4096: 89 us).
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                                       static_cast<uint32_t>(ab.at * BN + half * kCols);
+            // The sums go back to the last accumulator's columns, from where rolled loops can take them
+            // (registers cannot be indexed): code that runs once a tile stays small. Its fetching is what
+            // short products wait for (unrolled over the columns: 1500 rows, 1024 -> 4096: 89 us; 256 rows on pairs
+            // split in four: 41 us).
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                                   static_cast<uint32_t>(ab.at * BN + half * kCols);
 #pragma unroll
-                for (int q = 0; q < kCols / 32; ++q) {
-                    uint32_t r[32];
+            for (int q = 0; q < kCols / 32; ++q) {
+                uint32_t r[32];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    r[2 * j] = static_cast<uint32_t>(acc[q * 16 + j]);
+                    r[2 * j + 1] = static_cast<uint32_t>(acc[q * 16 + j] >> 32);
+                }
+                tmem_st32(taddr + q * 32, r);
+            }
+            tmem_st_wait();
+            // The CTAs that share a tile each finish a slice of its rows: every one sends its sums of a slice to
+            // the slice's CTA, which adds them in rank order. The stages are free: all of a CTA's products
+            // have been added up, here and, after the meeting, in the others.
+            const int slice = kCols / splits, log = __ffs(slice) - 1;
+            if (SPLIT) cluster_meet();
+#pragma unroll 1
+            for (int q = 0; q < kCols / 16; ++q) {
+                const int row = m0 + q * 16;
+                if (row >= p.m) break;
+                uint32_t r[16];
+                tmem_ld16(taddr + q * 16, r);
+                tmem_ld_wait();
+                if (!SPLIT) {
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                    if (n_ok) finish_rows<P, 16>(p, v, row, n, bias);
+                } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        r[2 * j] = static_cast<uint32_t>(acc[q * 16 + j]);
-                        r[2 * j + 1] = static_cast<uint32_t>(acc[q * 16 + j] >> 32);
+                        const int col = q * 16 + j;
+                        const uint32_t to = cluster_addr(smem, static_cast<uint32_t>((col >> log) * CG + pair));
+                        const int at = ((split * 2 + half) * slice + (col & (slice - 1))) * 128 + lane_row;
+                        st_cluster_f32(to + static_cast<uint32_t>(at * 4), __uint_as_float(r[j]));
                     }
-                    tmem_st32(taddr + q * 32, r);
                 }
-                tmem_st_wait();
-#pragma unroll 1
-                for (int q = 0; q < kCols / 16; ++q) {
-                    const int row = m0 + q * 16;
-                    if (row >= p.m) break;
-                    uint32_t r[16];
-                    tmem_ld16(taddr + q * 16, r);
-                    tmem_ld_wait();
-                    if (n_ok) finish_rows<P>(p, r, row, n, bias);
-                    __syncwarp();
-                }
+                __syncwarp();
+            }
+            if (!SPLIT) {
                 release();
                 continue;
             }
-            // The tile's CTAs each finish a slice of its rows: every CTA sends its sums of a slice to the
-            // slice's CTA, which adds them in rank order. The stages are free: all of a CTA's products
-            // have been added up, here and, after the barrier, in the others.
-            const int slice = kCols / splits, log = __ffs(slice) - 1;
-            cluster_meet();
-#pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-                const float2 pair_v = unpack_f2(acc[j / 2]);
-                const uint32_t to = cluster_addr(smem, static_cast<uint32_t>(j >> log));
-                st_cluster_f32(to + static_cast<uint32_t>((((split * 2 + half) * slice + (j & (slice - 1))) * 128 + lane_row) * 4),
-                               j % 2 ? pair_v.y : pair_v.x);
-            }
             cluster_meet();
             const float* parts = reinterpret_cast<const float*>(smem);
-            for (int j = 0; j < slice; ++j) {
+#pragma unroll 1
+            for (int j = 0; j < slice; j += 4) {  // a slice is four rows or more
                 const int row = m0 + split * slice + j;
                 if (row >= p.m || !n_ok) break;
-                float v = 0.0f;
-                for (int q = 0; q < splits; ++q) v += parts[((q * 2 + half) * slice + j) * 128 + lane_row];
-                if (P == 2) v *= __ldg(p.row_scale + row);
-                v = q4_act(v + bias, p.act) * p.scale;
-                const int64_t at = static_cast<int64_t>(row) * p.ldc + n;
-                if (p.accumulate) v += q4_load(p.c, p.c_type, at);
-                q4_store(p.c, p.c_type, at, v);
+                float v[4] = {};
+                for (int q = 0; q < splits; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] += parts[((q * 2 + half) * slice + j + i) * 128 + lane_row];
+                finish_rows<P, 4>(p, v, row, n, bias);
             }
         }
     }
 
-    if (CG == 1 && splits > 1 && warp < 8) {
+    if (SPLIT && warp < 8) {
         // The two meetings of the adding warps' exchange, which count every thread of the cluster.
         cluster_meet();
         cluster_meet();
@@ -644,19 +653,60 @@ __global__ void __launch_bounds__(kPrepThreads) q4_align_kernel(const uint16_t* 
     for (int i = threadIdx.x; i < ld; i += kPrepThreads) out[row * ld + i] = i < k ? __ldg(a + row * lda + i) : uint16_t(0);
 }
 
-template <bool BF16, int P, int BN, int CG>
-cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, int sms, cudaStream_t stream) {
+// A launch of the kernel with clusters of `cluster` CTAs.
+struct Launch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    Launch(int cluster, unsigned grid, size_t smem, cudaStream_t stream) {
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster > 1 ? 1 : 0;
+    }
+};
+
+// How many clusters of 1, 2, 4 or 8 CTAs the device runs at once (fewer than its SMs would hold: a cluster
+// stays within a GPC; 15 of eight CTAs on 148 SMs). Asked once per device, with the kernel's attributes set.
+template <bool BF16, int P, int BN, int CG, bool SPLIT>
+cudaError_t clusters_at_once(int cluster, int sms, int* count) {
     using S = Shape<P, BN, CG>;
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices][4];
     static DeviceOnce once;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const auto kernel = q4_gemm_kernel<BF16, P, BN, CG, SPLIT>;
     if (!once.done(dev)) {
-        if ((e = cudaFuncSetAttribute(q4_gemm_kernel<BF16, P, BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      S::kSmemBytes)) != cudaSuccess)
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes)) != cudaSuccess)
             return e;
         once.mark(dev);
     }
+    const int at = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+    int n = dev < kDevices ? known[dev][at].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        if (cluster == 1) {
+            n = sms;
+        } else {
+            const Launch l(cluster, static_cast<unsigned>(cluster), S::kSmemBytes, nullptr);
+            if ((e = cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg)) != cudaSuccess) return e;
+            n = std::max(n, 1);
+        }
+        if (dev < kDevices) known[dev][at].store(n, std::memory_order_relaxed);
+    }
+    *count = n;
+    return cudaSuccess;
+}
+
+template <bool BF16, int P, int BN, int CG, bool SPLIT>
+cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, int at_once, cudaStream_t stream) {
+    using S = Shape<P, BN, CG>;
     CUtensorMap map;
     if (!encode_map_2d(&map, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a,
                        static_cast<uint64_t>(p.k), static_cast<uint64_t>(p.m) * P, static_cast<uint64_t>(lda) * 2, kHalfK,
@@ -669,33 +719,60 @@ cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, in
     p.splits = splits;
     p.split_chunks = (p.chunks + splits - 1) / splits;
     const int cluster = CG * splits;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(cluster * std::min(p.tiles, splits > 1 ? p.tiles : sms / CG)));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = S::kSmemBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, q4_gemm_kernel<BF16, P, BN, CG>, map, p);
+    const Launch l(cluster, static_cast<unsigned>(cluster * (splits > 1 ? p.tiles : std::min(p.tiles, at_once))), S::kSmemBytes,
+                   stream);
+    return cudaLaunchKernelEx(&l.cfg, q4_gemm_kernel<BF16, P, BN, CG, SPLIT>, map, p);
 }
 
+template <int BN, bool SPLIT>
+struct Kernel {
+    static constexpr int kBN = BN, kCG = BN == 256 ? 2 : 1;
+    static constexpr bool kSplit = SPLIT;
+};
+
+// Calls f with the kernel's constants.
+template <bool BF16, int P, typename F>
+cudaError_t with_shape(int bn, int splits, F f) {
+    if (splits > 1) return bn == 256 ? f(Kernel<256, true>()) : bn == 128 ? f(Kernel<128, true>()) : f(Kernel<64, true>());
+    return bn == 256 ? f(Kernel<256, false>()) : bn == 128 ? f(Kernel<128, false>()) : f(Kernel<64, false>());
+}
+
+// The tile and the number of CTAs or pairs that share its inputs. A CTA's time is its chunks', nearly
+// whatever its tile's rows, since taking 128 outputs' codes apart is what a chunk waits for (about 1450
+// cycles; with two planes 256 rows on a pair take 2300 for the products): so the fewest rounds of
+// chunks win, of larger tiles that are not filled, smaller ones that take the codes apart again, and tiles
+// split among CTAs that exchange their sums.
 template <bool BF16, int P>
 cudaError_t launch_shape(const void* a, int64_t lda, const GemmParams& p, int sms, cudaStream_t stream) {
-    // Pairs on 256 x 256 tiles where they fill the GPU, else smaller tiles on single CTAs, and where
-    // those leave SMs idle clusters of up to eight CTAs that share a tile's inputs.
-    const auto tiles = [&](int bn, int features) {
-        return static_cast<int64_t>((p.m + bn - 1) / bn) * ((p.n + features - 1) / features);
-    };
-    if (tiles(256, 256) * 2 >= sms) return launch_gemm<BF16, P, 256, 2>(a, lda, p, 1, sms, stream);
-    if (tiles(128, 128) >= sms) return launch_gemm<BF16, P, 128, 1>(a, lda, p, 1, sms, stream);
-    int splits = 1;
-    while (splits < 8 && tiles(64, 128) * splits * 2 <= sms && splits * 4 <= p.chunks) splits *= 2;
-    return launch_gemm<BF16, P, 64, 1>(a, lda, p, splits, sms, stream);
+    int best_bn = 0, best_splits = 1, best_at_once = 1;
+    double best = 0.0;
+    for (const int bn : {64, 128, 256}) {
+        const int cg = bn == 256 ? 2 : 1;
+        const double tiles = static_cast<double>((p.m + bn - 1) / bn) * ((p.n + cg * 128 - 1) / (cg * 128));
+        for (int splits = 1; splits * cg <= 8 && (splits == 1 || p.chunks >= 2 * splits); splits *= 2) {
+            int at_once = 0;
+            const cudaError_t e = with_shape<BF16, P>(bn, splits, [&](auto shape) {
+                using K = decltype(shape);
+                return clusters_at_once<BF16, P, K::kBN, K::kCG, K::kSplit>(cg * splits, sms, &at_once);
+            });
+            if (e != cudaSuccess) return e;
+            const double chunk = P == 2 && bn == 256 ? 2300.0 : 1450.0;
+            // A first chunk's way through the roles, the epilogue, and the exchange of sums.
+            const double tile = 4000.0 + ((p.chunks + splits - 1) / splits) * chunk + bn * 10.0 / splits +
+                                (splits > 1 ? 4500.0 + bn * 25.0 : 0.0);
+            const double time = std::ceil(tiles / at_once) * tile;
+            if (best_bn == 0 || time < best) {
+                best = time;
+                best_bn = bn;
+                best_splits = splits;
+                best_at_once = at_once;
+            }
+        }
+    }
+    return with_shape<BF16, P>(best_bn, best_splits, [&](auto shape) {
+        using K = decltype(shape);
+        return launch_gemm<BF16, P, K::kBN, K::kCG, K::kSplit>(a, lda, p, best_splits, best_at_once, stream);
+    });
 }
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
