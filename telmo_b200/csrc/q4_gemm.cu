@@ -47,7 +47,7 @@ constexpr int kHalfK = 64;                    // inputs of one 128-byte swizzled
 constexpr int kAHalf = 128 * kHalfK * 2;      // one CTA's A tile of 64 inputs
 constexpr int kCodeBytes = 128 * 64;          // the codes of 128 outputs and one 128-input chunk
 constexpr int kCodeStage = kCodeBytes + 512;  // and their zero points
-constexpr int kCodeStages = 3;
+constexpr int kCodeStages = 4;
 constexpr int kDrainWarps = 8;
 constexpr int kDequantWarps = 4;
 constexpr int kStageBudget = 192 << 10;
@@ -60,7 +60,7 @@ struct Shape {
     static constexpr int kStages = std::min(4, kStageBudget / kStageBytes);
     static constexpr int kBufs = std::min(4, 512 / BN);  // accumulators in TMEM
     static constexpr int kTmemCols = kBufs * BN;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kCodeStages * kCodeStage + 1024 + 512;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kCodeStages * kCodeStage + 512;
 };
 
 struct GemmParams {
@@ -339,7 +339,11 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     using S = Shape<P, BN, CG>;
     constexpr int kCols = BN / 2;  // activation rows per adding thread
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem = smem_raw;
+    if (smem_u32(smem) % 1024 != 0) {  // the declaration's alignment, which the swizzled tiles rely on
+        if (threadIdx.x == 0 && p.error) atomicCAS(p.error, 0u, static_cast<uint32_t>(kErrWaitTimeout));
+        return;
+    }
     uint8_t* code_ring = smem + S::kStages * S::kStageBytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(code_ring + kCodeStages * kCodeStage);
     uint64_t* empty = full + S::kStages;
