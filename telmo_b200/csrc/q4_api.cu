@@ -21,6 +21,17 @@ float f16_value(float x) {
     return std::isfinite(h) ? h : std::nanf("");
 }
 
+// Whether x is a finite f16 value: 11 significant bits from 2^15 down to multiples of 2^-24.
+bool is_f16(float x) {
+    uint32_t u;
+    std::memcpy(&u, &x, 4);
+    const int e = static_cast<int>((u >> 23) & 255) - 127;
+    if ((u << 1) == 0) return true;
+    if (e > 15 || e < -24) return false;
+    const int dropped = e < -14 ? 13 + (-14 - e) : 13;
+    return (u & ((1u << dropped) - 1)) == 0;
+}
+
 void free_q4(Q4Weights* q) {
     if (!q) return;
     if (q->codes) cudaFree(q->codes);
@@ -45,7 +56,7 @@ int upload_q4(Ctx* ctx, size_t n, size_t k, size_t group, const uint8_t* codes, 
               const uint8_t* zeros, Weights* w) {
     const size_t groups = (k + group - 1) / group, rows = (n + 127) / 128 * 128, chunks = (k + 127) / 128;
     for (size_t i = 0; i < n * groups; ++i)
-        if (!(scales[i] == f16_value(scales[i])))
+        if (!is_f16(scales[i]))
             return ctx->fail(TELMO_ERR_ARGUMENT,
                              "telmo_weights_upload_q4: scale %zu (%g) is not a finite f16 value", i,
                              static_cast<double>(scales[i]));

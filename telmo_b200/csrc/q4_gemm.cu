@@ -59,7 +59,7 @@ struct Shape {
     static constexpr int kStageBytes = 2 * kAHalf + 2 * P * kBHalf;
     static constexpr int kStages = std::min(4, kStageBudget / kStageBytes);
     static constexpr int kBufs = std::min(4, 512 / BN);  // accumulators in TMEM
-    static constexpr int kTmemCols = kBufs * BN;
+    static constexpr int kTmemCols = BN == 192 ? 512 : kBufs * BN;  // a power of two
     static constexpr int kSmemBytes = kStages * kStageBytes + kCodeStages * kCodeStage + 512;
 };
 
@@ -79,7 +79,7 @@ struct GemmParams {
     int c_type;
     int64_t ldc;
     int tiles, num_n;
-    int splits;        // CTAs or pairs of one cluster that share a tile's inputs
+    int splits;        // CTAs of one cluster that share a tile's inputs
     int split_chunks;  // chunks of each
     uint32_t* error;
 };
@@ -138,12 +138,11 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
-// Arrives on the same barrier of both CTAs of the pair (the bits of their ranks: `both`) once this thread's
-// products are complete.
-__device__ __forceinline__ void commit_both(uint64_t* bar, uint16_t both) {
+// Arrives on the same barrier of both CTAs of the pair once this thread's products are complete.
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(smem_u32(bar)), "h"(both) : "memory");
+        ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
 // A ring position and its phase.
@@ -226,7 +225,7 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
     const uint32_t row = static_cast<uint32_t>((dw * 32 + g) * 128);
     const uint32_t at_a = row + static_cast<uint32_t>((4 * odd + t4) ^ g) * 16;
     const uint32_t at_b = row + static_cast<uint32_t>((4 * (odd ^ 1) + t4) ^ g) * 16;
-    const uint32_t full0 = CG == 2 ? cluster_addr(full, cluster_rank() & ~1u) : smem_u32(full);
+    const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : smem_u32(full);
     const uint32_t stage0 = smem_u32(smem);
     Ring<STAGES> st;
     Ring<kCodeStages> cs;
@@ -289,7 +288,6 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
     constexpr uint32_t idesc = idesc_f16(CG * 128, BN, false) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
     constexpr int kSteps = 8 / PER_CHUNK;  // K = 16 instructions to a group
     const bool issuer = elect_one();
-    const uint16_t both = CG == 2 ? static_cast<uint16_t>(3u << cluster_rank()) : 0;  // this rank is the pair's first
     Ring<S::kStages> st;
     Ring<S::kBufs> acc;
     const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + 2 * kAHalf);
@@ -317,13 +315,13 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
                         }
                     }
                     if (CG == 1) mma_commit(&acc_full[acc.at]);
-                    else commit_both(&acc_full[acc.at], both);
+                    else commit_both(&acc_full[acc.at]);
                 }
                 acc.next();
             }
             if (issuer) {
                 if (CG == 1) mma_commit(&empty[st.at]);
-                else commit_both(&empty[st.at], both);
+                else commit_both(&empty[st.at]);
             }
             st.next();
         }
@@ -331,7 +329,7 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
     return true;
 }
 
-// SPLIT: the CTAs or pairs of a cluster share a tile's inputs (apart, since the exchange's code costs the
+// SPLIT: the CTAs of a cluster share a tile's inputs (a kernel of its own, since the exchange's code costs the
 // adding warps registers: prompt of 4096 rows, groups of 32, 588 us with it, 470 without).
 template <bool BF16, int P, int BN, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -355,12 +353,13 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    // A cluster is the CTAs, or pairs of neighbouring ranks (CG = 2), that share a tile's inputs.
+    // A cluster is a pair (CG = 2) or the CTAs that share a tile's inputs (SPLIT).
+    static_assert(CG == 1 || !SPLIT, "pairs do not share inputs");
     const int splits = SPLIT ? p.splits : 1;
-    const uint32_t rank = CG == 2 || SPLIT ? cluster_rank() : 0, first_rank = CG == 2 ? rank & ~1u : rank;
-    const int pair = static_cast<int>(rank - first_rank);  // this CTA's 128 of the tile's outputs
+    const uint32_t rank = CG == 2 || SPLIT ? cluster_rank() : 0;
+    const int pair = CG == 2 ? static_cast<int>(rank) : 0;  // this CTA's 128 of the tile's outputs
     const bool leader = pair == 0;
-    const int split = static_cast<int>(rank) / CG;
+    const int split = SPLIT ? static_cast<int>(rank) : 0;
     const int first = blockIdx.x / (CG * splits), stride = gridDim.x / (CG * splits);
     const int c0 = split * p.split_chunks, c1 = min(p.chunks, c0 + p.split_chunks);
     const int per_chunk = p.per_chunk;
@@ -409,7 +408,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                     if (!(ok = wait_for(&empty[st.at], st.phase ^ 1))) break;
                     uint8_t* b = smem + st.at * S::kStageBytes + 2 * kAHalf;
                     // Both CTAs' loads of a pair count on the first CTA's barrier, which expects them all.
-                    const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], first_rank) : 0;
+                    const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], 0) : 0;
                     if (leader) mbar_arrive_expect_tx(&full[st.at], CG * P * 2 * S::kBHalf);
 #pragma unroll
                     for (int i = 0; i < 2 * P; ++i) {  // plane i / 2, inputs 64 (i % 2) ..
@@ -465,7 +464,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
         const int quad = warp & 3, half = (warp - 8) / 4;
         const int lane_row = quad * 32 + lane;
         Ring<S::kBufs> ab;
-        const uint32_t acc_empty0 = CG == 2 ? cluster_addr(&acc_empty[0], first_rank) : 0;
+        const uint32_t acc_empty0 = CG == 2 ? cluster_addr(&acc_empty[0], 0) : 0;
         for (int t = first; t < p.tiles; t += stride) {
             const int m0 = t / p.num_n * BN + half * kCols;
             const int n = (t % p.num_n * CG + pair) * 128 + lane_row;
@@ -575,7 +574,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const int col = q * 16 + j;
-                        const uint32_t to = cluster_addr(smem, static_cast<uint32_t>((col >> log) * CG + pair));
+                        const uint32_t to = cluster_addr(smem, static_cast<uint32_t>(col >> log));
                         const int at = ((split * 2 + half) * slice + (col & (slice - 1))) * 128 + lane_row;
                         st_cluster_f32(to + static_cast<uint32_t>(at * 4), __uint_as_float(r[j]));
                     }
@@ -618,22 +617,43 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     }
 }
 
-// The rows of a as the products read them: one block per row. f32: two fp16 planes and the row's
-// power of two. 16-bit types: a copy with rows that start on 16-byte boundaries.
-constexpr int kPrepThreads = 256;
+// The rows of a as the products read them. f32: two fp16 planes and the row's power of two, one block per
+// row, which keeps the row's first values in registers between looking for the largest and splitting.
+// 16-bit types: a copy with rows that start on 16-byte boundaries, 2048 values a block. (With few rows
+// these wait for loads alone: 24 rows of 11009 took 14 us in one block of 256 threads a row, a value at a time.)
+constexpr int kKeep = 4;  // fours of values a thread keeps
 
-__global__ void __launch_bounds__(kPrepThreads) q4_split_kernel(const float* a, int64_t lda, int m, int k, __half* planes,
-                                                                int64_t ld, float* row_scale) {
+__device__ __forceinline__ float4 load_four(const float* row, int i, int k, bool vec) {
+    if (vec && i + 4 <= k) return __ldg(reinterpret_cast<const float4*>(row + i));
+    float4 v;
+    v.x = i < k ? __ldg(row + i) : 0.0f;
+    v.y = i + 1 < k ? __ldg(row + i + 1) : 0.0f;
+    v.z = i + 2 < k ? __ldg(row + i + 2) : 0.0f;
+    v.w = i + 3 < k ? __ldg(row + i + 3) : 0.0f;
+    return v;
+}
+
+__global__ void __launch_bounds__(1024) q4_split_kernel(const float* a, int64_t lda, int m, int k, bool vec, __half* planes,
+                                                        int64_t ld, float* row_scale) {
     const int64_t row = blockIdx.x;
     const float* src = a + row * lda;
-    __shared__ float tops[kPrepThreads / 32];
+    const int step = static_cast<int>(blockDim.x) * 4, i0 = static_cast<int>(threadIdx.x) * 4;
+    __shared__ float tops[32];
+    float4 kept[kKeep];
     float top = 0.0f;  // fmaxf passes NaNs over
-    for (int i = threadIdx.x; i < k; i += kPrepThreads) top = fmaxf(top, fabsf(__ldg(src + i)));
+    const auto look = [&](const float4& v) {
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    };
+#pragma unroll
+    for (int q = 0; q < kKeep; ++q) kept[q] = load_four(src, i0 + q * step, k, vec);
+#pragma unroll
+    for (int q = 0; q < kKeep; ++q) look(kept[q]);
+    for (int i = i0 + kKeep * step; i < k; i += step) look(load_four(src, i, k, vec));
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
     __syncthreads();
-    for (int w = 0; w < kPrepThreads / 32; ++w) top = fmaxf(top, tops[w]);
+    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) top = fmaxf(top, tops[w]);
     // 2^e with the largest value 2^e times a number in [2^14, 2^15). e stops at -126, so that 2^-e
     // stays a normal f32: a row below 2^-112 keeps its values to 2^-150. An infinity's exponent makes e
     // 114, which holds every finite value below 2^14 and leaves the infinity one.
@@ -643,18 +663,40 @@ __global__ void __launch_bounds__(kPrepThreads) q4_split_kernel(const float* a, 
     if (threadIdx.x == 0) row_scale[row] = up;
     __half* hi = planes + row * ld;
     __half* lo = hi + static_cast<int64_t>(m) * ld;
-    for (int i = threadIdx.x; i < ld; i += kPrepThreads) {
-        const float x = i < k ? __ldg(src + i) * down : 0.0f;
-        const __half h = __float2half_rn(x);
-        hi[i] = h;
-        lo[i] = __float2half_rn(x - __half2float(h));
-    }
+    const auto write = [&](const float4& v, int i) {  // ld is a multiple of 8: whole fours
+        if (i >= ld) return;
+        const float x[4] = {v.x * down, v.y * down, v.z * down, v.w * down};
+        __half h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h[j] = __float2half_rn(x[j]);
+            l[j] = __float2half_rn(x[j] - __half2float(h[j]));
+        }
+        *reinterpret_cast<uint2*>(hi + i) = *reinterpret_cast<const uint2*>(h);
+        *reinterpret_cast<uint2*>(lo + i) = *reinterpret_cast<const uint2*>(l);
+    };
+#pragma unroll
+    for (int q = 0; q < kKeep; ++q) write(kept[q], i0 + q * step);
+    for (int i = i0 + kKeep * step; i < ld; i += step) write(load_four(src, i, k, vec), i);
 }
 
-__global__ void __launch_bounds__(kPrepThreads) q4_align_kernel(const uint16_t* a, int64_t lda, int k, uint16_t* out,
-                                                                int64_t ld) {
+constexpr int kAlignThreads = 256, kAlignValues = 2048;
+
+__global__ void __launch_bounds__(kAlignThreads) q4_align_kernel(const uint16_t* a, int64_t lda, int k, uint16_t* out,
+                                                                 int64_t ld) {
     const int64_t row = blockIdx.x;
-    for (int i = threadIdx.x; i < ld; i += kPrepThreads) out[row * ld + i] = i < k ? __ldg(a + row * lda + i) : uint16_t(0);
+    const int base = blockIdx.y * kAlignValues + threadIdx.x;
+    uint16_t v[kAlignValues / kAlignThreads];
+#pragma unroll
+    for (int j = 0; j < kAlignValues / kAlignThreads; ++j) {
+        const int i = base + j * kAlignThreads;
+        v[j] = i < k ? __ldg(a + row * lda + i) : uint16_t(0);
+    }
+#pragma unroll
+    for (int j = 0; j < kAlignValues / kAlignThreads; ++j) {
+        const int i = base + j * kAlignThreads;
+        if (i < ld) out[row * ld + i] = v[j];
+    }
 }
 
 // A launch of the kernel with clusters of `cluster` CTAs.
@@ -730,37 +772,44 @@ cudaError_t launch_gemm(const void* a, int64_t lda, GemmParams p, int splits, in
 
 template <int BN, bool SPLIT>
 struct Kernel {
-    static constexpr int kBN = BN, kCG = BN == 256 ? 2 : 1;
+    static constexpr int kBN = BN, kCG = BN >= 192 ? 2 : 1;
     static constexpr bool kSplit = SPLIT;
 };
 
 // Calls f with the kernel's constants.
 template <bool BF16, int P, typename F>
 cudaError_t with_shape(int bn, int splits, F f) {
-    if (splits > 1) return bn == 256 ? f(Kernel<256, true>()) : bn == 128 ? f(Kernel<128, true>()) : f(Kernel<64, true>());
-    return bn == 256 ? f(Kernel<256, false>()) : bn == 128 ? f(Kernel<128, false>()) : f(Kernel<64, false>());
+    if (splits > 1) return bn == 128 ? f(Kernel<128, true>()) : f(Kernel<64, true>());
+    return bn == 256   ? f(Kernel<256, false>())
+           : bn == 192 ? f(Kernel<192, false>())
+           : bn == 128 ? f(Kernel<128, false>())
+                       : f(Kernel<64, false>());
 }
 
-// The tile and the number of CTAs or pairs that share its inputs. A CTA's time is its chunks', nearly
-// whatever its tile's rows, since taking 128 outputs' codes apart is what a chunk waits for (about 1450
-// cycles; with two planes 256 rows on a pair take 2300 for the products): so the fewest rounds of
-// chunks win, of larger tiles that are not filled, smaller ones that take the codes apart again, and tiles
-// split among CTAs that exchange their sums.
+// The tile and the number of CTAs that share its inputs. Up to 192 rows a chunk's time is that of
+// taking 128 outputs' codes apart, about 1450 cycles whatever the rows (so larger tiles win even where they are
+// not filled, and tiles split among CTAs that exchange their sums, before the codes are taken apart again);
+// then it is the products', and with two planes from 128 rows on the activations' way from L2. Pairs do not
+// share inputs: their exchange of 128 KB a CTA cost more than it saved (200 rows, 4096 -> 8192: 40 us split in two,
+// 33 whole). The rounds of
+// tiles over the GPU count too: 1500 rows of f32, 1024 -> 4096, are 96 tiles of 256 rows on 74 pairs (42 us) or 128
+// of 192 (35 us).
 template <bool BF16, int P>
 cudaError_t launch_shape(const void* a, int64_t lda, const GemmParams& p, int sms, cudaStream_t stream) {
     int best_bn = 0, best_splits = 1, best_at_once = 1;
     double best = 0.0;
-    for (const int bn : {64, 128, 256}) {
-        const int cg = bn == 256 ? 2 : 1;
+    for (const int bn : {64, 128, 192, 256}) {
+        const int cg = bn >= 192 ? 2 : 1;
         const double tiles = static_cast<double>((p.m + bn - 1) / bn) * ((p.n + cg * 128 - 1) / (cg * 128));
-        for (int splits = 1; splits * cg <= 8 && (splits == 1 || p.chunks >= 2 * splits); splits *= 2) {
+        const int most_splits = cg == 2 ? 1 : 8;
+        for (int splits = 1; splits <= most_splits && (splits == 1 || p.chunks >= 2 * splits); splits *= 2) {
             int at_once = 0;
             const cudaError_t e = with_shape<BF16, P>(bn, splits, [&](auto shape) {
                 using K = decltype(shape);
                 return clusters_at_once<BF16, P, K::kBN, K::kCG, K::kSplit>(cg * splits, sms, &at_once);
             });
             if (e != cudaSuccess) return e;
-            const double chunk = P == 2 && bn == 256 ? 2300.0 : 1450.0;
+            const double chunk = P == 2 ? (bn == 64 ? 1700.0 : bn < 256 ? 2400.0 : 3200.0) : (bn < 256 ? 1450.0 : 1700.0);
             // A first chunk's way through the roles, the epilogue, and the exchange of sums.
             const double tile = 4000.0 + ((p.chunks + splits - 1) / splits) * chunk + bn * 10.0 / splits +
                                 (splits > 1 ? 4500.0 + bn * 25.0 : 0.0);
@@ -797,11 +846,13 @@ cudaError_t q4_make_planes(const Q4Args& g, void* workspace, Q4Planes* planes, c
         float* rs = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                              round_up(2 * static_cast<size_t>(g.m) * ld * sizeof(__half), 256));
         planes->row_scale = rs;
-        q4_split_kernel<<<g.m, kPrepThreads, 0, stream>>>(static_cast<const float*>(g.a), g.lda, g.m, g.w->k,
-                                                          static_cast<__half*>(workspace), ld, rs);
+        const int threads = std::min<int>(1024, static_cast<int>(round_up((static_cast<size_t>(g.w->k) + 7) / 8, 32)));
+        q4_split_kernel<<<g.m, threads, 0, stream>>>(static_cast<const float*>(g.a), g.lda, g.m, g.w->k, q4_rows_aligned(g),
+                                                     static_cast<__half*>(workspace), ld, rs);
     } else {
-        q4_align_kernel<<<g.m, kPrepThreads, 0, stream>>>(static_cast<const uint16_t*>(g.a), g.lda, g.w->k,
-                                                          static_cast<uint16_t*>(workspace), ld);
+        const dim3 grid(g.m, static_cast<unsigned>((ld + kAlignValues - 1) / kAlignValues));
+        q4_align_kernel<<<grid, kAlignThreads, 0, stream>>>(static_cast<const uint16_t*>(g.a), g.lda, g.w->k,
+                                                            static_cast<uint16_t*>(workspace), ld);
     }
     return cudaGetLastError();
 }
