@@ -52,6 +52,20 @@ struct Staged {
     }
 };
 
+// Workspaces come in stream order from the context's own pool: calls on several streams and captured graphs
+// each have their own, and a graph keeps its own while it lives. The pool is made with the first weights, so
+// that a product can be a capture's first call.
+int make_pool(Ctx* ctx) {
+    if (ctx->pool) return TELMO_OK;
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = ctx->device;
+    if (int rc = ctx->cuda(cudaMemPoolCreate(&ctx->pool, &props), "memory pool")) return rc;
+    uint64_t keep = UINT64_MAX;  // what a call gave back stays for the next
+    return ctx->cuda(cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep), "memory pool");
+}
+
 int upload_q4(Ctx* ctx, size_t n, size_t k, size_t group, const uint8_t* codes, const float* scales,
               const uint8_t* zeros, Weights* w) {
     const size_t groups = (k + group - 1) / group, rows = (n + 127) / 128 * 128, chunks = (k + 127) / 128;
@@ -65,6 +79,7 @@ int upload_q4(Ctx* ctx, size_t n, size_t k, size_t group, const uint8_t* codes, 
             if (zeros[i] > 15)
                 return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_weights_upload_q4: zero point %zu (%d) is above 15", i,
                                  static_cast<int>(zeros[i]));
+    if (int rc = make_pool(ctx)) return rc;
     Q4Weights* q = new Q4Weights();
     w->q4 = q;
     w->dev.n = q->n = static_cast<int>(n);
@@ -143,17 +158,6 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
         return rows ? q4_linear_rows(g, planes, stream) : q4_linear_gemm(g, planes, stream);
     };
     if (!(rows ? q4_rows_planes(g) : q4_gemm_planes(g))) return ctx->cuda(product(nullptr), "telmo_linear_q4");
-    // Workspace in stream order from the context's own pool: calls on several streams and captured
-    // graphs each have their own, and a graph keeps its own while it lives.
-    if (!ctx->pool) {
-        cudaMemPoolProps props = {};
-        props.allocType = cudaMemAllocationTypePinned;
-        props.location.type = cudaMemLocationTypeDevice;
-        props.location.id = ctx->device;
-        if (int rc = ctx->cuda(cudaMemPoolCreate(&ctx->pool, &props), "telmo_linear_q4: memory pool")) return rc;
-        uint64_t keep = UINT64_MAX;  // what a call gave back stays for the next
-        cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
-    }
     void* ws = nullptr;
     if (int rc = ctx->cuda(cudaMallocFromPoolAsync(&ws, q4_planes_bytes(g), ctx->pool, stream),
                            "telmo_linear_q4: workspace"))

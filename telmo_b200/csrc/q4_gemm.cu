@@ -607,6 +607,8 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag)  // copies that were under way land before the shared memory is given back
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     // A pair's CTAs leave together: the first CTA's products read the second's shared memory and
     // write its TMEM, and the second's loads signal the first's barriers.
     if (CG == 2) cluster_sync();

@@ -260,3 +260,117 @@ def test_streams_and_graphs(ctx, m, dtype):
             assert torch.equal(y, e)
     del graphs
     dev.free()
+
+
+def test_scales_are_f16_values(ctx):
+    """Every finite f16 value is taken as a scale; its f32 neighbours are not."""
+    from telmo_b200 import PackedWeights, Precision, TelmoError
+    bits = np.arange(1 << 16, dtype=np.uint16)
+    values = bits.view(np.float16).astype(np.float32)
+    values = values[np.isfinite(values)]
+    k = 32 * values.size
+    codes = np.zeros((1, k // 2), np.uint8)
+    PackedWeights(1, k, Precision.Q4, codes, values[None, :]).upload(ctx).free()
+    some = np.concatenate([values[::3001], np.float32([2.0 ** -24, 65504.0, 2.0 ** -14, -2.0 ** -24])])
+    for v in some[some != 0]:
+        for wrong in (np.nextafter(v, np.float32(np.inf)), np.nextafter(v, np.float32(-np.inf))):
+            with pytest.raises(TelmoError):
+                PackedWeights(1, 32, Precision.Q4, codes[:, :16], np.float32([[wrong]])).upload(ctx)
+
+
+@pytest.mark.parametrize("m,dtype", [(1, "f32"), (20, "f32"), (100, "f32"), (100, "bf16")])
+def test_a_context_first_product_is_captured(m, dtype):
+    """Nothing that a capture forbids is left to a product's first call."""
+    import torch
+    from telmo_b200 import Context, Kernels
+    own = Context(0)
+    n, k = 200, 300
+    dev, w = weights(own, n, k, 32, False, 4)
+    a = torch.randn((m, k), device="cuda").to(types()[dtype])
+    c = torch.zeros((m, n), device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        Kernels(own).linear(a, m, dev, c)
+    g.replay()
+    own.check()
+    av = a.double().cpu().numpy()
+    y = av @ w.T
+    assert (np.abs(c.double().cpu().numpy() - y) <= bound(av, w, y, None, 1.0, None, 32, "f32")).all()
+    del g
+    dev.free()
+    own.close()
+
+
+@pytest.mark.parametrize("m", [1, 2, 20, 100])
+def test_long_rows(ctx, m):
+    """Inputs beyond what shared memory holds of a row's digits, and an odd number of them."""
+    run(ctx, m, 33, 30001, 128, True, "f32", "f32", seed=m)
+    run(ctx, m, 17, 20000, 32, False, "bf16", "f32", seed=m)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Rows of a and c whose offsets pass 2^31 elements, in each kernel's range of rows."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 40, 64
+    dev, w = weights(ctx, n, k, 32, False, 8)
+    for m, ld in ((2, (1 << 31) + 8), (9, (1 << 28) + 8), (33, (1 << 26) + 8)):
+        store = torch.zeros((m - 1) * ld + k, dtype=torch.bfloat16, device="cuda")
+        out = torch.zeros((m - 1) * ld + n, dtype=torch.bfloat16, device="cuda")
+        rows = torch.randn((m, k), device="cuda").bfloat16()
+        for r in range(m):
+            store[r * ld:r * ld + k] = rows[r]
+        Kernels(ctx).matmul(store, ld, m, dev, out, ld)
+        ctx.check()
+        av = rows.double().cpu().numpy()
+        y = av @ w.T
+        got = np.stack([out[r * ld:r * ld + n].double().cpu().numpy() for r in range(m)])
+        assert (np.abs(got - y) <= bound(av, w, y, None, 1.0, None, 32, "bf16")).all()
+        del store, out
+    torch.cuda.empty_cache()
+    dev.free()
+
+
+@pytest.mark.parametrize("m", [2, 24, 130, 300])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_the_same_bits_again(ctx, m, dtype):
+    """No sum depends on timing."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 1000, 2100
+    dev, _ = weights(ctx, n, k, 64, True, 2)
+    a = torch.randn((m, k), device="cuda").to(types()[dtype])
+    first, again = (torch.empty((m, n), device="cuda") for _ in range(2))
+    Kernels(ctx).linear(a, m, dev, first)
+    for _ in range(5):
+        again.zero_()
+        Kernels(ctx).linear(a, m, dev, again)
+        ctx.check()
+        assert torch.equal(first, again)
+    dev.free()
+
+
+def test_two_streams_at_once(ctx):
+    """Products on two streams whose workspaces are live at the same time."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k, m = 512, 1024, 400
+    dev, _ = weights(ctx, n, k, 64, False, 6)
+    kern = Kernels(ctx)
+    a = [torch.randn((m, k), device="cuda") for _ in range(2)]
+    want = [torch.empty((m, n), device="cuda") for _ in range(2)]
+    for x, y in zip(a, want):
+        kern.linear(x, m, dev, y)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.zeros((m, n), device="cuda") for _ in range(10)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for s in range(2):
+            kern.linear(a[s], m, dev, got[s][i], stream=streams[s])
+    torch.cuda.synchronize()
+    ctx.check()
+    for s in range(2):
+        assert all(torch.equal(y, want[s]) for y in got[s])
+    dev.free()
