@@ -19,13 +19,13 @@
 //              logit), goes through the rules and is written.
 //   choose     leaves listed tokens out by a bit map of the window; then they go through the rules and
 //              join the others.
-// A block walks over windows of 16384 tokens: it sets a bit for each listed token's place, numbers the
-// bits in order (a prefix sum over the words' counts), and counts by number in shared memory with
+// A block walks over windows of 8192 to 65536 tokens: it sets a bit for each listed token's place, numbers
+// the bits in order (a prefix sum over the words' counts), and counts by number in shared memory with
 // integer atomics (the counts do not depend on their order); a token's first entry among the biases adds
-// the others in list order. Tokens go to threads by number, so no sum depends on timing. A window with
-// more listed tokens than there are numbers goes in sections of as many places. With the rules inside
-// the pass over the logits some lane of a warp nearly always had a listed token and all paid: 92 us for 256
-// rows of 131072 bf16 values with 2000 tokens each.
+// the others in list order. Tokens go to threads by number, so no sum depends on timing. Numbers beyond
+// kNumbers come in further rounds over the lists. With the rules inside the pass over the logits some lane
+// of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16 values with
+// 2000 tokens each, which take 52 us here (93 MB read and written; the pass alone 30 us).
 //
 // The k best are found by a bound: a token's key is its value's order and then its place, so no two are
 // equal; tokens whose key is below the block's bound are passed over, others go to a buffer in
@@ -53,7 +53,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8192;                        // tokens per tile
 constexpr int kPerThread = kTile / 8 / kThreads;   // groups of eight tokens a thread has in a tile
-constexpr int kWindow = 2 * kTile;                 // tokens per window
+constexpr int kMostWindow = 8 * kTile;             // tokens per window at most
 constexpr int kNumbers = 2048;                     // listed tokens with a number
 constexpr int kMaxK = 8;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
@@ -82,6 +82,7 @@ struct RuleParams {
     float* logprobs;
     int k;
     int slices;  // blocks per row
+    int window;  // tokens per window, a multiple of kTile
 };
 
 template <typename T>
@@ -124,7 +125,8 @@ __device__ __forceinline__ int token_of(uint64_t key) { return static_cast<int>(
 
 __device__ __forceinline__ uint64_t warp_max(uint64_t key) {
     const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32));
-    const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u);
+    const bool highest = static_cast<uint32_t>(key >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, highest ? static_cast<uint32_t>(key) : 0u);
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
@@ -256,9 +258,8 @@ __device__ __forceinline__ void keep_allowed(Eight<T>& y, uint32_t ok) {
 template <typename T, bool CHOOSE>
 __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const RuleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint32_t listed[kWindow / 32];          // a bit per place of the window
-    __shared__ uint32_t in_section[kWindow / 32];      // and per place of a section of it
-    __shared__ uint16_t before[kWindow / 32];          // bits in the words before
+    __shared__ uint32_t listed[kMostWindow / 32];      // a bit per place of the window
+    __shared__ uint16_t before[kMostWindow / 32];      // bits in the words before
     __shared__ int warp_bits[kWarps], twice;           // twice: a token stands twice among the biases
     __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
@@ -360,84 +361,114 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
         }
     };
 
-    for (int w_begin = slice * kWindow; w_begin < places; w_begin += p.slices * kWindow) {
+    // (Unsigned: one step behind 2^30 places still fits.)
+    const unsigned window = p.window;
+    for (unsigned begin = slice * window; begin < static_cast<unsigned>(places); begin += p.slices * window) {
+        const int w_begin = begin;
         const int w0 = w_begin - shift;  // the token at the window's first place (negative before the row)
-        const auto in_window = [&](int v) { return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u; };
-        // Sets the bits of the listed tokens at places s0 .. s0 + section of the window and numbers them, if
-        // there are numbers enough. Returns how many there are.
-        const auto give_numbers = [&](uint32_t* bits, unsigned s0, unsigned section) -> int {
-            for (int i = tid; i < kWindow / 32; i += kThreads) bits[i] = 0;
+        const auto in_window = [&](int v) {
+            return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u;
+        };
+        const auto clear = [&](int n) {
             if (tid == 0) twice = 0;
+            for (int i = tid; i < n; i += kThreads) {
+                count[i] = 0;
+                bias[i] = 0.0f;
+                entry[i] = ~0u;
+            }
+        };
+        // Sets the bits of the listed tokens' places, numbers them, and prepares the first kNumbers. Returns how
+        // many there are.
+        const auto give_numbers = [&]() -> int {
+            const int own_words = (window / 32 + kThreads - 1) / kThreads;  // neighbouring ones that a thread numbers
+            for (int i = tid; i < own_words * kThreads; i += kThreads) listed[i] = 0;
             __syncthreads();
             const auto give = [&](int v) {
                 const unsigned at = in_window(v);
-                if (at - s0 < section) atomicOr(bits + at / 32, 1u << (at % 32));
+                if (at < window) atomicOr(listed + at / 32, 1u << (at % 32));
             };
             each_said(give);
             each_bias([&](int v, float, int) { give(v); });
             __syncthreads();
-            static_assert(kWindow / 32 == kThreads, "a word of bits a thread");
-            const uint32_t word = bits[tid];
-            int upto = __popc(word);
+            int own = 0;
+            for (int q = 0; q < own_words; ++q) own += __popc(listed[tid * own_words + q]);
+            const auto scan = [&](int v) {  // over the warp, the lane's own included
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += up;
-            }
+                for (int d = 1; d < 32; d *= 2) {
+                    const int up = __shfl_up_sync(0xffffffffu, v, d);
+                    if (lane >= d) v += up;
+                }
+                return v;
+            };
+            const int upto = scan(own);
             if (lane == 31) warp_bits[warp] = upto;
             __syncthreads();
-            int all = 0;
-            for (int w = 0; w < kWarps; ++w) {
-                if (w == warp) upto += all;
-                all += warp_bits[w];
+            const int warps_upto = scan(lane < kWarps ? warp_bits[lane] : 0);
+            const int all = __shfl_sync(0xffffffffu, warps_upto, 31);
+            int i = upto - own + (warp ? __shfl_sync(0xffffffffu, warps_upto, warp ? warp - 1 : 0) : 0);
+            for (int q = 0; q < own_words; ++q) {
+                const int word = tid * own_words + q;
+                before[word] = static_cast<uint16_t>(i);
+                for (uint32_t b = listed[word]; b; b &= b - 1, ++i)
+                    if (i < kNumbers) list[i] = static_cast<uint16_t>(word * 32 + __ffs(b) - 1);
             }
-            int i = upto - __popc(word);
-            before[tid] = static_cast<uint16_t>(i);
-            if (all <= kNumbers)
-                for (uint32_t b = word; b; b &= b - 1, ++i) {
-                    list[i] = static_cast<uint16_t>(tid * 32 + __ffs(b) - 1);
-                    count[i] = 0;
-                    bias[i] = 0.0f;
-                    entry[i] = ~0u;
-                }
+            clear(min(all, kNumbers));
             __syncthreads();
             return all;
         };
-        // The numbered tokens' counts and biases. A token's biases add up in list order.
-        const auto add_up = [&](const uint32_t* bits, unsigned s0, unsigned section) {
-            const auto number = [&](unsigned at) { return before[at / 32] + __popc(bits[at / 32] & ((1u << (at % 32)) - 1)); };
+        // The counts and biases of the n tokens numbered from n0 (and their places, if they are not the first). A
+        // token's biases add up in list order.
+        const auto add_up = [&](int n0, int n) {
+            if (n0 > 0) {
+                clear(n);
+                for (unsigned word = tid; word < window / 32; word += kThreads) {
+                    int i = before[word] - n0;
+                    for (uint32_t b = i < n ? listed[word] : 0; b; b &= b - 1, ++i)
+                        if (i >= 0 && i < n) list[i] = static_cast<uint16_t>(word * 32 + __ffs(b) - 1);
+                }
+                __syncthreads();
+            }
+            // A place's number counted from n0; kNumbers or more behind these.
+            const auto number = [&](unsigned at) {
+                return before[at / 32] + __popc(listed[at / 32] & ((1u << (at % 32)) - 1)) - static_cast<unsigned>(n0);
+            };
             each_said([&](int v) {
                 const unsigned at = in_window(v);
-                if (at - s0 < section) atomicAdd(count + number(at), 1u);
+                if (at >= window) return;
+                const unsigned i = number(at);
+                if (i < kNumbers) atomicAdd(count + i, 1u);
             });
             if (!biasing) return;
-            each_bias([&](int v, float, int i) {
+            each_bias([&](int v, float, int j) {
                 const unsigned at = in_window(v);
-                if (at - s0 < section && atomicMin(entry + number(at), static_cast<uint32_t>(i)) != ~0u) twice = 1;
+                if (at >= window) return;
+                const unsigned i = number(at);
+                if (i < kNumbers && atomicMin(entry + i, static_cast<uint32_t>(j)) != ~0u) twice = 1;
             });
             __syncthreads();
             const bool search = twice != 0;
-            each_bias([&](int v, float b, int i) {
+            each_bias([&](int v, float b, int j) {
                 const unsigned at = in_window(v);
-                if (at - s0 >= section) return;
-                const int n = number(at);
-                if (entry[n] != static_cast<uint32_t>(i)) return;  // the token's first entry adds the others
+                if (at >= window) return;
+                const unsigned i = number(at);
+                // The token's first entry adds the others.
+                if (i >= kNumbers || entry[i] != static_cast<uint32_t>(j)) return;
                 if (search)
-                    for (int j = i + 1; j < p.n_bias; ++j)
-                        if (__ldg(bias_ids + j) == v) b += __ldg(bias_values + j);
-                bias[n] = b;
+                    for (int l = j + 1; l < p.n_bias; ++l)
+                        if (__ldg(bias_ids + l) == v) b += __ldg(bias_values + l);
+                bias[i] = b;
             });
         };
         int numbers = 0;
         if (listing) {
             __syncthreads();  // the previous window is done with
-            numbers = give_numbers(listed, 0, kWindow);
+            numbers = give_numbers();
         } else if (CHOOSE && !bounded) {
             __syncthreads();  // the bound has been set
         }
 
         // ---- the logits ----------------------------------------------------------------------------
-        for (int e0 = w_begin; e0 < min(places, w_begin + kWindow); e0 += kTile) {
+        for (int e0 = w_begin; e0 < min(places, w_begin + static_cast<int>(window)); e0 += kTile) {
             const int v0 = e0 - shift;
             Eight<T> raw[kPerThread];
 #pragma unroll
@@ -510,17 +541,13 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                     std::integral_constant<int, 8 * kPerThread>());
             }
         }
-        if (numbers == 0) continue;
 
-        // ---- the listed tokens: all at once, or in sections of as many places as there are numbers ----
-        const bool fits = numbers <= kNumbers;
-        const unsigned section = fits ? kWindow : kNumbers;
-        for (unsigned s0 = 0; s0 < kWindow; s0 += section) {
-            __syncthreads();  // the logits have been written (constrain), the previous section is done with
-            if (!fits) numbers = give_numbers(in_section, s0, section);
-            add_up(fits ? listed : in_section, s0, section);
+        // ---- the listed tokens, as many at once as there are numbers -----------------------------------
+        for (int n0 = 0; n0 < numbers; n0 += kNumbers) {
+            __syncthreads();  // the logits have been written (constrain), the previous ones are done with
+            const int n = min(numbers - n0, kNumbers);
+            add_up(n0, n);
             __syncthreads();
-            const int n = numbers;
             float top = -INFINITY;
             for (int i = tid; i < n; i += kThreads) {
                 const int v = w0 + list[i];
@@ -680,11 +707,12 @@ cudaError_t launch_type(const RuleParams& p, int dtype, cudaStream_t stream) {
     return launch<__half, CHOOSE>(p, stream);
 }
 
-// Windows of a row, some of whose rows may start up to seven values behind a 16-byte boundary.
-int windows(const RuleParams& p, size_t size) {
+// Places of a row, some of whose rows may start up to seven values behind a 16-byte boundary.
+int most_places(const RuleParams& p, size_t size) {
     const bool aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * size % 16 == 0;
-    return (p.vocab + (aligned ? 0 : 7) + kWindow - 1) / kWindow;
+    return p.vocab + (aligned ? 0 : 7);
 }
+int ceil_div(int64_t a, int b) { return static_cast<int>((a + b - 1) / b); }
 
 // Checks what both entry points share and fills `p`.
 int prepare(Ctx* ctx, const char* who, const void* logits, int dtype, size_t ld, size_t rows, size_t vocab,
@@ -758,12 +786,19 @@ extern "C" int telmo_logits_constrain(telmo_ctx* c, const void* logits, int dtyp
     if (int rc = prepare(ctx, "telmo_logits_constrain", logits, dtype, ld, rows, vocab, rules, &p)) return rc;
     if (!out || reinterpret_cast<uintptr_t>(out) % (dtype == TELMO_DTYPE_F32 ? 4 : 2) || out_ld < vocab ||
         out_ld > (size_t(1) << 40))
-        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out is NULL or misaligned, or its rows are short");
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out is NULL or misaligned, or its rows short");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     p.out = out;
     p.out_ld = static_cast<int64_t>(out_ld);
-    p.slices = windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    const int places = most_places(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    // A block's lists cost about as much as a tile, so windows are four tiles long, and shorter where the blocks
+    // still fit on the SMs at once (three on each). 256 rows of 131072: 49 us at four tiles, 55 at two, 53 at
+    // eight; 32 rows: 8.2 us at two tiles, 11.4 at one; 148 rows of 32000: 9.4 at two, 13.7 at one.
+    p.window = 4 * kTile;
+    const auto blocks = [&](int window) { return static_cast<int64_t>(ceil_div(places, window)) * p.rows; };
+    while (p.window > kTile && blocks(p.window / 2) <= 3 * ctx->sms) p.window /= 2;
+    p.slices = ceil_div(places, p.window);
     return ctx->cuda(launch_type<false>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_constrain");
 }
 
@@ -784,11 +819,18 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    // A block for each window, up to a cluster of eight, until all SMs have the two blocks they can hold: a
-    // block's first bound and its end cost as much as a window (256 rows of 131072: 103 us on two blocks a row,
-    // 114 on four).
+    const int places = most_places(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    // A cluster of up to eight blocks a row: the number that takes the least time, if the SMs hold two blocks
+    // each and a block's lists, first bound and end cost as much as two tiles. 256 rows of 131072: 72 us on one
+    // block a row, 78 on two; 300 rows: 75 on eight, 82 on one.
+    const auto cost = [&](int slices) {
+        return static_cast<int64_t>(ceil_div(static_cast<int64_t>(slices) * p.rows, 2 * ctx->sms)) *
+               (ceil_div(places, slices) + 2 * kTile);
+    };
     p.slices = 1;
-    const int most = windows(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
-    while (p.slices < 8 && p.slices < most && static_cast<int64_t>(p.slices) * p.rows < 2 * ctx->sms) p.slices *= 2;
+    for (int s = 2; s <= 8; s *= 2)
+        if (cost(s) < cost(p.slices)) p.slices = s;
+    p.window = std::min(kMostWindow, ceil_div(ceil_div(places, p.slices), kTile) * kTile);
+    p.slices = std::min(p.slices, ceil_div(places, p.window));
     return ctx->cuda(launch_type<true>(p, dtype, static_cast<cudaStream_t>(stream)), "telmo_logits_choose");
 }

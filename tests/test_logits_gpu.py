@@ -290,6 +290,15 @@ def test_many_rows(ctx):
     check_constrain(ctx, 70001, 3, "bf16", history=4, biases=2, states=3, seed=2)
 
 
+@pytest.mark.parametrize("rows,vocab,history,biases", [(3, 9001, 9000, 2500), (2, 40000, 30000, 3000), (500, 33000, 9000, 0),
+                                                       (200, 65540, 12000, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_listed_tokens_than_numbers(ctx, rows, vocab, history, biases, dtype):
+    """Thousands of listed tokens in every window, which are numbered 2048 at a time."""
+    check_constrain(ctx, rows, vocab, dtype, history=history, biases=biases, states=3, seed=5)
+    check_choose(ctx, rows, vocab, dtype, 5, history=history, biases=biases, states=3, seed=5)
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Rows whose offsets pass 2^31 elements."""
     import torch
@@ -303,6 +312,25 @@ def test_offsets_beyond_32_bits(ctx):
     k.constrain_logits(store, ld, 3, 100, None, store, ld)
     ctx.check()
     assert ids[:, 0].tolist() == [0, 0, 42] and store[2 * ld + 42] == 5
+
+
+def test_the_largest_vocabulary(ctx):
+    """2^30 tokens, the last of them listed."""
+    import torch
+    from telmo_b200 import Kernels, LogitRules, TelmoError
+    v = 1 << 30
+    store = torch.zeros(v + 1, dtype=torch.bfloat16, device="cuda")
+    store[0], store[v - 1], store[v] = 4, 8, 9
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    r = LogitRules(history=i32([[v - 1, v - 1]]), history_len=i32([2]), frequency=torch.tensor([1.5], device="cuda"))
+    ids, k = i32([[0, 0]]), Kernels(ctx)
+    k.choose_tokens(store, v, 1, v, r, 2, ids)
+    k.constrain_logits(store, v, 1, v, r, store, v)
+    ctx.check()
+    assert ids.tolist() == [[v - 1, 0]]
+    assert store[v - 1] == 5 and store[v] == 9 and store[0] == 4 and store[1:v - 1].count_nonzero() == 0
+    with pytest.raises(TelmoError):
+        k.choose_tokens(store, v + 1, 1, v + 1, None, 2, ids)
 
 
 def test_streams_and_graphs(ctx):
