@@ -72,7 +72,7 @@ inline bool q4_rows_aligned(const Q4Args& g) {
 }
 
 // Whether the product wants Q4Planes, their bytes, and their making.
-bool q4_rows_planes(const Q4Args& g);  // up to 32 rows
+bool q4_rows_planes(const Q4Args& g);  // up to 32 rows, f32 up to 16
 inline bool q4_gemm_planes(const Q4Args& g) { return g.a_type == kQ4F32 || !q4_rows_aligned(g); }
 size_t q4_planes_bytes(const Q4Args& g);
 cudaError_t q4_make_planes(const Q4Args& g, void* workspace, Q4Planes* planes, cudaStream_t stream);
@@ -82,7 +82,7 @@ constexpr size_t kQ4VecSmem = 222 << 10;
 bool q4_vec_fits(const Q4Args& g);
 cudaError_t q4_linear_vec(const Q4Args& g, cudaStream_t stream);
 
-// The product for up to 32 rows, and for any number of rows on tcgen05 tiles. `planes`: null where not wanted.
+// The product for up to 32 rows (f32: 16), and for any number of rows on tcgen05 tiles. `planes`: null where not wanted.
 cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream);
 cudaError_t q4_linear_gemm(const Q4Args& g, const Q4Planes* planes, cudaStream_t stream);
 

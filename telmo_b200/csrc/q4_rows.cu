@@ -57,19 +57,18 @@ namespace q4rows {
 namespace {
 
 template <int MODE>
-cudaError_t by_height(const RowsParams& p, int group, int r, cudaStream_t stream) {
+cudaError_t by_shape(const RowsParams& p, int group, cudaStream_t stream) {
     return by_group(p, group, [&](auto groups, auto zeros) {
-        return r == 2 ? launch_direct<MODE, decltype(groups)::value, decltype(zeros)::value, 2>(p, stream)
-                      : launch_direct<MODE, decltype(groups)::value, decltype(zeros)::value, 1>(p, stream);
+        return launch_direct<MODE, decltype(groups)::value, decltype(zeros)::value>(p, stream);
     });
 }
 
 }  // namespace
 
-cudaError_t launch_small(const RowsParams& p, int mode, int group, int r, cudaStream_t stream) {
-    if (mode == kModeF32) return by_height<kModeF32>(p, group, r, stream);
-    if (mode == kModeBF16) return by_height<kModeBF16>(p, group, r, stream);
-    return by_height<kModeF16>(p, group, r, stream);
+cudaError_t launch_small(const RowsParams& p, int mode, int group, cudaStream_t stream) {
+    if (mode == kModeF32) return by_shape<kModeF32>(p, group, stream);
+    if (mode == kModeBF16) return by_shape<kModeBF16>(p, group, stream);
+    return by_shape<kModeF16>(p, group, stream);
 }
 
 }  // namespace q4rows
@@ -99,17 +98,19 @@ cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t
     p.ldc = g.ldc;
     p.splits = 1;
     const int mode = g.a_type == kQ4BF16 ? kModeBF16 : g.a_type == kQ4F16 ? kModeF16 : kModeF32;
+    // Up to 8 rows of f32 or of any alignment are read as they are (8 f32 rows, 4096 -> 8192: 16 us; as planes
+    // the split kernel's 4 us come before a product), and aligned ones where a warp has one chunk at most, so
+    // that a ring has nothing to run ahead to (1024 -> 4096: 3.3 us, staged 4.3; 4096 -> 4096: 8.6 us, staged 7.3).
     if (!p.vec || mode == kModeF32 ? g.m <= 8 : g.m <= 8 && p.chunks <= kWarps) {
-        // Two 16-output slabs a warp share the activations' operands; one where that leaves SMs without work.
-        const int r = (p.n + 31) / 32 >= 2 * g.sms ? 2 : 1;
         p.split_chunks = p.chunks;
-        return launch_small(p, mode, g.w->group, r, stream);
+        return launch_small(p, mode, g.w->group, stream);
     }
     // Warps side by side read the same activations; the chunks are split over clusters as long as the
-    // blocks all run at once and a share keeps two chunks.
+    // blocks all run at once and a share keeps two chunks (4096 -> 4096: 24 rows 9.2 us, 22 without; 8 rows 7.3,
+    // 10.1 without; 4096 -> 8192, 32 rows: 16.8, 25 without).
     const int row_warps = g.m <= 8 ? 2 : 4, shares = kWarps / row_warps;
     const int blocks = (p.n + 32 * row_warps - 1) / (32 * row_warps);
-    const int resident = (g.m <= (mode == kModeF32 ? 8 : 16) ? 2 : 1) * g.sms;
+    const int resident = (mode != kModeF32 && g.m <= 24 ? 2 : 1) * g.sms;
     while (p.splits < 8 && blocks * p.splits * 2 <= resident && p.chunks >= 4 * shares * p.splits) p.splits *= 2;
     p.split_chunks = (p.chunks + p.splits - 1) / p.splits;
     return launch_aligned(p, mode == kModeF32 ? kModePlanes : mode, g.w->group, stream);

@@ -18,11 +18,17 @@
 // below 2^-126 vanish), and three products are summed. More than eight f32 rows come as two fp16 planes
 // (q4_split) and a power of two per row s_r, two instructions.
 //
-// A warp takes 16 R outputs and a share of the 128-input chunks, with its next chunks under way while
-// it works on one: in registers (q4_rows_kernel, rows of any alignment and f32), or in a ring in
-// shared memory together with the activations (q4_rows_staged_kernel). Warps that share outputs add up in shared memory, in order.
-// Where n gives too few blocks, the blocks of a cluster take a share of the chunks each and add up
-// through distributed shared memory, in rank order.
+// A warp takes 16 or 32 outputs and a share of the 128-input chunks, with its next chunks under way
+// while it works on one: in registers (q4_rows_kernel, rows of any alignment and f32), or in a ring
+// in shared memory together with the activations (q4_rows_staged_kernel). Warps that share outputs
+// add up in shared memory, in order. Where n gives too few blocks, the blocks of a cluster take a
+// share of the chunks each and add up through distributed shared memory, in rank order (24 rows,
+// 4096 -> 4096 in groups of 64: 9.2 us, 22 without).
+//
+// Measured (captured, weights from memory): 8 rows of bf16, 4096 -> 4096: 7.3 us (1.2 TB/s of codes and
+// scales); 24 rows of f16, 11009 -> 4096 with zero points: 17 us, 1.4 TB/s. A launch, the first
+// loads' way and the sums are 3 us of it; then the chunks' latencies: an SM holds 8 to 16 warps at
+// 141 registers, and 30% of its issue slots are used.
 #pragma once
 
 #include "ptx.cuh"
@@ -270,23 +276,23 @@ __device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, i
     cluster_sync();  // the other blocks have read this one's sums
 }
 
-template <int MODE, int GROUPS, bool ZEROS, int R>
+template <int MODE, int GROUPS, bool ZEROS>
 __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p) {
     constexpr bool BF16 = MODE != kModeF16;
-    constexpr int CB = 1;
+    constexpr int R = 1, CB = 1;  // slabs of 16 outputs a warp, of 8 activation rows
     constexpr int kParts = MODE == kModeF32 ? 3 : 1;
     constexpr int kWordsPerGroup = 4 / GROUPS;
     constexpr int kCols = 8;  // activation rows of the block
     __shared__ __align__(16) float sums[kWarps * 16 * R * kCols];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int g = lane >> 2, t = lane & 3;
-    constexpr int row_warps = 1, shares = kWarps, rw = 0;
+    constexpr int shares = kWarps;
     const int share = warp;
     const int split = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int block = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x;
     const int m0 = blockIdx.y * kCols;
-    const int64_t out0 = static_cast<int64_t>(block) * (16 * R * row_warps);  // the block's first output
-    const int64_t tile0 = out0 / 8 + rw * 2 * R;                              // the warp's first 8-output tile
+    const int64_t out0 = static_cast<int64_t>(block) * 16;  // the block's first output
+    const int64_t tile0 = out0 / 8;                         // the warp's first 8-output tile
     const int c_end = min(p.chunks, (split + 1) * p.split_chunks);
     int c = split * p.split_chunks + share;
 
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
     }
 
     // sums[share][column][output of the block]
-    const int outs = 16 * R * row_warps;
+    const int outs = 16 * R;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int col = 8 * cb + 2 * t + (j & 1);
-                sums[(share * kCols + col) * outs + rw * 16 * R + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
+                sums[(share * kCols + col) * outs + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
             }
     __syncthreads();
     finish_block<false, kWarps, 16 * R, kCols>(p, sums, out0, m0, split);
@@ -378,7 +384,9 @@ struct Staged {
     static constexpr int kShares = kWarps / kRowWarps;
     static constexpr int kStageBytes = kActBytes + kRowWarps * kCodeBytes;
     static constexpr int kSmem = std::max(kShares * kRing * kStageBytes, kWarps * 16 * R * 8 * CB * 4);
-    static constexpr int kBlocks = CB * kParts <= 2 ? 2 : 1;  // per SM, which bounds the registers
+    // Blocks per SM, which bounds the registers (24 rows, 4096 -> 8192: 13.9 us with two, 15.0 with one; two of
+    // 32 rows spill).
+    static constexpr int kBlocks = CB * kParts <= 3 ? 2 : 1;
 };
 
 template <int MODE, int GROUPS, bool ZEROS, int R, int CB>
@@ -540,19 +548,18 @@ cudaError_t launch_staged(const RowsParams& p, cudaStream_t stream) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!once.done(dev)) {
-        e = cudaFuncSetAttribute(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 S::kSmem);
+        e = cudaFuncSetAttribute(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (e != cudaSuccess) return e;
         once.mark(dev);
     }
-    return rows_launch(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, p, rows_grid(p, 16 * R * S::kRowWarps, 8 * CB), S::kSmem,
-                       stream);
+    return rows_launch(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, p,
+                       rows_grid(p, 16 * R * S::kRowWarps, 8 * CB), S::kSmem, stream);
 }
 
-template <int MODE, int GROUPS, bool ZEROS, int R>
+template <int MODE, int GROUPS, bool ZEROS>
 cudaError_t launch_direct(const RowsParams& p, cudaStream_t stream) {
-    return rows_launch(q4_rows_kernel<MODE, GROUPS, ZEROS, R>, p,
-                       rows_grid(p, 16 * R, 8), 0, stream);
+    return rows_launch(q4_rows_kernel<MODE, GROUPS, ZEROS>, p, rows_grid(p, 16, 8), 0, stream);
 }
 
 // Calls f with the group's and the zero points' constants.
@@ -570,7 +577,7 @@ cudaError_t by_group(const RowsParams& p, int group, F f) {
 }
 
 // Up to 8 rows as they are (q4_rows.cu); up to 32 aligned rows (q4_rows_staged.cu).
-cudaError_t launch_small(const RowsParams& p, int mode, int group, int r, cudaStream_t stream);
+cudaError_t launch_small(const RowsParams& p, int mode, int group, cudaStream_t stream);
 cudaError_t launch_aligned(const RowsParams& p, int mode, int group, cudaStream_t stream);
 
 }  // namespace q4rows

@@ -1,4 +1,5 @@
-// q4_rows_staged.cu -- products of up to 32 aligned activation rows with 4-bit weights (q4_rows.cuh).
+// q4_rows_staged.cu -- products of up to 32 aligned activation rows with 4-bit weights (q4_rows.cuh), of up to 16 in
+// two planes.
 #include "q4_rows.cuh"
 
 namespace telmo {
@@ -12,10 +13,14 @@ cudaError_t by_rows(const RowsParams& p, int group, cudaStream_t stream) {
     return by_group(p, group, [&](auto groups, auto zeros) {
         constexpr int kGroups = decltype(groups)::value;
         constexpr bool kZeros = decltype(zeros)::value;
-        if (MODE != kModePlanes && p.m <= 8) return launch_staged<MODE, kGroups, kZeros, 2, 1>(p, stream);
-        if (p.m <= 16) return launch_staged<MODE, kGroups, kZeros, 2, 2>(p, stream);
-        if (p.m <= 24) return launch_staged<MODE, kGroups, kZeros, 2, 3>(p, stream);
-        return launch_staged<MODE, kGroups, kZeros, 2, 4>(p, stream);
+        if constexpr (MODE == kModePlanes) {  // 9 to 16 rows
+            return launch_staged<MODE, kGroups, kZeros, 2, 2>(p, stream);
+        } else {
+            if (p.m <= 8) return launch_staged<MODE, kGroups, kZeros, 2, 1>(p, stream);
+            if (p.m <= 16) return launch_staged<MODE, kGroups, kZeros, 2, 2>(p, stream);
+            if (p.m <= 24) return launch_staged<MODE, kGroups, kZeros, 2, 3>(p, stream);
+            return launch_staged<MODE, kGroups, kZeros, 2, 4>(p, stream);
+        }
     });
 }
 

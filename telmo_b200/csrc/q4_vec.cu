@@ -23,6 +23,10 @@
 // Each block writes the digits of the whole rows into shared memory once and walks over blocks of
 // 32 outputs; its eight warps share the chunks, each with a ring of chunks of codes, scales and
 // zero points in shared memory (cp.async), and add up in order.
+//
+// Measured: one bf16 row, 4096 -> 32768, 69 MB of codes and scales from memory, 15.2 us captured: 4.5 TB/s
+// (70% of a copy's rate); the digits of the first block and the rings' first chunks take 3 us before the
+// stream runs.
 #include "q4_device.cuh"
 #include "ptx.cuh"
 #include "q4_async.cuh"
@@ -370,6 +374,8 @@ auto by_shape(int m, int group, bool zeros, F f) {
 
 }  // namespace
 
+// One or two rows whose digits and rings fit into shared memory. 4096 -> 8192, bf16: one row 8.2 us, 10.0 on the
+// row kernels; two rows 10.1 against 10.3. 1024 -> 4096, f32: 2.9 against 4.2, two rows 3.6 against 4.4.
 bool q4_vec_fits(const Q4Args& g) {
     if (g.m > 2) return false;
     return by_shape(g.m, g.w->group, g.w->zeros != nullptr, [&](auto m, auto groups, auto zeros) {
