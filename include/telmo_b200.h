@@ -127,7 +127,7 @@ int telmo_linear(telmo_ctx *ctx, const float *a, size_t lda, size_t m, const tel
  * are and f32 to at least 22 significant bits, codes exactly, sums and scales in f32; c is rounded
  * once. A row of a that holds an infinity or a NaN gives outputs that are not finite in that row
  * alone. a and c need no more than their elements' alignment; rows that start on 16-byte
- * boundaries are read fastest. a and c must not overlap. */
+ * boundaries are read fastest. a and c must not overlap (TELMO_ERR_ARGUMENT). */
 int telmo_linear_q4(telmo_ctx *ctx, const void *a, int a_dtype, size_t lda, size_t m,
                     const telmo_weights *w, const float *bias, int act, float scale, int accumulate,
                     void *c, int c_dtype, size_t ldc, void *stream);
@@ -204,7 +204,7 @@ typedef struct telmo_logit_rules {
 
 /* The values above for logits [rows, ld] of dtype (F32, BF16 or F16), vocab of each row, into out
  * [rows, out_ld] of the same type; what lies behind a row's vocab is left as it is. out may be
- * logits itself with the same ld, but must not overlap them otherwise. rules NULL: none. There is no
+ * logits itself with the same ld, but must not overlap them otherwise (TELMO_ERR_ARGUMENT). rules NULL: none. There is no
  * counterpart in the reference, whose decoders choose from the logits as they are or search with
  * word bonuses (src/biasing.rs). */
 int telmo_logits_constrain(telmo_ctx *ctx, const void *logits, int dtype, size_t ld, size_t rows,

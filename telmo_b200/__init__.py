@@ -88,7 +88,8 @@ def _refuse(message: str):
 
 def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
     """The address of a [rows, cols] matrix with rows `ld` elements apart that starts at tensor `t`,
-    which must lie on the context's device, be of one of `dtypes` and reach to the last element."""
+    which must lie on the context's device, be of one of `dtypes` and reach to the last element. A
+    view with gaps must have its own rows `ld` apart and its elements next to one another."""
     if t.get_device() != ctx.device:  # -1 in host memory
         _refuse(f"{name}: a tensor on {t.device}, the context is on cuda:{ctx.device}")
     if t.dtype not in dtypes:
@@ -96,8 +97,13 @@ def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
     if rows > 0 and cols > 0:
         if ld < cols:
             _refuse(f"{name}: rows {ld} elements apart hold no {cols} elements")
-        have = t.numel() if t.is_contiguous() else \
-            t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+        if t.is_contiguous():
+            have = t.numel()
+        else:
+            if t.stride(-1) != 1 or cols > t.shape[-1] or (rows > 1 and t.stride(-2) != ld):
+                _refuse(f"{name}: {list(t.shape)} with strides {list(t.stride())} has no rows of {cols} "
+                        f"elements, {ld} apart")
+            have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
         if have < (rows - 1) * ld + cols:
             _refuse(f"{name}: {have} elements, {(rows - 1) * ld + cols} are needed")
     return t.data_ptr()

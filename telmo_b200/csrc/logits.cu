@@ -787,11 +787,15 @@ extern "C" int telmo_logits_constrain(telmo_ctx* c, const void* logits, int dtyp
     if (!out || reinterpret_cast<uintptr_t>(out) % (dtype == TELMO_DTYPE_F32 ? 4 : 2) || out_ld < vocab ||
         out_ld > (size_t(1) << 40))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out is NULL or misaligned, or its rows short");
+    const size_t size = dtype == TELMO_DTYPE_F32 ? 4 : 2;
+    if (!(out == logits && (out_ld == ld || rows == 1)) &&
+        overlap(logits, ld * size, vocab * size, out, out_ld * size, vocab * size, rows))
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out overlaps the logits and is not the logits");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     p.out = out;
     p.out_ld = static_cast<int64_t>(out_ld);
-    const int places = most_places(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    const int places = most_places(p, size);
     // A block's lists cost about as much as a tile, so windows are four tiles long, and shorter where the blocks
     // still fit on the SMs at once (three on each). 256 rows of 131072: 49 us at four tiles, 55 at two, 53 at
     // eight; 32 rows: 8.2 us at two tiles, 11.4 at one; 148 rows of 32000: 9.4 at two, 13.7 at one.

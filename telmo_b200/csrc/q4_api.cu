@@ -131,9 +131,12 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     if (!out || ldc < n || ldc > (size_t(1) << 40))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: c is NULL or ldc %zu is below n %zu", ldc, n);
     if (act < TELMO_ACT_NONE || act > TELMO_ACT_SILU) return ctx->fail(TELMO_ERR_ARGUMENT, "unknown act %d", act);
+    const size_t as = at == kQ4F32 ? 4 : 2, cs = ct == kQ4F32 ? 4 : 2;
     const auto misaligned = [](const void* p, uintptr_t b) { return reinterpret_cast<uintptr_t>(p) % b != 0; };
-    if (misaligned(a, at == kQ4F32 ? 4 : 2) || misaligned(out, ct == kQ4F32 ? 4 : 2) || misaligned(bias, 4))
+    if (misaligned(a, as) || misaligned(out, cs) || misaligned(bias, 4))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: a, c or bias is not aligned to its elements");
+    if (overlap(a, lda * as, k * as, out, ldc * cs, n * cs, m))
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: a and c overlap");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     Q4Args g;

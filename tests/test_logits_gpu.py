@@ -364,6 +364,40 @@ def test_streams_and_graphs(ctx):
             assert all(torch.equal(a, b) for a, b in zip(outs[i], outs[2 + i]))
 
 
+def test_columns_and_overlaps_are_refused(ctx):
+    """Views whose elements are not where a row's are (a column to write tokens to, a column of parameters), and
+    outputs that overlap the logits."""
+    import torch
+    from telmo_b200 import Kernels, LogitRules, TelmoError
+    k = Kernels(ctx)
+    store = torch.randn((4, 200), device="cuda")
+    x, y = store[:, :100], store[:, 100:]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    said, n, ids = torch.zeros((4, 9), **i32), torch.ones(4, **i32), torch.zeros((4, 1), **i32)
+    table = torch.ones((4, 3), device="cuda")
+    before = store.clone()
+    for call in (lambda: k.choose_tokens(x, 200, 4, 100, None, 1, said[:, 3:4]),
+                 lambda: k.choose_tokens(x, 200, 4, 100, None, 1, said[:, 3]),
+                 lambda: k.choose_tokens(x, 200, 4, 100, None, 1, ids, store[:, 1:2]),
+                 lambda: k.choose_tokens(x, 100, 4, 100, None, 1, ids),
+                 lambda: k.choose_tokens(x, 200, 4, 101, None, 1, ids),
+                 lambda: k.choose_tokens(x, 200, 4, 100, LogitRules(said, n, repetition=table[:, 1]), 1, ids),
+                 lambda: k.choose_tokens(x, 200, 4, 100, LogitRules(said, n, presence=table[:, :1]), 1, ids),
+                 lambda: k.choose_tokens(x, 200, 4, 100, LogitRules(said, said[:, 0]), 1, ids),
+                 lambda: k.constrain_logits(store, 200, 4, 100, None, store, 150),
+                 lambda: k.constrain_logits(store, 200, 4, 100, None, store[0, 50:], 200),
+                 lambda: k.constrain_logits(store[0, 50:], 200, 3, 100, None, store, 200),
+                 lambda: k.constrain_logits(store, 200, 4, 100, None, store[1], 150)):
+        with pytest.raises(TelmoError):
+            call()
+    ctx.check()
+    assert torch.equal(store, before) and not said.any()
+    k.constrain_logits(x, 200, 4, 100, None, y, 200)  # side by side
+    k.constrain_logits(store, 200, 1, 100, None, store, 100)  # one row, in place
+    ctx.check()
+    assert torch.equal(y, before[:, :100]) and torch.equal(x, before[:, :100])
+
+
 def test_refusals(ctx):
     import ctypes
     import torch

@@ -223,6 +223,31 @@ def test_no_rows_and_refusals(ctx):
     dev.free()
 
 
+def test_columns_and_overlaps_are_refused(ctx):
+    """A bias that is a column, transposed activations, rows other than the view's, and outputs that overlap."""
+    import torch
+    from telmo_b200 import Epilogue, Kernels, TelmoError
+    kern = Kernels(ctx)
+    dev, _ = weights(ctx, 40, 64, 32, False, 1)
+    store = torch.randn((64, 128), device="cuda")
+    c = torch.zeros((4, 40), device="cuda")
+    before = store.clone()
+    for call in (lambda: kern.linear(store[:4, :64].contiguous(), 4, dev, c, Epilogue(bias=store[:40, 0])),
+                 lambda: kern.matmul(store.t(), 64, 4, dev, c, 40), lambda: kern.matmul(store[:, :64], 64, 4, dev, c, 40),
+                 lambda: kern.matmul(store, 128, 4, dev, store[0, 63:], 128),
+                 lambda: kern.matmul(store[0, 39:], 128, 4, dev, store, 128),
+                 lambda: kern.matmul(store, 128, 4, dev, store[1], 64), lambda: kern.matmul(store, 128, 1, dev, store, 40)):
+        with pytest.raises(TelmoError):
+            call()
+    ctx.check()
+    assert torch.equal(store, before) and not c.any()
+    kern.matmul(store[:, :64], 128, 4, dev, c, 40)
+    kern.matmul(store[:, :64], 128, 4, dev, store[:, 64:104], 128)  # side by side
+    ctx.check()
+    assert torch.equal(store[:4, 64:104], c) and torch.equal(store[:, 104:], before[:, 104:])
+    assert torch.equal(store[:, :64], before[:, :64]) and torch.equal(store[4:], before[4:])
+
+
 @pytest.mark.parametrize("m", [1, 24, 300])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_streams_and_graphs(ctx, m, dtype):
