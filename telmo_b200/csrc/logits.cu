@@ -25,7 +25,7 @@
 // the others in list order. Tokens go to threads by number, so no sum depends on timing. Numbers beyond
 // kNumbers come in further rounds over the lists. With the rules inside the pass over the logits some lane
 // of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16 values with
-// 2000 tokens each, which take 52 us here (93 MB read and written; the pass alone 30 us).
+// 2000 tokens each, which take 50 us here (93 MB read and written; the pass alone 30 us).
 //
 // The k best are found by a bound: a token's key is its value's order and then its place, so no two are
 // equal; tokens whose key is below the block's bound are passed over, others go to a buffer in
@@ -154,10 +154,14 @@ struct MaxSum {
         }
     }
     __device__ __forceinline__ void add(float x) { s += exp_of(x - m); }
-    __device__ __forceinline__ void merge(float m2, float s2) {
-        const float top = fmaxf(m, m2);
-        s = s * exp_of(m - top) + s2 * exp_of(m2 - top);
+    // The warp's lanes together, in every lane.
+    __device__ __forceinline__ void join() {
+        const uint32_t order = __reduce_max_sync(0xffffffffu, order_of(m));  // m is no NaN
+        const float top = value_of(static_cast<uint64_t>(order) << 32);
+        s *= exp_of(m - top);
         m = top;
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
     }
 };
 
@@ -278,8 +282,9 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
     const bool same_cut = !CHOOSE && static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T)) == shift;
     const int places = p.vocab + shift;
 
-    // The row's lists. What lies outside the vocabulary becomes kNowhere. (They are read again for each
-    // window, from L1 or L2: keeping them in registers cost the pass over the logits spills.)
+    // The row's lists. What lies outside the vocabulary becomes kNowhere. A thread's first entries stay in
+    // registers, on their way before the first meeting (256 rows of 131072: constrain 52.6 -> 49.7 us, choose 74 ->
+    // 71.5); further ones are read again for each window, from L1 or L2: keeping them too cost the pass spills.
     constexpr int kNowhere = INT_MIN;
     int said = 0;
     float theta = 1.0f, freq = 0.0f, pres = 0.0f;
@@ -297,13 +302,17 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
         if (p.presence) pres = __ldg(p.presence + row);
     }
     // Calls f(token) for each of this thread's tokens so far, f(token, bias, entry) for its biases.
+    const int first_said = tid < said ? token(history + tid) : kNowhere;
     const auto each_said = [&](auto f) {
+        f(first_said);
 #pragma unroll 4
-        for (int i = tid; i < said; i += kThreads) f(token(history + i));
+        for (int i = tid + kThreads; i < said; i += kThreads) f(token(history + i));
     };
+    const int first_biased = biasing && tid < p.n_bias ? token(bias_ids + tid) : kNowhere;
     const auto each_bias = [&](auto f) {
-        if (biasing)
-            for (int i = tid; i < p.n_bias; i += kThreads) f(token(bias_ids + i), __ldg(bias_values + i), i);
+        if (!biasing) return;
+        f(first_biased, tid < p.n_bias ? __ldg(bias_values + tid) : 0.0f, tid);
+        for (int i = tid + kThreads; i < p.n_bias; i += kThreads) f(token(bias_ids + i), __ldg(bias_values + i), i);
     };
 
     const uint32_t* mask = nullptr;
@@ -580,11 +589,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
     if constexpr (CHOOSE) {
         if (tid < kMaxK) choice.best[tid] = 0;
         __syncthreads();  // the buffer is complete; a block without a window has set it
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, total.m, d), s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
-            total.merge(m2, s2);
-        }
+        total.join();
         if (lane == 0) {
             choice.warp_m[warp] = total.m;
             choice.warp_s[warp] = total.s;
@@ -597,12 +602,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 total.m = m;
                 total.s = s;
             }
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, total.m, d);
-                const float s2 = __shfl_xor_sync(0xffffffffu, total.s, d);
-                total.merge(m2, s2);
-            }
+            total.join();
         };
         if (warp == 0) {
             across(lane < kWarps, choice.warp_m[lane % kWarps], choice.warp_s[lane % kWarps]);
@@ -825,11 +825,12 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
     p.k = static_cast<int>(k);
     const int places = most_places(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
     // A cluster of up to eight blocks a row: the number that takes the least time, if the SMs hold two blocks
-    // each and a block's lists, first bound and end cost as much as two tiles. 256 rows of 131072: 72 us on one
+    // each, a block's lists, first bound and end cost as much as two tiles, and a cluster's meetings too. 256 rows of 131072: 72 us on one
     // block a row, 78 on two; 300 rows: 75 on eight, 82 on one.
     const auto cost = [&](int slices) {
         return static_cast<int64_t>(ceil_div(static_cast<int64_t>(slices) * p.rows, 2 * ctx->sms)) *
-               (ceil_div(places, slices) + 2 * kTile);
+                   (ceil_div(places, slices) + 2 * kTile) +
+               (slices > 1 ? 2 * kTile : 0);
     };
     p.slices = 1;
     for (int s = 2; s <= 8; s *= 2)
