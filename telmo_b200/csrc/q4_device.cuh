@@ -9,6 +9,28 @@
 
 namespace telmo {
 
+// A product behind the kernel that makes its planes is launched while that one still runs
+// (programmatic stream serialisation) and waits where it first needs them; weights it reads before
+// (200 rows of f32, 1024 -> 4096: 18.5 us without, 16.8 with; 1500 rows: 39.0 and 36.7).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Adds a launch's attributes: a cluster of `cluster` blocks, and such a start.
+inline void add_attributes(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int cluster, bool early) {
+    cfg.attrs = attr;
+    cfg.numAttrs = 0;
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    if (early) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+}
+
 // Codes 2 p and 2 p + 1 of a word less their zero point, as two exact operands; `base` is
 // code_base of the zero point: a pair of 128 + zero (bf16) or 1024 + zero (fp16).
 template <bool BF16>

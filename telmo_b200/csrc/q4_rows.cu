@@ -88,6 +88,7 @@ cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t
     p.lda = planes ? planes->ld : g.lda;
     p.m = g.m;
     p.vec = planes || q4_rows_aligned(g);
+    p.planes = planes != nullptr;
     p.row_scale = planes ? planes->row_scale : nullptr;
     p.bias = g.bias;
     p.act = g.act;

@@ -61,6 +61,7 @@ struct RowsParams {
     int m;
     bool vec;                // rows of a start on 16-byte boundaries
     const float* row_scale;  // [m] with planes
+    bool planes;             // a was made by the kernel before
     const float* bias;
     int act;
     float scale;
@@ -238,7 +239,7 @@ __device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, i
     const auto finish = [&](int e, const float4& s) {
         const int row = m0 + e / (OUTS / 4);
         if (row >= p.m) return;
-        const float rs = SCALED ? __ldg(p.row_scale + row) : 1.0f;
+        const float rs = SCALED ? p.row_scale[row] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t out = out0 + e % (OUTS / 4) * 4 + j;
@@ -414,8 +415,17 @@ __global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_
     const uint8_t* scales = reinterpret_cast<const uint8_t*>(p.scales) + (first * 8 + g) * GROUPS * 2;
     const uint8_t* zeros = ZEROS ? p.zeros + (first * 8 + g) * GROUPS : nullptr;
 
-    // Starts the copies of chunk c into a ring place: 16 pieces of 16 bytes to each row of activations.
-    const auto fetch = [&](int c, int place) {
+    // Start the copies of chunk c into a ring place: the codes, and 16 pieces of 16 bytes to each row of
+    // activations.
+    const auto fetch_codes = [&](int c, int place) {
+        if (c < c_end && live) {
+            const uint32_t to = mine + static_cast<uint32_t>(place * stage_bytes + S::kActBytes + rw * S::kCodeBytes + lane * 16);
+#pragma unroll
+            for (int r = 0; r < 2 * R; ++r)
+                cp_async16(to + r * 512, codes + static_cast<int64_t>(c) * 512 + r * 32, 16);
+        }
+    };
+    const auto fetch_rows = [&](int c, int place) {
         if (c < c_end) {
             const uint32_t at = mine + static_cast<uint32_t>(place * stage_bytes);
             for (int e = rw * 32 + lane; e < kParts * kCols * 16; e += row_warps * 32) {
@@ -425,14 +435,8 @@ __global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_
                 if (left) src += (static_cast<int64_t>(row / kCols) * p.m + m) * p.lda + c * 128 + piece * 8;
                 cp_async16(at + row * kPitch + piece * 16, src, left * 2);
             }
-            if (live) {
-                const uint32_t to = at + S::kActBytes + rw * S::kCodeBytes + lane * 16;
-#pragma unroll
-                for (int r = 0; r < 2 * R; ++r)
-                    cp_async16(to + r * 512, codes + static_cast<int64_t>(c) * 512 + r * 32, 16);
-            }
         }
-        cp_commit();  // an empty group where there is no such chunk, so that the counts stay even
+        cp_commit();  // of both; an empty group where there is no such chunk, so that the counts stay even
     };
     const auto load_scales = [&](int c, uint32_t (&d)[2 * R][GROUPS == 4 ? 2 : 1], uint32_t (&z)[2 * R]) {
 #pragma unroll
@@ -458,8 +462,10 @@ __global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_
 
     float acc[R][CB][4] = {}, part[R][CB][4] = {};
     uint32_t d_next[2 * R][GROUPS == 4 ? 2 : 1], z_next[2 * R] = {};
-    for (int i = 0; i < kRing - 1; ++i) fetch(c0 + i * shares, i);
+    for (int i = 0; i < kRing - 1; ++i) fetch_codes(c0 + i * shares, i);
     if (c0 < c_end) load_scales(c0, d_next, z_next);
+    wait_for_previous();
+    for (int i = 0; i < kRing - 1; ++i) fetch_rows(c0 + i * shares, i);
     int place = 0;
     for (int c = c0; c < c_end; c += shares) {
         uint32_t d[2 * R][GROUPS == 4 ? 2 : 1], z[2 * R];
@@ -472,7 +478,9 @@ __global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_
         cp_wait<kRing - 2>();
         // The share's copies are complete, and its warps are done with the place that is filled next.
         asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
-        fetch(c + (kRing - 1) * shares, place == 0 ? kRing - 1 : place - 1);
+        const int ahead = place == 0 ? kRing - 1 : place - 1;
+        fetch_codes(c + (kRing - 1) * shares, ahead);
+        fetch_rows(c + (kRing - 1) * shares, ahead);
         if (c + shares < c_end) load_scales(c + shares, d_next, z_next);
         const uint32_t at = mine + static_cast<uint32_t>(place * stage_bytes);
         const uint32_t acts = at + static_cast<uint32_t>(g * kPitch + t * 16);
@@ -530,13 +538,8 @@ inline cudaError_t rows_launch(void (*kernel)(RowsParams), const RowsParams& p, 
     cfg.blockDim = dim3(32 * kWarps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.splits > 1 ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    add_attributes(cfg, attr, p.splits, p.planes);
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

@@ -399,3 +399,40 @@ def test_two_streams_at_once(ctx):
     for s in range(2):
         assert all(torch.equal(y, want[s]) for y in got[s])
     dev.free()
+
+
+@pytest.mark.parametrize("m,k,dtype", [(12, 512, "f32"), (24, 515, "f16"), (40, 515, "bf16"), (300, 512, "f32")])
+def test_each_product_reads_the_one_before(ctx, m, k, dtype):
+    """A chain of products, each of whose activations are the output of the one before, gives the bits that it
+    gives with a wait after each; captured too. (A product starts while its activations are still prepared.)"""
+    import torch
+    from telmo_b200 import Epilogue, Kernels
+    devs = [weights(ctx, k, k, 32, True, s)[0] for s in range(3)]
+    kern, t = Kernels(ctx), types()[dtype]
+    x = torch.randn((m, k), device="cuda").to(t)
+    # f16's last outputs underflow (each product is about a tenth of its activations): all outputs are compared.
+    want, got = ([torch.zeros((m, k), device="cuda", dtype=t) for _ in range(13)] for _ in range(2))
+
+    def chain(to, wait):
+        to[0].copy_(x)
+        for i in range(12):
+            kern.linear(to[i], m, devs[i % 3], to[i + 1], Epilogue(scale=1e-3))
+            if wait:
+                torch.cuda.synchronize()
+    chain(want, True)
+    assert all(y.float().abs().max() > 0 for y in want[:4]) and all(torch.isfinite(y).all() for y in want)
+    for _ in range(20):
+        chain(got, False)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(got, False)
+    for _ in range(5):
+        for y in got:
+            y.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ctx.check()
+    del graph
+    for d in devs:
+        d.free()
