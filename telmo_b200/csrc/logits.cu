@@ -57,6 +57,7 @@ constexpr int kMostWindow = 8 * kTile;             // tokens per window at most
 constexpr int kNumbers = 2048;                     // listed tokens with a number
 constexpr int kMaxK = 8;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
+constexpr uint32_t kTwice = 1u << 31;               // of a count: the token stands twice among the biases
 constexpr float kLowest = -3.402823466e38f;
 
 struct RuleParams {
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t listed[kMostWindow / 32];      // a bit per place of the window
     __shared__ uint16_t before[kMostWindow / 32];      // bits in the words before
-    __shared__ int warp_bits[kWarps], twice;           // twice: a token stands twice among the biases
+    __shared__ int warp_bits[kWarps];
     __shared__ typename std::conditional<CHOOSE, Choice, int>::type choice;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -379,7 +380,6 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
             return v >= 0 ? static_cast<unsigned>(v) - static_cast<unsigned>(w0) : ~0u;
         };
         const auto clear = [&](int n) {
-            if (tid == 0) twice = 0;
             for (int i = tid; i < n; i += kThreads) {
                 count[i] = 0;
                 bias[i] = 0.0f;
@@ -452,17 +452,16 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 const unsigned at = in_window(v);
                 if (at >= window) return;
                 const unsigned i = number(at);
-                if (i < kNumbers && atomicMin(entry + i, static_cast<uint32_t>(j)) != ~0u) twice = 1;
+                if (i < kNumbers && atomicMin(entry + i, static_cast<uint32_t>(j)) != ~0u) atomicOr(count + i, kTwice);
             });
             __syncthreads();
-            const bool search = twice != 0;
             each_bias([&](int v, float b, int j) {
                 const unsigned at = in_window(v);
                 if (at >= window) return;
                 const unsigned i = number(at);
                 // The token's first entry adds the others.
                 if (i >= kNumbers || entry[i] != static_cast<uint32_t>(j)) return;
-                if (search)
+                if (count[i] & kTwice)
                     for (int l = j + 1; l < p.n_bias; ++l)
                         if (__ldg(bias_ids + l) == v) b += __ldg(bias_values + l);
                 bias[i] = b;
@@ -562,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 const int v = w0 + list[i];
                 const uint32_t bits = mask ? __ldg(mask + v / 32) : ~0u;
                 float x = to_f32(in[v]);
-                x = penalised(x, count[i], theta, freq, pres);
+                x = penalised(x, count[i] & ~kTwice, theta, freq, pres);
                 if (biasing) x = __fadd_rn(x, bias[i]);
                 const bool ok = !none && ((bits >> (v % 32)) & 1);
                 if (CHOOSE) {

@@ -290,6 +290,12 @@ def test_many_rows(ctx):
     check_constrain(ctx, 70001, 3, "bf16", history=4, biases=2, states=3, seed=2)
 
 
+def test_a_bias_for_every_token(ctx):
+    """Lists as long as the vocabulary, tokens among them twice and many times: time for those alone."""
+    check_constrain(ctx, 2, 20000, "f32", history=40, biases=20000, states=3, seed=6)
+    check_choose(ctx, 2, 20000, "bf16", 4, history=40, biases=20000, states=3, seed=6)
+
+
 @pytest.mark.parametrize("rows,vocab,history,biases", [(3, 9001, 9000, 2500), (2, 40000, 30000, 3000), (500, 33000, 9000, 0),
                                                        (200, 65540, 12000, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
