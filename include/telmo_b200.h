@@ -194,8 +194,8 @@ typedef struct telmo_logit_rules {
     const float *frequency;     /* [rows]; NULL: 0 */
     const float *presence;      /* [rows]; NULL: 0 */
     const int32_t *bias_ids;    /* [rows, bias_ld], n_bias of them used; one outside the vocabulary */
-    const float *bias;          /* is left out. Biases of one token add up, in list order */
-    size_t n_bias, bias_ld;
+    const float *bias;          /* is left out. Biases of one token add up, in list order; at most */
+    size_t n_bias, bias_ld;     /* 2^20 entries */
     const uint32_t *allowed;    /* [n_states, allowed_ld] bit masks: bit v % 32 of word v / 32 */
     size_t n_states, allowed_ld;
     const int32_t *state;       /* [rows] the row's mask; negative: every token, n_states or more: */

@@ -293,7 +293,7 @@ class LogitRules:
     repetition: Optional[object] = None   # f32 [rows], above 0
     frequency: Optional[object] = None    # f32 [rows]
     presence: Optional[object] = None     # f32 [rows]
-    bias_ids: Optional[object] = None     # int32 [rows, entries], negative: unused
+    bias_ids: Optional[object] = None     # int32 [rows, entries <= 2^20], negative: unused
     bias: Optional[object] = None         # f32 [rows, entries]
     allowed: Optional[object] = None      # int32 (or uint32) [states, ceil(vocab / 32)] bit masks
     state: Optional[object] = None        # int32 [rows], negative: no mask; None: row r has mask r

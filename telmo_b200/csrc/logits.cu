@@ -21,8 +21,8 @@
 //              join the others.
 // A block walks over windows of 8192 to 65536 tokens: it sets a bit for each listed token's place, numbers
 // the bits in order (a prefix sum over the words' counts), and counts by number in shared memory with
-// integer atomics (the counts do not depend on their order); a token's first entry among the biases adds
-// the others in list order. Tokens go to threads by number, so no sum depends on timing. Numbers beyond
+// integer atomics (the counts do not depend on their order); a token's biases add up in list order, an
+// entry a round where many tokens have several, else by a search from the first. Tokens go to threads by number, so no sum depends on timing. Numbers beyond
 // kNumbers come in further rounds over the lists. With the rules inside the pass over the logits some lane
 // of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16 values with
 // 2000 tokens each, which take 50 us here (93 MB read and written; the pass alone 30 us).
@@ -57,7 +57,6 @@ constexpr int kMostWindow = 8 * kTile;             // tokens per window at most
 constexpr int kNumbers = 2048;                     // listed tokens with a number
 constexpr int kMaxK = 8;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
-constexpr uint32_t kTwice = 1u << 31;               // of a count: the token stands twice among the biases
 constexpr float kLowest = -3.402823466e38f;
 
 struct RuleParams {
@@ -273,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
     uint16_t* list = reinterpret_cast<uint16_t*>(smem);  // places by number
     uint32_t* count = reinterpret_cast<uint32_t*>(list + kNumbers);
     float* bias = reinterpret_cast<float*>(count + kNumbers);
-    uint32_t* entry = reinterpret_cast<uint32_t*>(bias + kNumbers);  // a bias of the token
+    uint32_t* entry = reinterpret_cast<uint32_t*>(bias + kNumbers);  // the token's last entry added to its bias
+    uint32_t* later = entry + kNumbers;                              // and the one behind it
 
     const T* in = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.ld;
     T* out = CHOOSE ? nullptr : static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_ld;
@@ -448,24 +448,62 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 if (i < kNumbers) atomicAdd(count + i, 1u);
             });
             if (!biasing) return;
-            each_bias([&](int v, float, int j) {
-                const unsigned at = in_window(v);
-                if (at >= window) return;
-                const unsigned i = number(at);
-                if (i < kNumbers && atomicMin(entry + i, static_cast<uint32_t>(j)) != ~0u) atomicOr(count + i, kTwice);
+            // Calls f(number, bias, entry, token) for this thread's biases of these tokens.
+            const auto each_number = [&](auto f) {
+                each_bias([&](int v, float b, int j) {
+                    const unsigned at = in_window(v);
+                    if (at >= window) return;
+                    const unsigned i = number(at);
+                    if (i < kNumbers) f(i, b, static_cast<uint32_t>(j), v);
+                });
+            };
+            bool again = false;  // this thread has an entry of a token that has another
+            each_number([&](unsigned i, float, uint32_t j, int) { again |= atomicMin(entry + i, j) != ~0u; });
+            int more = __syncthreads_count(again);
+            each_number([&](unsigned i, float b, uint32_t j, int) {
+                if (entry[i] == j) bias[i] = b;
             });
-            __syncthreads();
-            each_bias([&](int v, float b, int j) {
+            if (more == 0) return;
+            // Further entries: one of each token a round, as long as many tokens have some ...
+            constexpr uint32_t kAdded = ~1u;
+            do {
+                for (int i = tid; i < n; i += kThreads) later[i] = ~0u;
+                __syncthreads();
+                each_number([&](unsigned i, float, uint32_t j, int) {
+                    if (j > entry[i]) atomicMin(later + i, j);
+                });
+                __syncthreads();
+                bool added = false;
+                each_number([&](unsigned i, float b, uint32_t j, int) {
+                    if (later[i] != j) return;
+                    bias[i] = __fadd_rn(bias[i], b);
+                    entry[i] = j;
+                    later[i] = kAdded;
+                    added = true;
+                });
+                more = __syncthreads_count(added);
+            } while (more > 2 * kWarps);
+            if (more == 0) return;
+            // ... then the warp that has a token's last entry looks for the others, 32 at once.
+            for (int j0 = warp * 32; j0 < p.n_bias; j0 += kThreads) {
+                const int v = j0 + lane < p.n_bias ? token(bias_ids + j0 + lane) : kNowhere;
                 const unsigned at = in_window(v);
-                if (at >= window) return;
-                const unsigned i = number(at);
-                // The token's first entry adds the others.
-                if (i >= kNumbers || entry[i] != static_cast<uint32_t>(j)) return;
-                if (count[i] & kTwice)
-                    for (int l = j + 1; l < p.n_bias; ++l)
-                        if (__ldg(bias_ids + l) == v) b += __ldg(bias_values + l);
-                bias[i] = b;
-            });
+                unsigned i = kNumbers;
+                if (at < window) i = min(i, number(at));
+                const bool last = i < kNumbers && later[i] == kAdded && entry[i] == static_cast<uint32_t>(j0 + lane);
+                for (unsigned todo = __ballot_sync(0xffffffffu, last); todo; todo &= todo - 1) {
+                    const int from = __ffs(todo) - 1, it = __shfl_sync(0xffffffffu, v, from);
+                    const unsigned to = __shfl_sync(0xffffffffu, i, from);
+                    float b = bias[to];
+                    for (int l0 = j0 + from + 1; l0 < p.n_bias; l0 += 32) {
+                        const bool hit = l0 + lane < p.n_bias && __ldg(bias_ids + l0 + lane) == it;
+                        for (unsigned hits = __ballot_sync(0xffffffffu, hit); hits; hits &= hits - 1)
+                            b = __fadd_rn(b, __ldg(bias_values + l0 + __ffs(hits) - 1));
+                    }
+                    __syncwarp();
+                    if (lane == 0) bias[to] = b;
+                }
+            }
         };
         int numbers = 0;
         if (listing) {
@@ -561,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 const int v = w0 + list[i];
                 const uint32_t bits = mask ? __ldg(mask + v / 32) : ~0u;
                 float x = to_f32(in[v]);
-                x = penalised(x, count[i] & ~kTwice, theta, freq, pres);
+                x = penalised(x, count[i], theta, freq, pres);
                 if (biasing) x = __fadd_rn(x, bias[i]);
                 const bool ok = !none && ((bits >> (v % 32)) & 1);
                 if (CHOOSE) {
@@ -647,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
 template <typename T, bool CHOOSE>
 cudaError_t launch(const RuleParams& p, cudaStream_t stream) {
     static DeviceOnce once;
-    constexpr size_t kLists = kNumbers * 14;
+    constexpr size_t kLists = kNumbers * 18;
     const size_t bytes = p.history || p.n_bias > 0 ? kLists : 0;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -749,7 +787,7 @@ int prepare(Ctx* ctx, const char* who, const void* logits, int dtype, size_t ld,
         return bad("penalties without the tokens so far");
     }
     if (r.n_bias) {
-        if (!r.bias_ids || !r.bias || r.n_bias > (1u << 30) || r.bias_ld < r.n_bias || r.bias_ld > kMost)
+        if (!r.bias_ids || !r.bias || r.n_bias > (1u << 20) || r.bias_ld < r.n_bias || r.bias_ld > kMost)
             return bad("bad bias lists");
         p->bias_ids = r.bias_ids;
         p->bias = r.bias;

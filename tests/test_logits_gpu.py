@@ -296,6 +296,41 @@ def test_a_bias_for_every_token(ctx):
     check_choose(ctx, 2, 20000, "bf16", 4, history=40, biases=20000, states=3, seed=6)
 
 
+def test_too_many_biases_are_refused(ctx):
+    import torch
+    from telmo_b200 import Kernels, LogitRules, TelmoError
+    x, most = torch.zeros((1, 10), device="cuda"), 1 << 20
+    ids, bias = torch.full((1, most + 1), 3, dtype=torch.int32, device="cuda"), torch.zeros((1, most + 1), device="cuda")
+    bias[0, most - 1] = 2.5
+    for call in (lambda r: Kernels(ctx).constrain_logits(x, 10, 1, 10, r, x, 10),
+                 lambda r: Kernels(ctx).choose_tokens(x, 10, 1, 10, r, 1, ids)):
+        with pytest.raises(TelmoError):
+            call(LogitRules(bias_ids=ids, bias=bias))
+    Kernels(ctx).constrain_logits(x, 10, 1, 10, LogitRules(bias_ids=ids[:, :most], bias=bias[:, :most]), x, 10)
+    ctx.check()
+    assert x.tolist() == [[0, 0, 0, 2.5, 0, 0, 0, 0, 0, 0]]
+
+
+@pytest.mark.parametrize("times", [1, 2, 5])
+def test_biases_of_tokens_that_stand_several_times(ctx, times):
+    """Every token `times` times, some once more, one many times, in mixed order."""
+    import torch
+    from telmo_b200 import LogitRules
+    vocab, g = 5000, torch.Generator().manual_seed(9)
+    ids = torch.cat([torch.arange(vocab).repeat(times), torch.arange(0, vocab, 7), torch.full((300,), 77)])
+    ids = torch.stack([ids[torch.randperm(len(ids), generator=g)] for _ in range(3)]).int()
+    bias = torch.randn(ids.shape, generator=g)
+    logits = torch.randn((3, vocab), generator=g).cuda()
+    r = LogitRules(bias_ids=ids.cuda(), bias=bias.cuda())
+    check_choose(ctx, 3, vocab, "f32", 8, logits=logits, r=r)
+    from telmo_b200 import Kernels
+    x, tol = values(logits, vocab, r)
+    out = torch.empty_like(logits)
+    Kernels(ctx).constrain_logits(logits, vocab, 3, vocab, r, out, vocab)
+    ctx.check()
+    assert (np.abs(out.double().cpu().numpy() - x) <= tol).all()
+
+
 @pytest.mark.parametrize("rows,vocab,history,biases", [(3, 9001, 9000, 2500), (2, 40000, 30000, 3000), (500, 33000, 9000, 0),
                                                        (200, 65540, 12000, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
