@@ -335,7 +335,9 @@ def test_biases_of_tokens_that_stand_several_times(ctx, times):
                                                        (200, 65540, 12000, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_more_listed_tokens_than_numbers(ctx, rows, vocab, history, biases, dtype):
-    """Thousands of listed tokens in every window, which are numbered 2048 at a time."""
+    """Thousands of listed tokens in every window, which are numbered 2048 at a time. (Where one block has a row of
+    65540, a thread adds up to 150 values: 150 2^-24 in place of 2^-17 adds 1.4e-6 to the bound on a log-probability;
+    the values' own bound, at least 2 * 5 * 2^-24 * 4 there, covers it.)"""
     check_constrain(ctx, rows, vocab, dtype, history=history, biases=biases, states=3, seed=5)
     check_choose(ctx, rows, vocab, dtype, 5, history=history, biases=biases, states=3, seed=5)
 
