@@ -89,7 +89,8 @@ def _refuse(message: str):
 def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
     """The address of a [rows, cols] matrix with rows `ld` elements apart that starts at tensor `t`,
     which must lie on the context's device, be of one of `dtypes` and reach to the last element. A
-    view with gaps must have its own rows `ld` apart and its elements next to one another."""
+    view with gaps must have that many rows itself, `ld` apart, and their elements next to one
+    another."""
     if t.get_device() != ctx.device:  # -1 in host memory
         _refuse(f"{name}: a tensor on {t.device}, the context is on cuda:{ctx.device}")
     if t.dtype not in dtypes:
@@ -99,14 +100,28 @@ def _matrix(ctx, t, name: str, dtypes, rows: int, cols: int, ld: int) -> int:
             _refuse(f"{name}: rows {ld} elements apart hold no {cols} elements")
         if t.is_contiguous():
             have = t.numel()
-        else:
-            if t.stride(-1) != 1 or cols > t.shape[-1] or (rows > 1 and t.stride(-2) != ld):
-                _refuse(f"{name}: {list(t.shape)} with strides {list(t.stride())} has no rows of {cols} "
-                        f"elements, {ld} apart")
-            have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-        if have < (rows - 1) * ld + cols:
-            _refuse(f"{name}: {have} elements, {(rows - 1) * ld + cols} are needed")
+            if have < (rows - 1) * ld + cols:
+                _refuse(f"{name}: {have} elements, {(rows - 1) * ld + cols} are needed")
+        elif not _has_rows(t.shape, t.stride(), rows, cols, ld):
+            _refuse(f"{name}: {list(t.shape)} with strides {list(t.stride())} has no {rows} rows of {cols} "
+                    f"elements, {ld} apart")
     return t.data_ptr()
+
+
+def _has_rows(shape, strides, rows: int, cols: int, ld: int) -> bool:
+    """Whether a view's first `rows` rows (all its dimensions but the last, in order) lie `ld` elements
+    apart and hold `cols` elements next to one another. Dimensions behind the last row that is used
+    may lie anywhere."""
+    if strides[-1] != 1 or cols > shape[-1]:
+        return False
+    have = 1  # rows that the dimensions so far hold
+    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if have >= rows:
+            break
+        if size != 1 and stride != ld * have:
+            return False
+        have *= size
+    return have >= rows
 
 
 @functools.lru_cache(maxsize=None)
