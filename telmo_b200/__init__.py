@@ -124,6 +124,28 @@ def _has_rows(shape, strides, rows: int, cols: int, ld: int) -> bool:
     return have >= rows
 
 
+def _vector(ctx, t, name: str, dtypes, rows: int) -> int:
+    """The address of a value per row, or 0 where there is no tensor."""
+    if t is None:
+        return 0
+    if t.get_device() == ctx.device and t.dtype in dtypes and t.numel() >= rows and t.is_contiguous():
+        return t.data_ptr()
+    return _matrix(ctx, t, name, dtypes, 1, rows, rows)  # says what is wrong
+
+
+def _table(ctx, t, name: str, dtypes, least_rows: int, least_cols: int) -> tuple:
+    """The rows, address, columns and row distance of a matrix of at least that size."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or strides[1] != 1 or shape[0] < least_rows or shape[1] < least_cols:
+        _refuse(f"{name}: a matrix of at least [{least_rows}, {least_cols}] with unit stride "
+                f"along its rows, not {list(shape)}")
+    rows, cols = shape
+    ld = strides[0] if rows > 1 else max(cols, 1)
+    if ld < cols or t.get_device() != ctx.device or t.dtype not in dtypes:
+        _matrix(ctx, t, name, dtypes, rows, cols, ld)  # says what is wrong
+    return rows, t.data_ptr(), cols, ld
+
+
 @functools.lru_cache(maxsize=None)
 def _float_types() -> dict:
     """torch dtype -> TELMO_DTYPE_* of the entry points that take f32, bf16 and f16."""
@@ -141,6 +163,12 @@ def _f32_only() -> tuple:
 def _i32_only() -> tuple:
     import torch
     return (torch.int32,)
+
+
+@functools.lru_cache(maxsize=None)
+def _mask_types() -> tuple:
+    import torch
+    return (torch.int32, torch.uint32)
 
 
 def _stream_on(ctx, stream) -> Optional[int]:
@@ -313,74 +341,43 @@ class LogitRules:
     allowed: Optional[object] = None      # int32 (or uint32) [states, ceil(vocab / 32)] bit masks
     state: Optional[object] = None        # int32 [rows], negative: no mask; None: row r has mask r
 
-    def __post_init__(self):
-        self._checked = None  # the last structure, and what it was made of
-
-    def _struct(self, ctx, rows: int, vocab: int) -> "_lib.LogitRules":
-        """The checked C structure. It is made again unless the call's sizes, the tensors and their
-        addresses and element counts are those of the last call."""
-        tensors = (self.history, self.history_len, self.repetition, self.frequency, self.presence,
-                   self.bias_ids, self.bias, self.allowed, self.state)
-        if self._checked is not None:
-            device, r, v, known, s = self._checked
-            if device == ctx.device and r == rows and v == vocab:
-                for t, (u, address, count) in zip(tensors, known):
-                    if t is not u or (t is not None and (t.data_ptr() != address or t.numel() != count)):
-                        break
-                else:
-                    return s
-        s = self._check(ctx, rows, vocab)
-        known = tuple((t, None if t is None else t.data_ptr(), None if t is None else t.numel())
-                      for t in tensors)
-        self._checked = (ctx.device, rows, vocab, known, s)
-        return s
-
-    def _check(self, ctx, rows: int, vocab: int) -> "_lib.LogitRules":
-        import torch
-        i32, f32 = (torch.int32,), (torch.float32,)
-
-        def row(t, name, types):
-            return None if t is None else _matrix(ctx, t, name, types, 1, rows, rows)
-
-        def table(t, name, types, least_rows, least_cols):
-            if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < least_rows or t.shape[1] < least_cols:
-                _refuse(f"{name}: a matrix of at least [{least_rows}, {least_cols}] with unit stride "
-                        f"along its rows, not {list(t.shape)}")
-            ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-            return _matrix(ctx, t, name, types, t.shape[0], t.shape[1], ld), ld
-
-        s = _lib.LogitRules()
-        if self.history is not None:
+    def _struct(self, ctx, rows: int, vocab: int) -> bytes:
+        """The C structure's bytes, checked and made anew for each call: a tensor may have been reshaped
+        in place since the last one (6 us with all rules; comparing what a kept one was made of would
+        read as much of each tensor)."""
+        i32, f32 = _i32_only(), _f32_only()
+        h, ids, masks = self.history, self.bias_ids, self.allowed
+        history = n_history = history_ld = said = theta = freq = pres = 0
+        bias = n_bias = bias_ld = n_states = masks_ld = state = 0
+        if h is not None:
             if self.history_len is None:
                 _refuse("history: its lengths are missing")
-            s.history, s.history_ld = table(self.history, "history", i32, rows, 0)
-            s.n_history = self.history.shape[1]
-            s.history_len = row(self.history_len, "history_len", i32)
-            s.repetition = row(self.repetition, "repetition", f32)
-            s.frequency = row(self.frequency, "frequency", f32)
-            s.presence = row(self.presence, "presence", f32)
-            if s.n_history == 0:  # an empty tensor has no address; without tokens no penalty applies
-                s.history = s.repetition = s.frequency = s.presence = None
+            history, n_history, history_ld = _table(ctx, h, "history", i32, rows, 0)[1:]
+            said = _vector(ctx, self.history_len, "history_len", i32, rows)
+            theta = _vector(ctx, self.repetition, "repetition", f32, rows)
+            freq = _vector(ctx, self.frequency, "frequency", f32, rows)
+            pres = _vector(ctx, self.presence, "presence", f32, rows)
+            if n_history == 0:  # an empty tensor has no address; without tokens no penalty applies
+                history = theta = freq = pres = 0
         elif not (self.history_len is self.repetition is self.frequency is self.presence is None):
             _refuse("penalties need the tokens so far (history)")
-        if self.bias_ids is not None or self.bias is not None:
-            if self.bias_ids is None or self.bias is None or self.bias_ids.shape != self.bias.shape:
+        if ids is not None or self.bias is not None:
+            if ids is None or self.bias is None or ids.shape != self.bias.shape:
                 _refuse("bias_ids and bias are two matrices of one shape")
-            s.bias_ids, s.bias_ld = table(self.bias_ids, "bias_ids", i32, rows, 0)
-            s.bias, ld = table(self.bias, "bias", f32, rows, 0)
-            if ld != s.bias_ld:
+            ids, n_bias, bias_ld = _table(ctx, ids, "bias_ids", i32, rows, 0)[1:]
+            bias, _, ld = _table(ctx, self.bias, "bias", f32, rows, 0)[1:]
+            if ld != bias_ld:
                 _refuse("bias_ids and bias must have the same stride")
-            s.n_bias = self.bias.shape[1]
-        if self.allowed is not None:
-            s.allowed, s.allowed_ld = table(self.allowed, "allowed", (torch.int32, torch.uint32), 1,
-                                            -(-vocab // 32))
-            s.n_states = self.allowed.shape[0]
-            s.state = row(self.state, "state", i32)
-            if self.state is None and s.n_states < rows:
-                _refuse(f"{s.n_states} masks for {rows} rows, and no states")
+        if masks is not None:
+            n_states, masks, _, masks_ld = _table(ctx, masks, "allowed", _mask_types(), 1, -(-vocab // 32))
+            if self.state is not None:
+                state = _vector(ctx, self.state, "state", i32, rows)
+            elif n_states < rows:
+                _refuse(f"{n_states} masks for {rows} rows, and no states")
         elif self.state is not None:
             _refuse("state needs the masks (allowed)")
-        return s
+        return _lib.LOGIT_RULES.pack(history, n_history, history_ld, said, theta, freq, pres, ids or 0, bias, n_bias,
+                                     bias_ld, masks or 0, n_states, masks_ld, state)
 
 
 class Kernels:
@@ -437,7 +434,7 @@ class Kernels:
         types = _float_types()
         pl = _matrix(self.ctx, logits, "logits", types, rows, vocab, ld)
         po = _matrix(self.ctx, out, "out", (logits.dtype,), rows, vocab, out_ld)
-        st = None if rules is None else ctypes.byref(rules._struct(self.ctx, rows, vocab))
+        st = None if rules is None else rules._struct(self.ctx, rows, vocab)
         check(_lib.load().telmo_logits_constrain(self.ctx.handle, pl, types[logits.dtype], ld, rows,
                                                  vocab, st, po, out_ld, _stream_on(self.ctx, stream)),
               self.ctx.handle)
@@ -451,7 +448,7 @@ class Kernels:
         pl = _matrix(self.ctx, logits, "logits", types, rows, vocab, ld)
         pi = _matrix(self.ctx, ids, "ids", _i32_only(), rows, k, k)
         pp = None if logprobs is None else _matrix(self.ctx, logprobs, "logprobs", _f32_only(), rows, k, k)
-        st = None if rules is None else ctypes.byref(rules._struct(self.ctx, rows, vocab))
+        st = None if rules is None else rules._struct(self.ctx, rows, vocab)
         check(_lib.load().telmo_logits_choose(self.ctx.handle, pl, types[logits.dtype], ld, rows, vocab,
                                               st, k, pi, pp, _stream_on(self.ctx, stream)),
               self.ctx.handle)

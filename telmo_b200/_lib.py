@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtelmo_b200.so")
@@ -58,6 +59,10 @@ class LogitRules(ctypes.Structure):
                 ("frequency", _vp), ("presence", _vp), ("bias_ids", _vp), ("bias", _vp),
                 ("n_bias", _sz), ("bias_ld", _sz), ("allowed", _vp), ("n_states", _sz),
                 ("allowed_ld", _sz), ("state", _vp)]
+
+
+# The same as bytes: pointers and sizes of 8 bytes each, in the order of the fields.
+LOGIT_RULES = struct.Struct(f"{len(LogitRules._fields_)}Q")
 
 
 # name -> (restype, argtypes); every function include/telmo_b200.h declares.

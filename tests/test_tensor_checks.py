@@ -79,3 +79,100 @@ def test_outputs_leave_what_lies_outside_a_view(ctx):
     assert (cube[0, :5, :16] != 7).all() and (cube[0, 5:, :16] == 7).all() and (cube[1, :, :16] == 7).all()
     assert (cube[:, :, 16:32] != 7).all() and (cube[:, :, 32:] == 7).all()
     w.free()
+
+
+def rules_of(r, rows, vocab):
+    """The C structure that a call with these sizes would pass."""
+    return telmo_b200._lib.LogitRules.from_buffer_copy(r._struct(Host(), rows, vocab))
+
+
+def test_rules_are_read_anew_in_each_call():
+    """Tensors reshaped in place between two calls, with the same address and as many elements as before."""
+    import torch
+    from telmo_b200 import LogitRules
+    ids, bias = torch.zeros((4, 6), dtype=torch.int32), torch.zeros((4, 6))
+    r = LogitRules(bias_ids=ids, bias=bias)
+    s = rules_of(r, 4, 100)
+    assert (s.n_bias, s.bias_ld, s.bias_ids, s.bias) == (6, 6, ids.data_ptr(), bias.data_ptr())
+    ids.resize_(6, 4), bias.resize_(6, 4)
+    s = rules_of(r, 4, 100)
+    assert (s.n_bias, s.bias_ld) == (4, 4)
+    ids.t_(), bias.t_()
+    with pytest.raises(TelmoError):
+        rules_of(r, 4, 100)
+
+    history, n = torch.zeros((4, 8), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    theta = torch.ones(8)
+    r = LogitRules(history=history, history_len=n, repetition=theta)
+    s = rules_of(r, 4, 100)
+    assert (s.n_history, s.history_ld, s.history, s.history_len) == (8, 8, history.data_ptr(), n.data_ptr())
+    assert s.repetition == theta.data_ptr() and not s.frequency and not s.presence and not s.state
+    history.as_strided_((4, 4), (8, 1))
+    s = rules_of(r, 4, 100)
+    assert (s.n_history, s.history_ld) == (4, 8)
+    theta.as_strided_((4,), (2,))
+    with pytest.raises(TelmoError):
+        rules_of(r, 4, 100)
+    r.repetition = None
+    rules_of(r, 4, 100)
+    history.data = history.data.view(torch.float32)
+    with pytest.raises(TelmoError):
+        rules_of(r, 4, 100)
+
+    masks, state = torch.zeros((4, 4), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    r = LogitRules(allowed=masks, state=state)
+    s = rules_of(r, 4, 128)
+    assert (s.allowed, s.n_states, s.allowed_ld, s.state) == (masks.data_ptr(), 4, 4, state.data_ptr())
+    masks.resize_(2, 8)
+    s = rules_of(r, 4, 128)
+    assert (s.n_states, s.allowed_ld) == (2, 8)
+    state.resize_(3)
+    with pytest.raises(TelmoError):
+        rules_of(r, 4, 128)
+
+
+def test_rules_on_the_host_are_refused_one_by_one():
+    """Each of the nine tensors with a fault of its own."""
+    import torch
+    from telmo_b200 import LogitRules
+    i32 = dict(dtype=torch.int32)
+    table, vec, f, m = torch.zeros((4, 5), **i32), torch.zeros(4, **i32), torch.ones(4), torch.zeros((4, 4), **i32)
+    good = dict(history=table, history_len=vec, repetition=f, frequency=f, presence=f, bias_ids=table,
+                bias=torch.zeros((4, 5)), allowed=m, state=vec)
+    rules_of(LogitRules(**good), 4, 100)
+    for name, t in good.items():
+        wrong = [t.double(), t[:3]]
+        if t.dim() == 1:
+            wrong += [torch.stack((t, t), dim=1)[:, 0]]
+        else:
+            wrong += [t.t().contiguous().t(), t[:1].expand(4, -1), t.flatten()]
+        for bad in wrong:
+            if name == "allowed" and bad.shape[0] == 3 and bad.dim() == 2:
+                continue  # fewer masks than rows will do where there are states
+            with pytest.raises(TelmoError):
+                rules_of(LogitRules(**{**good, name: bad}), 4, 100)
+    for absent in ("history", "history_len", "bias_ids", "bias", "allowed"):
+        with pytest.raises(TelmoError):
+            rules_of(LogitRules(**{**good, absent: None}), 4, 100)
+    assert bytes(rules_of(LogitRules(), 4, 100)) == bytes(120)
+    with pytest.raises(TelmoError):  # on another device than the context's
+        LogitRules(**good)._struct(types.SimpleNamespace(device=0), 4, 100)
+
+
+@pytest.mark.gpu
+def test_rules_reshaped_between_two_calls(ctx):
+    """The same lists as [4, 6] and then as [6, 4], against new ones of that shape."""
+    import torch
+    from telmo_b200 import Kernels, LogitRules
+    k, g = Kernels(ctx), torch.Generator().manual_seed(5)
+    ids = torch.randint(0, 50, (4, 6), generator=g, dtype=torch.int32).cuda()
+    bias = torch.randn((4, 6), generator=g).cuda()
+    x = torch.randn((4, 50), generator=g).cuda()
+    got, want = torch.empty_like(x), torch.empty_like(x)
+    r = LogitRules(bias_ids=ids, bias=bias)
+    for shape in ((4, 6), (6, 4), (4, 6)):
+        ids.resize_(shape), bias.resize_(shape)
+        k.constrain_logits(x, 50, 4, 50, r, got, 50)
+        k.constrain_logits(x, 50, 4, 50, LogitRules(bias_ids=ids.clone(), bias=bias.clone()), want, 50)
+        ctx.check()
+        assert torch.equal(got, want)
