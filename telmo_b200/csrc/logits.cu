@@ -21,9 +21,9 @@
 //              join the others.
 // A block walks over windows of 8192 to 65536 tokens: it sets a bit for each listed token's place, numbers
 // the bits in order (a prefix sum over the words' counts), and counts by number in shared memory with
-// integer atomics (the counts do not depend on their order); a token's biases add up in list order, an
-// entry a round where many tokens have several, else by a search from the first. Tokens go to threads by number, so no sum depends on timing. Numbers beyond
-// kNumbers come in further rounds over the lists. With the rules inside the pass over the logits some lane
+// integer atomics (the counts do not depend on their order); a token's biases add up in list order, the
+// first ones an entry a round, further ones by one walk over the list. Tokens go to threads by number, so no sum
+// depends on timing. Numbers beyond kNumbers come in further rounds over the lists. With the rules inside the pass over the logits some lane
 // of a warp nearly always had a listed token and all paid: 92 us for 256 rows of 131072 bf16 values with
 // 2000 tokens each, which take 50 us here (93 MB read and written; the pass alone 30 us).
 //
@@ -56,6 +56,10 @@ constexpr int kPerThread = kTile / 8 / kThreads;   // groups of eight tokens a t
 constexpr int kMostWindow = 8 * kTile;             // tokens per window at most
 constexpr int kNumbers = 2048;                     // listed tokens with a number
 constexpr int kMaxK = 8;
+// Rounds over a list of biases that give each token its next one, before a walk over the whole list adds the rest.
+// (256 entries, each token twice, 64 rows: 7.8 us with two rounds, 10.2 with none; 4096 entries of 64 tokens: 91 us
+// with two, 125 with sixteen, 233 with as many as there are entries of a token, which is quadratic.)
+constexpr int kBiasRounds = 2;
 constexpr int kBuffer = 1024;                      // keys a block keeps before it raises its bound
 constexpr float kLowest = -3.402823466e38f;
 
@@ -289,9 +293,10 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
     constexpr int kNowhere = INT_MIN;
     int said = 0;
     float theta = 1.0f, freq = 0.0f, pres = 0.0f;
-    const int32_t* history = counting ? p.history + static_cast<int64_t>(row) * p.history_ld : nullptr;
-    const int32_t* bias_ids = biasing ? p.bias_ids + static_cast<int64_t>(row) * p.bias_ld : nullptr;
-    const float* bias_values = biasing ? p.bias + static_cast<int64_t>(row) * p.bias_ld : nullptr;
+    // Made again where they are used, which is cheaper than three pointers kept through the pass.
+    const auto history = [&] { return p.history + static_cast<int64_t>(row) * p.history_ld; };
+    const auto bias_ids = [&] { return p.bias_ids + static_cast<int64_t>(row) * p.bias_ld; };
+    const auto bias_values = [&] { return p.bias + static_cast<int64_t>(row) * p.bias_ld; };
     const auto token = [&](const int32_t* list_at) {
         const int v = __ldg(list_at);
         return v >= 0 && v < p.vocab ? v : kNowhere;
@@ -303,17 +308,17 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
         if (p.presence) pres = __ldg(p.presence + row);
     }
     // Calls f(token) for each of this thread's tokens so far, f(token, bias, entry) for its biases.
-    const int first_said = tid < said ? token(history + tid) : kNowhere;
+    const int first_said = tid < said ? token(history() + tid) : kNowhere;
     const auto each_said = [&](auto f) {
         f(first_said);
 #pragma unroll 4
-        for (int i = tid + kThreads; i < said; i += kThreads) f(token(history + i));
+        for (int i = tid + kThreads; i < said; i += kThreads) f(token(history() + i));
     };
-    const int first_biased = biasing && tid < p.n_bias ? token(bias_ids + tid) : kNowhere;
+    const int first_biased = biasing && tid < p.n_bias ? token(bias_ids() + tid) : kNowhere;
     const auto each_bias = [&](auto f) {
         if (!biasing) return;
-        f(first_biased, tid < p.n_bias ? __ldg(bias_values + tid) : 0.0f, tid);
-        for (int i = tid + kThreads; i < p.n_bias; i += kThreads) f(token(bias_ids + i), __ldg(bias_values + i), i);
+        f(first_biased, tid < p.n_bias ? __ldg(bias_values() + tid) : 0.0f, tid);
+        for (int i = tid + kThreads; i < p.n_bias; i += kThreads) f(token(bias_ids() + i), __ldg(bias_values() + i), i);
     };
 
     const uint32_t* mask = nullptr;
@@ -464,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                 if (entry[i] == j) bias[i] = b;
             });
             if (more == 0) return;
-            // Further entries: one of each token a round, as long as many tokens have some ...
-            constexpr uint32_t kAdded = ~1u;
-            do {
+            __syncthreads();
+            // Further entries: one of each token a round, while many threads find some, ...
+            for (int round = 0; round < kBiasRounds && more > 2 * kWarps; ++round) {
                 for (int i = tid; i < n; i += kThreads) later[i] = ~0u;
                 __syncthreads();
                 each_number([&](unsigned i, float, uint32_t j, int) {
@@ -478,31 +483,35 @@ __global__ void __launch_bounds__(kThreads, CHOOSE ? 2 : 3) logits_kernel(const 
                     if (later[i] != j) return;
                     bias[i] = __fadd_rn(bias[i], b);
                     entry[i] = j;
-                    later[i] = kAdded;
                     added = true;
                 });
                 more = __syncthreads_count(added);
-            } while (more > 2 * kWarps);
+            }
             if (more == 0) return;
-            // ... then the warp that has a token's last entry looks for the others, 32 at once.
-            for (int j0 = warp * 32; j0 < p.n_bias; j0 += kThreads) {
-                const int v = j0 + lane < p.n_bias ? token(bias_ids + j0 + lane) : kNowhere;
-                const unsigned at = in_window(v);
+            // ... then every warp walks over the list once, 32 entries at a time, and adds what is left of the tokens
+            // whose number is its own modulo the warps: the lowest lane of a token takes its lanes' values in order.
+            const auto id_at = [&](int j) { return j < p.n_bias ? __ldg(bias_ids() + j) : -1; };
+            int next = id_at(lane);
+            for (int j0 = 0; j0 < p.n_bias; j0 += 32) {
+                const int j = j0 + lane, v = next;
+                next = id_at(j + 32);
+                const unsigned at = v < p.vocab ? in_window(v) : ~0u;
                 unsigned i = kNumbers;
                 if (at < window) i = min(i, number(at));
-                const bool last = i < kNumbers && later[i] == kAdded && entry[i] == static_cast<uint32_t>(j0 + lane);
-                for (unsigned todo = __ballot_sync(0xffffffffu, last); todo; todo &= todo - 1) {
-                    const int from = __ffs(todo) - 1, it = __shfl_sync(0xffffffffu, v, from);
-                    const unsigned to = __shfl_sync(0xffffffffu, i, from);
-                    float b = bias[to];
-                    for (int l0 = j0 + from + 1; l0 < p.n_bias; l0 += 32) {
-                        const bool hit = l0 + lane < p.n_bias && __ldg(bias_ids + l0 + lane) == it;
-                        for (unsigned hits = __ballot_sync(0xffffffffu, hit); hits; hits &= hits - 1)
-                            b = __fadd_rn(b, __ldg(bias_values + l0 + __ffs(hits) - 1));
-                    }
-                    __syncwarp();
-                    if (lane == 0) bias[to] = b;
+                const bool mine = i < kNumbers && i % kWarps == warp && static_cast<uint32_t>(j) > entry[i];
+                if (!__any_sync(0xffffffffu, mine)) continue;
+                const float b = mine ? __ldg(bias_values() + j) : 0.0f;
+                const unsigned lanes = __match_any_sync(0xffffffffu, mine ? i : kNumbers + lane);
+                const bool lowest = mine && lane == __ffs(lanes) - 1;
+                unsigned todo = lowest ? lanes : 0u;
+                float sum = lowest ? bias[i] : 0.0f;
+                for (unsigned most = __reduce_max_sync(0xffffffffu, __popc(todo)); most; --most) {
+                    const float x = __shfl_sync(0xffffffffu, b, todo ? __ffs(todo) - 1 : lane);
+                    if (todo) sum = __fadd_rn(sum, x);
+                    todo &= todo - 1;
                 }
+                if (lowest) bias[i] = sum;
+                __syncwarp();
             }
         };
         int numbers = 0;

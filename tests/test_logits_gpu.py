@@ -331,6 +331,38 @@ def test_biases_of_tokens_that_stand_several_times(ctx, times):
     assert (np.abs(out.double().cpu().numpy() - x) <= tol).all()
 
 
+@pytest.mark.parametrize("tokens,times", [(2, 3), (40, 3), (33, 40), (64, 300), (700, 30), (5000, 20), (64, 16384), (1, 1 << 20)])
+@pytest.mark.parametrize("order", ["mixed", "in turn", "in runs"])
+def test_some_tokens_very_many_times(ctx, tokens, times, order):
+    """Biases of each token add up one after another, in list order: the very bits of that. The longest lists take
+    milliseconds (2^20 entries are read a bounded number of times, not once for each time a token stands there)."""
+    import torch
+    from telmo_b200 import Kernels, LogitRules
+    vocab, g = 9000, np.random.default_rng(tokens)
+    names = g.permutation(vocab)[:tokens]
+    ids = np.repeat(names, times) if order == "in runs" else np.tile(names, times)
+    if order == "mixed":
+        ids = g.permutation(ids)
+    bias = g.standard_normal(len(ids)).astype(np.float32)
+    x = g.standard_normal((1, vocab)).astype(np.float32)
+    want = x.copy()
+    for v in names:
+        want[0, v] += np.cumsum(bias[ids == v], dtype=np.float32)[-1]
+    r = LogitRules(bias_ids=torch.from_numpy(ids.astype(np.int32))[None].cuda(), bias=torch.from_numpy(bias)[None].cuda())
+    logits = torch.from_numpy(x).cuda()
+    out, best = torch.empty_like(logits), torch.zeros((1, 4), dtype=torch.int32, device="cuda")
+    k = Kernels(ctx)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    k.constrain_logits(logits, vocab, 1, vocab, r, out, vocab)
+    k.choose_tokens(logits, vocab, 1, vocab, r, 4, best)
+    end.record()
+    ctx.check()
+    assert np.array_equal(out.cpu().numpy().view(np.int32), want.view(np.int32))
+    assert best[0].tolist() == np.argsort(-want[0], kind="stable")[:4].tolist()
+    assert begin.elapsed_time(end) < 200  # ms
+
+
 @pytest.mark.parametrize("rows,vocab,history,biases", [(3, 9001, 9000, 2500), (2, 40000, 30000, 3000), (500, 33000, 9000, 0),
                                                        (200, 65540, 12000, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
