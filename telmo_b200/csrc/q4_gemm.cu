@@ -126,18 +126,42 @@ __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// Arrives on a barrier of either CTA of the pair. What it announces is shared memory that the
-// arriving warp's own SM will read (each lane's fence.proxy.async comes first) or TMEM that it has
-// finished reading, so no release at cluster scope is needed; one cost a membar of about 1000 cycles
-// per step (prompt of 4096 rows, 4096 -> 8192: 452 us with it, 289 without).
+// Arrives on a barrier of either CTA of the pair. With DATA it announces what the arriving CTA's threads wrote to
+// their shared memory (each lane's fence.proxy.async comes first) to an instruction that the other CTA issues, so
+// the release is at cluster scope. It is restricted to this CTA's shared memory: a full one also waits for the
+// epilogue's stores to global memory (4096 rows, 4096 -> 8192: 218 us with this one, 320 with a full one). Without
+// DATA it says that TMEM has been read, which the tcgen05 fences around an arrival and a wait order.
+template <bool DATA>
 __device__ __forceinline__ void arrive_pair(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    if (DATA) asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 // mbar_wait with a longer run of polls before it sleeps: these waits are short and follow one another.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kWaitPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
+        if (i > 4096) __nanosleep(256);
+    }
+    return false;
+}
+
+// The same for a barrier on which the other CTA of a pair arrives, or its products; with DATA what arrive_pair
+// releases is acquired.
+template <int CG, bool DATA>
+__device__ __forceinline__ bool wait_for_pair(uint64_t* bar, uint32_t parity) {
+    if (CG == 1) return wait_for(bar, parity);
+    for (uint32_t i = 0; i < kWaitPolls; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) {
+            if (DATA) asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+            return true;
+        }
         if (i > 4096) __nanosleep(256);
     }
     return false;
@@ -251,7 +275,7 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
                                               : *zs * 0x01010101u;
                 }
             }
-            if (!wait_for(&empty[st.at], st.phase ^ 1)) return false;
+            if (!wait_for_pair<CG, true>(&empty[st.at], st.phase ^ 1)) return false;
             const uint32_t a = stage0 + st.at * STAGE_BYTES;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -272,7 +296,7 @@ __device__ __forceinline__ bool dequant_role(const GemmParams& p, uint8_t* smem,
             __syncwarp();
             if (lane == 0) {
                 if (CG == 1) mbar_arrive(&full[st.at]);
-                else arrive_pair(full0 + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
+                else arrive_pair<true>(full0 + static_cast<uint32_t>(st.at * sizeof(uint64_t)));
                 // Only now: the codes have reached registers, since their operands are stored.
                 mbar_arrive(&code_empty[cs.at]);
             }
@@ -298,13 +322,13 @@ __device__ __forceinline__ bool issue_role(const GemmParams& p, uint8_t* smem, u
     const uint64_t a0 = sw128_desc(smem_u32(smem)), b0 = sw128_desc(smem_u32(smem) + 2 * kAHalf);
     for (int t = first; t < p.tiles; t += stride) {
         for (int c = c0; c < c1; ++c) {
-            if (!wait_for(&full[st.at], st.phase)) return false;
+            if (!wait_for_pair<CG, true>(&full[st.at], st.phase)) return false;
             tc_fence_after();
             const uint64_t off = static_cast<uint64_t>(st.at * S::kStageBytes) >> 4;
 #pragma unroll
             for (int q = 0; q < PER_CHUNK; ++q) {
                 if (q > 0 && c * 128 + q * (128 / PER_CHUNK) >= p.k) break;
-                if (!wait_for(&acc_empty[acc.at], acc.phase ^ 1)) return false;
+                if (!wait_for_pair<CG, false>(&acc_empty[acc.at], acc.phase ^ 1)) return false;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * BN);
                 if (issuer) {
@@ -411,7 +435,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
             for (int t = first; t < p.tiles && ok; t += stride) {
                 const int m0 = t / p.num_n * BN + pair * S::kBRows;
                 for (int c = c0; c < c1; ++c) {
-                    if (!(ok = wait_for(&empty[st.at], st.phase ^ 1))) break;
+                    if (!(ok = wait_for_pair<CG, true>(&empty[st.at], st.phase ^ 1))) break;
                     uint8_t* b = smem + st.at * S::kStageBytes + 2 * kAHalf;
                     // Both CTAs' loads of a pair count on the first CTA's barrier, which expects them all.
                     const uint32_t bar = CG == 2 ? cluster_addr(&full[st.at], 0) : 0;
@@ -498,7 +522,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
                 __syncwarp();
                 if (lane == 0) {
                     if (CG == 1) mbar_arrive(&acc_empty[ab.at]);
-                    else arrive_pair(acc_empty0 + static_cast<uint32_t>(ab.at * sizeof(uint64_t)));
+                    else arrive_pair<false>(acc_empty0 + static_cast<uint32_t>(ab.at * sizeof(uint64_t)));
                 }
                 ab.next();
             };
@@ -510,7 +534,7 @@ q4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const GemmParams p) {
 #pragma unroll 1
                 for (int i = 0; i < left && i < 128; i += size, now >>= 16) {
                     const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(now & 0xffff)));
-                    ok = wait_for(&acc_full[ab.at], ab.phase);
+                    ok = wait_for_pair<CG, false>(&acc_full[ab.at], ab.phase);
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
                         break;
