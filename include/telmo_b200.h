@@ -123,11 +123,19 @@ int telmo_linear(telmo_ctx *ctx, const float *a, size_t lda, size_t m, const tel
 
 /* telmo_linear with 4-bit weights (telmo_weights_upload_q4) and activations of a_dtype (F32, BF16 or
  * F16), c of c_dtype (the same three): the same Epilogue, c[m, n] = (accumulate ? c : 0) + scale *
- * act(a[m, k] . w^T + bias). Activations are not quantized: bf16 and fp16 are multiplied as they
- * are and f32 to at least 22 significant bits, codes exactly, sums and scales in f32; c is rounded
- * once. A row of a that holds an infinity or a NaN gives outputs that are not finite in that row
- * alone. a and c need no more than their elements' alignment; rows that start on 16-byte
- * boundaries are read fastest. a and c must not overlap (TELMO_ERR_ARGUMENT). */
+ * act(a[m, k] . w^T + bias). Codes are multiplied exactly, sums and scales are f32, c is rounded
+ * once. Activations are not quantized to the weights' size. How an element x of a enters depends on
+ * m, with A the largest |x| of its row:
+ *   m <= 2    to 2^-55 A (fixed point; f16 exactly);
+ *   m <= 8    as it is (f32 parts below 2^-126 vanish);
+ *   m > 8     bf16 and f16 as they are; f32 to the larger of 2^-22 |x| and 2^-39 A: 22 bits down to
+ *             2^-17 A, fewer below (two f16 planes under a power of two per row).
+ * So a row's last bits may depend on how many rows come with it, and where one f32 activation is more
+ * than 2^17 times the others while its weights are 0, the others keep fewer than 22 bits from
+ * nine rows on. A row of a that holds an infinity or a NaN has sums that are not finite in that row
+ * alone (TELMO_ACT_RELU makes 0 of -infinity). a and c need no more than their elements'
+ * alignment; rows that start on 16-byte boundaries are read fastest. a and c must not overlap
+ * (TELMO_ERR_ARGUMENT). */
 int telmo_linear_q4(telmo_ctx *ctx, const void *a, int a_dtype, size_t lda, size_t m,
                     const telmo_weights *w, const float *bias, int act, float scale, int accumulate,
                     void *c, int c_dtype, size_t ldc, void *stream);

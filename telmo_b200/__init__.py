@@ -385,7 +385,8 @@ class Kernels:
     packed int8 weights, with the reference's Epilogue. Tensors are torch CUDA tensors.
 
     With Q4 weights ``a`` and ``c`` may each be f32, bf16 or f16 and must lie on the context's
-    device; ``stream`` defaults to torch's current stream there."""
+    device; ``stream`` defaults to torch's current stream there. What is kept of small activations
+    beside large ones depends on the type and on m (telmo_linear_q4)."""
 
     def __init__(self, ctx: Context):
         self.ctx = ctx

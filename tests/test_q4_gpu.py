@@ -436,3 +436,68 @@ def test_each_product_reads_the_one_before(ctx, m, k, dtype):
     del graph
     for d in devs:
         d.free()
+
+
+def weights_without(ctx, n, k, j, seed):
+    """Weights in which input j of every output is 0: its code is the zero point."""
+    from telmo_b200 import PackedWeights, Precision
+    from test_q4 import decode
+    g = np.random.default_rng(seed)
+    z = g.integers(0, 16, (n, -(-k // 32)), dtype=np.uint8)
+    q = g.integers(0, 16, (n, 2 * -(-k // 2)), dtype=np.uint8)
+    q[:, j] = z[:, j // 32]
+    scales = (0.5 + g.random((n, -(-k // 32)))).astype(np.float16).astype(np.float32)
+    p = PackedWeights(n, k, Precision.Q4, q[:, 0::2] | (q[:, 1::2] << 4), scales, zeros=z, group=32)
+    assert (decode(p)[:, j] == 0).all()
+    return p.upload(ctx), decode(p)
+
+
+@pytest.mark.parametrize("m", [1, 2, 4, 8, 9, 16, 24, 33, 100, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ratio", [10, 17, 24, 30, 38])
+def test_a_large_activation_without_weight(ctx, m, dtype, ratio):
+    """One activation 2^ratio times the others whose weights are 0, so the others alone decide. With A the row's
+    largest, an activation enters the product to 2^-55 A (one or two rows, whatever the type), as it is (up to eight
+    rows, and 16-bit types), or to the larger of 2^-22 of itself, which `bound` has, and 2^-39 A (more rows of f32)."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k, j = 40, 512, 77
+    dev, w = weights_without(ctx, n, k, j, 3)
+    a = torch.randn((m, k), generator=torch.Generator().manual_seed(ratio)).clamp(-4, 4)
+    a[:, j] = 2.0 ** ratio
+    a = a.to(types()[dtype])
+    c = torch.empty((m, n), device="cuda")
+    Kernels(ctx).linear(a.cuda(), m, dev, c)
+    ctx.check()
+    av = a.double().numpy()
+    y = av @ w.T
+    held = 2.0 ** -55 if m <= 2 else 2.0 ** -39 if m > 8 and dtype == "f32" else 0.0
+    lim = bound(av, w, y, None, 1.0, None, 32, "f32") + np.abs(av).max(axis=1)[:, None] * held * np.abs(w).sum(axis=1)
+    assert (np.abs(c.double().cpu().numpy() - y) <= lim).all()
+    dev.free()
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 16, 30, 100, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act", ["RELU", "SILU"])
+def test_a_row_that_is_not_finite_under_an_activation_function(ctx, m, dtype, act):
+    """Sums that are not finite, in that row alone: RELU makes 0 of -infinity, and nothing else is finite."""
+    import torch
+    from telmo_b200 import Act, Epilogue, Kernels
+    n, k = 70, 200
+    dev, w = weights(ctx, n, k, 32, True, 5)
+    a = torch.randn((m, k), generator=torch.Generator().manual_seed(6)).to(types()[dtype]).cuda()
+    clean, c = (torch.empty((m, n), device="cuda") for _ in range(2))
+    epi = Epilogue(act=Act[act])
+    Kernels(ctx).linear(a, m, dev, clean, epi)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        b = a.clone()
+        b[m // 2, 77] = bad
+        Kernels(ctx).linear(b, m, dev, c, epi)
+        ctx.check()
+        row = c[m // 2]
+        assert (~torch.isfinite(row) | ((row == 0) & (act == "RELU"))).all()
+        assert not np.isnan(bad) or row.isnan().all()
+        keep = torch.arange(m, device="cuda") != m // 2
+        assert torch.equal(c[keep], clean[keep])
+    dev.free()
