@@ -134,8 +134,8 @@ int telmo_linear(telmo_ctx *ctx, const float *a, size_t lda, size_t m, const tel
  * than 2^17 times the others while its weights are 0, the others keep fewer than 22 bits from
  * nine rows on. A row of a that holds an infinity or a NaN has sums that are not finite in that row
  * alone (TELMO_ACT_RELU makes 0 of -infinity). a and c need no more than their elements'
- * alignment; rows that start on 16-byte boundaries are read fastest. a and c must not overlap
- * (TELMO_ERR_ARGUMENT). */
+ * alignment; rows that start on 16-byte boundaries are read fastest. c must overlap neither a nor
+ * the bias (TELMO_ERR_ARGUMENT), but a single f32 row may be written over its bias. */
 int telmo_linear_q4(telmo_ctx *ctx, const void *a, int a_dtype, size_t lda, size_t m,
                     const telmo_weights *w, const float *bias, int act, float scale, int accumulate,
                     void *c, int c_dtype, size_t ldc, void *stream);
@@ -212,9 +212,9 @@ typedef struct telmo_logit_rules {
 
 /* The values above for logits [rows, ld] of dtype (F32, BF16 or F16), vocab of each row, into out
  * [rows, out_ld] of the same type; what lies behind a row's vocab is left as it is. out may be
- * logits itself with the same ld, but must not overlap them otherwise (TELMO_ERR_ARGUMENT). rules NULL: none. There is no
- * counterpart in the reference, whose decoders choose from the logits as they are or search with
- * word bonuses (src/biasing.rs). */
+ * logits itself with the same ld, but must not overlap them otherwise, nor the rules' arrays
+ * (TELMO_ERR_ARGUMENT). rules NULL: none. There is no counterpart in the reference, whose decoders
+ * choose from the logits as they are or search with word bonuses (src/biasing.rs). */
 int telmo_logits_constrain(telmo_ctx *ctx, const void *logits, int dtype, size_t ld, size_t rows,
                            size_t vocab, const telmo_logit_rules *rules, void *out, size_t out_ld,
                            void *stream);
@@ -222,8 +222,10 @@ int telmo_logits_constrain(telmo_ctx *ctx, const void *logits, int dtype, size_t
  * lowest token first where several tie (as telmo_granite_frame_ids), into ids [rows, k], and their
  * log-probabilities x - log(sum over the vocabulary of e^x) into logprobs [rows, k] (NULL: not
  * wanted). A token whose value is -infinity is never chosen: where fewer than k are left, the rest
- * of ids is -1 and of logprobs -infinity. A NaN value is not chosen; a NaN or
- * +infinity makes its row's log-probabilities NaN. */
+ * of ids is -1 and of logprobs -infinity. A NaN value is not chosen; a NaN or +infinity makes its
+ * row's log-probabilities NaN. A row's ids and logprobs may lie among that row's inputs (the next
+ * place of its tokens so far, say), but must overlap neither other rows' nor each other
+ * (TELMO_ERR_ARGUMENT). */
 int telmo_logits_choose(telmo_ctx *ctx, const void *logits, int dtype, size_t ld, size_t rows,
                         size_t vocab, const telmo_logit_rules *rules, size_t k, int32_t *ids,
                         float *logprobs, void *stream);

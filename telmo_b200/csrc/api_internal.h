@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "overlap.h"
 
 #include <cstdarg>
 #include <string>
@@ -82,16 +83,6 @@ struct DeviceScope {
 int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const Weights* w, const float* bias, int act,
               float scale, int accumulate, void* out, int c_dtype, size_t ldc, cudaStream_t stream);
 void free_q4_weights(Weights* w);
-
-// Whether two matrices of as many rows share a byte: rows of a_row and b_row bytes, a_pitch and b_pitch bytes
-// apart. Matrices of one pitch may lie side by side; of two pitches, their ranges must be apart.
-inline bool overlap(const void* a, size_t a_pitch, size_t a_row, const void* b, size_t b_pitch, size_t b_row, size_t rows) {
-    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
-    if (a0 + (rows - 1) * a_pitch + a_row <= b0 || b0 + (rows - 1) * b_pitch + b_row <= a0) return false;
-    if (rows == 1 || a_pitch != b_pitch) return true;
-    const uintptr_t behind = b0 >= a0 ? (b0 - a0) % a_pitch : (a_pitch - (a0 - b0) % a_pitch) % a_pitch;
-    return behind < a_row || a_pitch - behind < b_row;
-}
 
 inline Ctx* as_ctx(telmo_ctx* c) { return reinterpret_cast<Ctx*>(c); }
 

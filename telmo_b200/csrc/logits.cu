@@ -817,6 +817,20 @@ int prepare(Ctx* ctx, const char* who, const void* logits, int dtype, size_t ld,
     return TELMO_OK;
 }
 
+// Calls f with the memory of each of the rules' arrays. Masks are one row: any row may read any.
+template <typename F>
+bool any_rule(const RuleParams& p, F f) {
+    const size_t rows = static_cast<size_t>(p.rows), word = 4;
+    const auto table = [&](const void* q, int64_t ld, int entries) {
+        return f(Span{q, static_cast<size_t>(ld) * word, static_cast<size_t>(entries) * word, rows});
+    };
+    const auto vector = [&](const void* q) { return f(Span{q, word, word, rows}); };
+    const size_t masks = p.allowed ? ((p.n_states - size_t(1)) * p.allowed_ld + (p.vocab + size_t(31)) / 32) * word : 0;
+    return table(p.history, p.history_ld, p.n_history) || table(p.bias_ids, p.bias_ld, p.n_bias) ||
+           table(p.bias, p.bias_ld, p.n_bias) || vector(p.history_len) || vector(p.repetition) || vector(p.frequency) ||
+           vector(p.presence) || vector(p.state) || f(Span{p.allowed, 0, masks, 1});
+}
+
 }  // namespace
 
 }  // namespace telmo
@@ -834,9 +848,11 @@ extern "C" int telmo_logits_constrain(telmo_ctx* c, const void* logits, int dtyp
         out_ld > (size_t(1) << 40))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out is NULL or misaligned, or its rows short");
     const size_t size = dtype == TELMO_DTYPE_F32 ? 4 : 2;
-    if (!(out == logits && (out_ld == ld || rows == 1)) &&
-        overlap(logits, ld * size, vocab * size, out, out_ld * size, vocab * size, rows))
+    const Span written{out, out_ld * size, vocab * size, rows};
+    if (!(out == logits && (out_ld == ld || rows == 1)) && overlap(Span{logits, ld * size, vocab * size, rows}, written))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out overlaps the logits and is not the logits");
+    if (any_rule(p, [&](const Span& s) { return overlap(s, written); }))
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_constrain: out overlaps a rule's array");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     p.out = out;
@@ -864,12 +880,22 @@ extern "C" int telmo_logits_choose(telmo_ctx* c, const void* logits, int dtype, 
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_choose: 1 to %d tokens a row, not %zu", kMaxK, k);
     if (!ids || reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(logprobs) % 4)
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_choose: ids are NULL, or ids or logprobs misaligned");
+    // A row's tokens are written once the row has been read, so they may lie among its own inputs (the next place of
+    // its tokens so far, say), but not among other rows'.
+    const size_t size = dtype == TELMO_DTYPE_F32 ? 4 : 2;
+    const Span to_ids{ids, k * 4, k * 4, rows}, to_logprobs{logprobs, k * 4, k * 4, rows};
+    const auto read_elsewhere = [&](const Span& s) {
+        return overlaps_other_rows(s, to_ids) || overlaps_other_rows(s, to_logprobs);
+    };
+    if (overlap(to_ids, to_logprobs) || read_elsewhere(Span{logits, ld * size, vocab * size, rows}) ||
+        any_rule(p, read_elsewhere))
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_logits_choose: ids or logprobs overlap each other or another row's inputs");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     p.ids = ids;
     p.logprobs = logprobs;
     p.k = static_cast<int>(k);
-    const int places = most_places(p, dtype == TELMO_DTYPE_F32 ? 4 : 2);
+    const int places = most_places(p, size);
     // A cluster of up to eight blocks a row: the number that takes the least time, if the SMs hold two blocks
     // each, a block's lists, first bound and end cost as much as two tiles, and a cluster's meetings too. 256 rows of 131072: 72 us on one
     // block a row, 78 on two; 300 rows: 75 on eight, 82 on one.

@@ -135,8 +135,12 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     const auto misaligned = [](const void* p, uintptr_t b) { return reinterpret_cast<uintptr_t>(p) % b != 0; };
     if (misaligned(a, as) || misaligned(out, cs) || misaligned(bias, 4))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: a, c or bias is not aligned to its elements");
-    if (overlap(a, lda * as, k * as, out, ldc * cs, n * cs, m))
+    const Span c_span{out, ldc * cs, n * cs, m};
+    if (overlap(Span{a, lda * as, k * as, m}, c_span))
         return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: a and c overlap");
+    // One row may be written over its bias: the thread that reads a value writes its output.
+    if (!(m == 1 && out == bias && ct == kQ4F32) && overlap(Span{bias, 0, n * sizeof(float), 1}, c_span))
+        return ctx->fail(TELMO_ERR_ARGUMENT, "telmo_linear_q4: bias and c overlap");
     DeviceScope scope;
     if (int rc = scope.enter(ctx)) return rc;
     Q4Args g;
