@@ -100,8 +100,8 @@ int telmo_weights_shape(const telmo_weights *w, size_t *n, size_t *k);
  * telmo_encode_q4 rounds a row-major f32 [n, k] matrix to them on the host: codes receives n rows
  * of ceil(k / 2) bytes (the even input in the low half), scales [n, ceil(k / group)], and zeros,
  * where not NULL, as many zero points: with zeros, codes span the group's range (0 included) in 15
- * steps; without, every zero point is 8. TELMO_ERR_ARGUMENT for weights that are not finite or
- * whose scale passes the f16 range. */
+ * steps; without, every zero point is 8. Scales are rounded to f16, below 2^-14 upwards.
+ * TELMO_ERR_ARGUMENT for weights that are not finite or whose scale passes the f16 range. */
 int telmo_encode_q4(const float *rows, size_t n, size_t k, size_t group, uint8_t *codes,
                     float *scales, uint8_t *zeros);
 /* Uploads such weights (host memory, laid out as telmo_encode_q4 writes them; zeros NULL: 8

@@ -21,6 +21,14 @@ float f16_value(float x) {
     return std::isfinite(h) ? h : std::nanf("");
 }
 
+// A group's scale for the step x >= 0 that its range needs: x rounded to f16, NaN where that is not finite. Below
+// 2^-14, where f16 values are 2^-24 apart, it is rounded up: a smaller one would leave the group's largest weights out
+// of reach of the codes, or be 0.
+float f16_scale(float x) {
+    const float h = f16_value(x);
+    return h < x && x < 0x1p-14f ? h + 0x1p-24f : h;
+}
+
 // Whether x is a finite f16 value: 11 significant bits from 2^15 down to multiples of 2^-24.
 bool is_f16(float x) {
     uint32_t u;
@@ -198,7 +206,7 @@ extern "C" int telmo_encode_q4(const float* rows, size_t n, size_t k, size_t gro
             }
             // Without zero points codes stand for -8..7: the step is the larger of what the
             // group's extremes need. With them the range is [lo, hi], 0 included, in 15 steps.
-            const float d = f16_value(zeros ? hi / 15.0f - lo / 15.0f : std::max(hi / 7.0f, -lo / 8.0f));
+            const float d = f16_scale(zeros ? hi / 15.0f - lo / 15.0f : std::max(hi / 7.0f, -lo / 8.0f));
             if (std::isnan(d)) return TELMO_ERR_ARGUMENT;
             const float id = d != 0.0f ? 1.0f / d : 0.0f;
             const float z = zeros ? std::fmin(std::fmax(std::round(-lo * id), 0.0f), 15.0f) : 8.0f;

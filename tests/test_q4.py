@@ -87,3 +87,16 @@ def test_null_handles_are_refused():
     assert L.telmo_weights_upload_q4(None, 1, 32, 32, p, p, None, ctypes.byref(h)) == _lib.TELMO_ERR_ARGUMENT
     assert L.telmo_linear_q4(None, p, 0, 32, 1, None, None, 0, 1.0, 0, p, 0, 1, None) == _lib.TELMO_ERR_ARGUMENT
 
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("largest", [2.0 ** -13, 2.0 ** -17, 3e-6, 1e-6, 2.0 ** -20, 4e-7, 2.0 ** -23, 1e-9])
+def test_small_weights_keep_their_range(zeros, largest):
+    """Scales below 2^-14 are multiples of 2^-24, far apart against themselves: they are rounded up, so that codes reach
+    the group's largest weights. Off by half a step, and half a step more where a zero point is rounded."""
+    g = np.random.default_rng(3)
+    rows = (g.uniform(-1, 1, (4, 96)) * largest).astype(np.float32)
+    rows[:, ::32] = largest * np.float32([[1], [-1], [1], [-1]])
+    p = PackedWeights.encode(rows, 4, 96, Precision.Q4, group=32, zeros=zeros)
+    d = p.scales.reshape(4, 3)[:, np.arange(96) // 32].astype(np.float64)
+    assert (d == p.scales.astype(np.float16).reshape(4, 3)[:, np.arange(96) // 32]).all() and (d > 0).all()
+    assert (np.abs(decode(p) - rows) <= d * (0.5 + 0.5 * zeros + 1e-5)).all()
