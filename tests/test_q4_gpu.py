@@ -501,3 +501,52 @@ def test_a_row_that_is_not_finite_under_an_activation_function(ctx, m, dtype, ac
         keep = torch.arange(m, device="cuda") != m // 2
         assert torch.equal(c[keep], clean[keep])
     dev.free()
+
+
+@pytest.mark.parametrize("m", [9, 33])
+def test_rows_of_more_pieces_than_a_grid_is_high(ctx, m):
+    """16-bit rows off 16-byte boundaries are copied in pieces of 2048: rows with more than 65535 of them. A few of the
+    134 million weights are not 0, in the first, the last and the pieces around the last of a grid's."""
+    import torch
+    from telmo_b200 import Kernels, PackedWeights, Precision
+    k = 65535 * 2048 + 2049
+    at = np.array([0, 5, 2047, 2048, 65535 * 2048 - 1, 65535 * 2048, 65535 * 2048 + 77, k - 2, k - 1])
+    codes = np.full((1, (k + 1) // 2), 0x88, np.uint8)
+    for i, q in zip(at, range(9, 16 + len(at))):
+        q = q if q < 16 else q - 16
+        codes[0, i // 2] = codes[0, i // 2] & (0x0f if i & 1 else 0xf0) | (q << 4 if i & 1 else q)
+    w = np.stack([codes[0, at // 2] & 15, codes[0, at // 2] >> 4])[at & 1, np.arange(len(at))].astype(np.float64) - 8
+    assert (w != 0).all()
+    dev = PackedWeights(1, k, Precision.Q4, codes, np.ones((1, -(-k // 128)), np.float32), group=128).upload(ctx)
+    a = torch.ones((m, k), dtype=torch.bfloat16, device="cuda")
+    a[:, torch.from_numpy(at).cuda()] = torch.randn((m, len(at)), generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    c = torch.zeros((m, 1), device="cuda")
+    Kernels(ctx).linear(a, m, dev, c)
+    ctx.check()
+    av = a[:, torch.from_numpy(at).cuda()].double().cpu().numpy()
+    # Every other product is exactly 0, and so are the sums without these inputs.
+    lim = (np.abs(av) @ np.abs(w)) * len(at) * 2.0 ** -23
+    assert (np.abs(c[:, 0].double().cpu().numpy() - av @ w) <= lim).all()
+    dev.free()
+    del a
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 9, 20, 33, 130, 200, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_behind_the_last_stay_as_they_were(ctx, m, dtype):
+    """A buffer of more rows than the call names, and rows of a that are not finite behind the last."""
+    import torch
+    from telmo_b200 import Kernels
+    n, k = 300, 520
+    dev, w = weights(ctx, n, k, 64, True, 7)
+    a = torch.randn((m + 300, k), generator=torch.Generator().manual_seed(8)).to(types()[dtype]).cuda()
+    a[m:] = float("nan")
+    c = torch.full((m + 300, n), 5.0, device="cuda")
+    Kernels(ctx).linear(a, m, dev, c)
+    ctx.check()
+    av = a[:m].double().cpu().numpy()
+    y = av @ w.T
+    assert (np.abs(c[:m].double().cpu().numpy() - y) <= bound(av, w, y, None, 1.0, None, 64, "f32")).all()
+    assert (c[m:] == 5).all()
+    dev.free()
