@@ -150,21 +150,24 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
 // releases is acquired.
 template <int CG, bool DATA>
 __device__ __forceinline__ bool wait_for_pair(uint64_t* bar, uint32_t parity) {
-    if (CG == 1) return wait_for(bar, parity);
-    for (uint32_t i = 0; i < kWaitPolls; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (ok) {
-            if (DATA) asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
-            return true;
+    if constexpr (CG == 1) {
+        return wait_for(bar, parity);
+    } else {
+        for (uint32_t i = 0; i < kWaitPolls; ++i) {
+            uint32_t ok;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.b32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+            if (ok) {
+                if (DATA) asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+                return true;
+            }
+            if (i > 4096) __nanosleep(256);
         }
-        if (i > 4096) __nanosleep(256);
+        return false;
     }
-    return false;
 }
 
 // Arrives on the same barrier of both CTAs of the pair once this thread's products are complete.

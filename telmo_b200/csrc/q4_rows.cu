@@ -102,10 +102,8 @@ cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t
     // Up to 8 rows of f32 or of any alignment are read as they are (8 f32 rows, 4096 -> 8192: 16 us; as planes
     // the split kernel's 4 us come before a product), and aligned ones where a warp has one chunk at most, so
     // that a ring has nothing to run ahead to (1024 -> 4096: 3.3 us, staged 4.3; 4096 -> 4096: 8.6 us, staged 7.3).
-    if (!p.vec || mode == kModeF32 ? g.m <= 8 : g.m <= 8 && p.chunks <= kWarps) {
-        p.split_chunks = p.chunks;
+    if (!p.vec || mode == kModeF32 ? g.m <= 8 : g.m <= 8 && p.chunks <= kWarps)
         return launch_small(p, mode, g.w->group, stream);
-    }
     // Warps side by side read the same activations; the chunks are split over clusters as long as the
     // blocks all run at once and a share keeps two chunks (4096 -> 4096: 24 rows 9.2 us, 22 without; 8 rows 7.3,
     // 10.1 without; 4096 -> 8192, 32 rows: 16.8, 25 without).

@@ -145,19 +145,19 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
     return v;
 }
 
-// A chunk's codes, scales and zero points of this lane's 2 R rows, as loaded.
-template <int GROUPS, bool ZEROS, int R>
+// A chunk's codes, scales and zero points of this lane's two rows, as loaded.
+template <int GROUPS, bool ZEROS>
 struct Chunk {
-    uint4 words[2 * R];
-    uint32_t d[2 * R][GROUPS == 4 ? 2 : 1];  // f16 pairs
-    uint32_t z[2 * R];                       // bytes
+    uint4 words[2];
+    uint32_t d[2][GROUPS == 4 ? 2 : 1];  // f16 pairs
+    uint32_t z[2];                       // bytes
 };
 
-template <int GROUPS, bool ZEROS, int R>
-__device__ __forceinline__ void load_chunk(Chunk<GROUPS, ZEROS, R>& x, const uint4* codes, const uint8_t* scales,
+template <int GROUPS, bool ZEROS>
+__device__ __forceinline__ void load_chunk(Chunk<GROUPS, ZEROS>& x, const uint4* codes, const uint8_t* scales,
                                            const uint8_t* zeros) {
 #pragma unroll
-    for (int r = 0; r < 2 * R; ++r) {
+    for (int r = 0; r < 2; ++r) {
         // Tiles of the same 128 outputs follow one another: 512 bytes of codes, 16 GROUPS of scales.
         x.words[r] = __ldg(codes + r * 32);
         const uint8_t* s = scales + r * (8 * GROUPS * 2);
@@ -227,7 +227,7 @@ __device__ __forceinline__ void operands(uint32_t x0, uint32_t x1, uint32_t z0, 
 // The sums of a block's shares, and of a cluster's blocks, and the epilogue, four outputs a thread at a
 // time. `sums`: [share][column][output of the block] in shared memory, written and synchronised.
 template <bool SCALED, int SHARES, int OUTS, int COLS>
-__device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, int64_t out0, int m0, int split) {
+__device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, int64_t out0, int split) {
     constexpr int kAll = OUTS * COLS / 4;
     float4* s4 = reinterpret_cast<float4*>(sums);
     const auto add = [](float4& a, const float4& b) {
@@ -237,7 +237,7 @@ __device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, i
         a.w += b.w;
     };
     const auto finish = [&](int e, const float4& s) {
-        const int row = m0 + e / (OUTS / 4);
+        const int row = e / (OUTS / 4);
         if (row >= p.m) return;
         const float rs = SCALED ? p.row_scale[row] : 1.0f;
 #pragma unroll
@@ -277,46 +277,41 @@ __device__ __forceinline__ void finish_block(const RowsParams& p, float* sums, i
     cluster_sync();  // the other blocks have read this one's sums
 }
 
+// Up to eight rows: a block's warps share the chunks of 16 outputs.
 template <int MODE, int GROUPS, bool ZEROS>
 __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p) {
     constexpr bool BF16 = MODE != kModeF16;
-    constexpr int R = 1, CB = 1;  // slabs of 16 outputs a warp, of 8 activation rows
     constexpr int kParts = MODE == kModeF32 ? 3 : 1;
     constexpr int kWordsPerGroup = 4 / GROUPS;
-    constexpr int kCols = 8;  // activation rows of the block
-    __shared__ __align__(16) float sums[kWarps * 16 * R * kCols];
+    constexpr int kOuts = 16, kCols = 8;  // outputs and activation rows of the block
+    __shared__ __align__(16) float sums[kWarps * kOuts * kCols];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int g = lane >> 2, t = lane & 3;
-    constexpr int shares = kWarps;
-    const int share = warp;
-    const int split = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int block = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x;
-    const int m0 = blockIdx.y * kCols;
-    const int64_t out0 = static_cast<int64_t>(block) * 16;  // the block's first output
-    const int64_t tile0 = out0 / 8;                         // the warp's first 8-output tile
-    const int c_end = min(p.chunks, (split + 1) * p.split_chunks);
-    int c = split * p.split_chunks + share;
+    const int64_t out0 = static_cast<int64_t>(blockIdx.x) * kOuts;
+    int c = warp;
+    // The compiler is not to know that rows are 0..7: with that it orders the loads of rows off 16-byte boundaries
+    // worse (3 rows of bf16, 4096 -> 8192: 15.4 us, 13.8 so).
+    int row = g;
+    asm("" : "+r"(row));
 
-    float acc[R][CB][4] = {}, part[R][CB][4] = {};
-    // Tiles past the last 128 outputs do not exist: such a warp has nothing to do.
-    if (tile0 * 8 < p.n && c < c_end) {
-        const int64_t first = q4_tile(tile0, p.chunks, c);
+    float acc[1][1][4] = {}, part[1][1][4] = {};
+    if (c < p.chunks) {
+        const int64_t first = q4_tile(out0 / 8, p.chunks, c);
         const uint4* codes = p.codes + first * 32 + lane;
         const uint8_t* scales = reinterpret_cast<const uint8_t*>(p.scales) + (first * 8 + g) * GROUPS * 2;
         const uint8_t* zeros = ZEROS ? p.zeros + (first * 8 + g) * GROUPS : nullptr;
-        Chunk<GROUPS, ZEROS, R> now, next;
+        Chunk<GROUPS, ZEROS> now, next;
         load_chunk(now, codes, scales, zeros);
         next = now;
-        for (; c < c_end; c += shares) {
-            codes += shares * (16 * 32);
-            scales += shares * (16 * 8 * GROUPS * 2);
-            if (ZEROS) zeros += shares * (16 * 8 * GROUPS);
-            if (c + shares < c_end) load_chunk(next, codes, scales, zeros);
+        for (; c < p.chunks; c += kWarps) {
+            codes += kWarps * (16 * 32);
+            scales += kWarps * (16 * 8 * GROUPS * 2);
+            if (ZEROS) zeros += kWarps * (16 * 8 * GROUPS);
+            if (c + kWarps < p.chunks) load_chunk(next, codes, scales, zeros);
 
 #pragma unroll 1
             for (int w = 0; w < 4; ++w) {
                 const int i = c * 128 + 32 * w + 8 * t;
-                const int row = m0 + g;
                 uint32_t b[kParts][4];
                 if (MODE == kModeF32) {
                     float x[8];
@@ -326,47 +321,38 @@ __global__ void __launch_bounds__(32 * kWarps) q4_rows_kernel(const RowsParams p
                     const uint4 v = load_a16(static_cast<const uint16_t*>(p.a) + row * p.lda + i, row < p.m, p.vec, p.k - i);
                     b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
                 }
+                uint32_t a[2][4];
+                operands<BF16>(now.words[0].x, now.words[1].x, code_base<BF16>(ZEROS ? now.z[0] & 0xffu : 8u),
+                               code_base<BF16>(ZEROS ? now.z[1] & 0xffu : 8u), a);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    uint32_t a[2][4];
-                    operands<BF16>(now.words[2 * r].x, now.words[2 * r + 1].x, code_base<BF16>(ZEROS ? now.z[2 * r] & 0xffu : 8u),
-                                   code_base<BF16>(ZEROS ? now.z[2 * r + 1] & 0xffu : 8u), a);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int pl = 0; pl < kParts; ++pl)
+                        mma_16816<BF16>(part[0][0], a[h], b[pl][2 * h], b[pl][2 * h + 1]);
 #pragma unroll
-                        for (int pl = 0; pl < kParts; ++pl)
-                            mma_16816<BF16>(part[r][0], a[h], b[pl][2 * h], b[pl][2 * h + 1]);
-                }
-#pragma unroll
-                for (int r = 0; r < 2 * R; ++r) {
+                for (int r = 0; r < 2; ++r) {
                     now.words[r].x = now.words[r].y;
                     now.words[r].y = now.words[r].z;
                     now.words[r].z = now.words[r].w;
                 }
                 if ((w + 1) % kWordsPerGroup == 0) {
-                    add_group<GROUPS, R, CB>(acc, part, now.d);
-                    if (ZEROS)
-#pragma unroll
-                        for (int r = 0; r < 2 * R; ++r) now.z[r] >>= 8;
+                    add_group<GROUPS, 1, 1>(acc, part, now.d);
+                    if (ZEROS) {
+                        now.z[0] >>= 8;
+                        now.z[1] >>= 8;
+                    }
                 }
             }
             now = next;
         }
     }
 
-    // sums[share][column][output of the block]
-    const int outs = 16 * R;
+    // sums[warp][column][output of the block]
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int col = 8 * cb + 2 * t + (j & 1);
-                sums[(share * kCols + col) * outs + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
-            }
+    for (int j = 0; j < 4; ++j)
+        sums[(warp * kCols + 2 * t + (j & 1)) * kOuts + g + 8 * (j >> 1)] = acc[0][0][j];
     __syncthreads();
-    finish_block<false, kWarps, 16 * R, kCols>(p, sums, out0, m0, split);
+    finish_block<false, kWarps, kOuts, kCols>(p, sums, out0, 0);
 }
 
 // Rows that start on 16-byte boundaries (16-bit activations, or planes): activations and codes come
@@ -525,16 +511,13 @@ __global__ void __launch_bounds__(32 * kWarps, Staged<MODE, R, CB>::kBlocks) q4_
             for (int j = 0; j < 4; ++j)
                 sums[(share * kCols + 8 * cb + 2 * t + (j & 1)) * outs + rw * 16 * R + 16 * r + g + 8 * (j >> 1)] = acc[r][cb][j];
     __syncthreads();
-    finish_block<MODE == kModePlanes, S::kShares, 16 * R * S::kRowWarps, kCols>(p, sums, out0, 0, split);
+    finish_block<MODE == kModePlanes, S::kShares, 16 * R * S::kRowWarps, kCols>(p, sums, out0, split);
 }
 
-inline dim3 rows_grid(const RowsParams& p, int outs, int cols) {
-    return dim3(static_cast<unsigned>((p.n + outs - 1) / outs) * p.splits, (p.m + cols - 1) / cols);
-}
-
-inline cudaError_t rows_launch(void (*kernel)(RowsParams), const RowsParams& p, dim3 grid, size_t smem, cudaStream_t stream) {
+// `outs`: outputs of a block, or of a cluster of p.splits blocks.
+inline cudaError_t rows_launch(void (*kernel)(RowsParams), const RowsParams& p, int outs, size_t smem, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(static_cast<unsigned>((p.n + outs - 1) / outs) * p.splits);
     cfg.blockDim = dim3(32 * kWarps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -556,13 +539,12 @@ cudaError_t launch_staged(const RowsParams& p, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
         once.mark(dev);
     }
-    return rows_launch(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, p,
-                       rows_grid(p, 16 * R * S::kRowWarps, 8 * CB), S::kSmem, stream);
+    return rows_launch(q4_rows_staged_kernel<MODE, GROUPS, ZEROS, R, CB>, p, 16 * R * S::kRowWarps, S::kSmem, stream);
 }
 
 template <int MODE, int GROUPS, bool ZEROS>
 cudaError_t launch_direct(const RowsParams& p, cudaStream_t stream) {
-    return rows_launch(q4_rows_kernel<MODE, GROUPS, ZEROS>, p, rows_grid(p, 16, 8), 0, stream);
+    return rows_launch(q4_rows_kernel<MODE, GROUPS, ZEROS>, p, 16, 0, stream);
 }
 
 // Calls f with the group's and the zero points' constants.
