@@ -532,3 +532,36 @@ def test_refusals(ctx):
     assert L.telmo_logits_choose(hd, px, 0, 100, 4, 100, None, 2, pi + 2, None, None) == arg
     assert L.telmo_logits_choose(None, px, 0, 100, 4, 100, None, 2, pi, None, None) == arg
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("vocab", [700, 8192, 20011, 131072])
+@pytest.mark.parametrize("k", [1, 3, 8])
+def test_rows_in_order(ctx, vocab, k):
+    """Rising rows, whose every tile holds larger values than all before, falling ones, rows that rise within tiles and
+    from thread to thread, and one value alone: the bound of the choice rises at every step or never."""
+    import torch
+    from telmo_b200 import LogitRules
+    v = torch.arange(vocab)
+    rows = torch.stack([v, -v, v % 16 * 8192 + v // 16, (v % 8192) * 16 + v // 8192, torch.zeros(vocab, dtype=torch.int64)])
+    check_choose(ctx, 5, vocab, "f32", k, logits=(rows.float() / vocab).cuda(), r=LogitRules())
+
+
+@pytest.mark.parametrize("vocab", [33, 2049, 70001])
+def test_masks_of_either_type(ctx, vocab):
+    """32-bit words as torch.int32 or torch.uint32; the highest bit of a word is a token like the others."""
+    import torch
+    from telmo_b200 import Kernels, LogitRules
+    k, words = Kernels(ctx), -(-vocab // 32)
+    x = torch.randn((3, vocab), generator=torch.Generator().manual_seed(vocab)).cuda()
+    masks = torch.randint(-2 ** 31, 2 ** 31, (3, words), generator=torch.Generator().manual_seed(1), dtype=torch.int64)
+    masks[0] = 1 << 31
+    got = []
+    for m in (masks.to(torch.int32).cuda(), (masks & 0xffffffff).to(torch.uint32).cuda()):
+        out, ids = torch.empty_like(x), torch.empty((3, 2), dtype=torch.int32, device="cuda")
+        k.constrain_logits(x, vocab, 3, vocab, LogitRules(allowed=m), out, vocab)
+        k.choose_tokens(x, vocab, 3, vocab, LogitRules(allowed=m), 2, ids)
+        ctx.check()
+        got.append((out, ids))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    allowed = torch.isfinite(got[0][0][0]).nonzero()[:, 0].cpu()
+    assert allowed.tolist() == list(range(31, vocab, 32))

@@ -550,3 +550,52 @@ def test_rows_behind_the_last_stay_as_they_were(ctx, m, dtype):
     assert (np.abs(c[:m].double().cpu().numpy() - y) <= bound(av, w, y, None, 1.0, None, 64, "f32")).all()
     assert (c[m:] == 5).all()
     dev.free()
+
+
+@pytest.mark.parametrize("m", [1, 7, 12, 50])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_the_general_entry_takes_the_handle(ctx, m, out):
+    """telmo_linear with 4-bit weights gives what telmo_linear_q4 gives; a pair of int32 sums is refused."""
+    import ctypes
+    import torch
+    from telmo_b200 import _lib
+    L, n, k = _lib.load(), 130, 200
+    dev, _ = weights(ctx, n, k, 64, True, 3)
+    a = torch.randn((m, k + 3), device="cuda")
+    bias = torch.randn(n, device="cuda")
+    one, two = (torch.randn((m, n + 1), generator=torch.Generator().manual_seed(1)).to(types()[out]).cuda() for _ in range(2))
+    dtype, stream = {"f32": 0, "bf16": 1}[out], torch.cuda.current_stream().cuda_stream
+    assert L.telmo_linear(ctx.handle, a.data_ptr(), k + 3, m, dev.handle, bias.data_ptr(), 2, 0.5, 1, one.data_ptr(), dtype,
+                          n + 1, stream) == 0
+    assert L.telmo_linear_q4(ctx.handle, a.data_ptr(), 0, k + 3, m, dev.handle, bias.data_ptr(), 2, 0.5, 1, two.data_ptr(),
+                             dtype, n + 1, stream) == 0
+    assert L.telmo_linear(ctx.handle, a.data_ptr(), k + 3, m, dev.handle, None, 0, 1.0, 0, one.data_ptr(), 2, n + 1,
+                          stream) == _lib.TELMO_ERR_ARGUMENT
+    ctx.check()
+    assert torch.equal(one, two)
+    rows, cols = ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.telmo_weights_shape(dev.handle, ctypes.byref(rows), ctypes.byref(cols)) == 0
+    assert (rows.value, cols.value) == (n, k)
+    dev.free()
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 12, 24, 100])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [2.0 ** -130, 2.0 ** -110, 2.0 ** 100])
+def test_rows_near_the_ends_of_the_range(ctx, m, dtype, size):
+    """Rows of subnormal values, of the smallest normal ones and of very large ones, scaled by c's scale to about 1."""
+    import torch
+    from telmo_b200 import Epilogue, Kernels
+    n, k = 70, 260
+    dev, w = weights(ctx, n, k, 32, True, 11)
+    a = (torch.randn((m, k), generator=torch.Generator().manual_seed(2)) * size).to(types()[dtype])
+    scale = float(np.float32(min(1 / size, 2.0 ** 120)))
+    c = torch.empty((m, n), device="cuda")
+    Kernels(ctx).linear(a.cuda(), m, dev, c, Epilogue(scale=scale))
+    ctx.check()
+    av = a.double().numpy()
+    y = av @ w.T * scale
+    # Parts below 2^-126 may vanish, and sums are f32: an error of 2^-126 for each product of size 8 and scale 1 / size.
+    lim = bound(av, w, y, None, scale, None, 32, "f32") + 2.0 ** -126 * scale * np.abs(w).sum(axis=1)
+    assert (np.abs(c.double().cpu().numpy() - y) <= lim).all()
+    dev.free()
