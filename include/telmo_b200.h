@@ -44,9 +44,10 @@ extern "C" {
 #define TELMO_ACT_RELU 1
 #define TELMO_ACT_SILU 2
 
-/* Element types (telmo_linear's outputs are f32, bf16 or an i32 pair). TELMO_DTYPE_I32_PAIR writes the two exact int32 sums of
- * the split-int8 product instead of the scaled result: plane 0 (rows 0..m-1, ldc apart) holds
- * the high level's sums and plane 1 (starting m * ldc elements later) the low level's. */
+/* Element types (telmo_linear's outputs are f32, bf16 or an i32 pair). TELMO_DTYPE_I32_PAIR writes
+ * the two exact int32 sums of the split-int8 product instead of the scaled result: plane 0 (rows
+ * 0..m-1, ldc apart) holds the high level's sums and plane 1 (starting m * ldc elements later) the
+ * low level's. */
 #define TELMO_DTYPE_F32 0
 #define TELMO_DTYPE_BF16 1
 #define TELMO_DTYPE_I32_PAIR 2

@@ -45,7 +45,7 @@ struct Ctx {
     uint32_t* error_word = nullptr;  // device error word the kernels record into
     void* ws = nullptr;              // growable workspace for telmo_linear's quantized operand
     size_t ws_bytes = 0;
-    cudaMemPool_t pool = nullptr;    // stream-ordered workspaces, created on first use
+    cudaMemPool_t pool = nullptr;    // stream-ordered workspaces, made with the first 4-bit weights
     PinnedRing uploads;              // the calls' small host-to-device uploads
     std::string last_error;
 

@@ -167,10 +167,10 @@ int linear_q4(Ctx* ctx, const void* a, int a_dtype, size_t lda, size_t m, const 
     g.sms = ctx->sms;
     g.error = ctx->error_word;
     if (q4_vec_fits(g)) return ctx->cuda(q4_linear_vec(g, stream), "telmo_linear_q4");
-    // Row kernels for few rows, tcgen05 tiles beyond: bf16 4096 -> 4096, 8 rows 7.3 us against 11.3, 24 rows 9.2
-    // against 11.8, 32 rows 10.5 against 11.8; 4096 -> 8192, 32 rows 16.8 against 17.1. f32 rows come in two planes
-    // there and take as many instructions as twice the rows: 16 rows 12.1 against 14.7, 4096 -> 8192 with 16 rows
-    // 19.1 against 20.8, with 24 23.2 against 21.0.
+    // Row kernels for few rows, tcgen05 tiles beyond: bf16 4096 -> 4096, 8 rows 8.2 us against 12.1, 24 rows 10.8
+    // against 12.4, 32 rows 11.0 against 12.4; 4096 -> 8192, 32 rows 17.1 against 18.4. f32 rows come in two planes
+    // there and take as many instructions as twice the rows: 16 rows 11.6 against 13.9, 4096 -> 8192 with 16 rows
+    // 17.7 against 20.9, with 24 23.2 against 21.2.
     const bool rows = m <= (at == kQ4F32 ? 16 : 32);
     const auto product = [&](const Q4Planes* planes) {
         return rows ? q4_linear_rows(g, planes, stream) : q4_linear_gemm(g, planes, stream);

@@ -29,9 +29,11 @@
 // their sums through distributed shared memory and finish a slice of the rows each, adding in rank
 // order. Every wait is bounded; on timeout the kernel records kErrWaitTimeout and returns.
 //
-// Measured: 4096 rows of bf16, 4096 -> 8192 in groups of 128: 219 us captured, 1253 TFLOP/s (75% of a dense bf16
-// product of the library), about 200 cycles an instruction of 256 x 256 x 16; 1500 rows of f32, 1024 -> 4096: 36.8 us
-// with their split, where eight chunks a tile leave its beginning and end uncovered (tensor pipe 34%).
+// Measured: 4096 rows of bf16, 4096 -> 8192 in groups of 128: 214 us in a short run, 1285 TFLOP/s (77% of the
+// library's dense bf16 product), about 200 cycles an instruction of 256 x 256 x 16; 251 us after seconds under the
+// power cap (1627 MHz), 1095 TFLOP/s (79% of the library's rate so). 1500 rows of f32, 1024 -> 4096: 36.9 us in a
+// stream of calls, 34.3 captured, with their split, where eight chunks a tile leave its beginning and end uncovered
+// (tensor pipe 34%).
 #include "ptx.cuh"
 #include "q4_device.cuh"
 #include "tma.h"
@@ -128,8 +130,8 @@ __device__ __forceinline__ void cluster_meet() {
 
 // Arrives on a barrier of either CTA of the pair. With DATA it announces what the arriving CTA's threads wrote to
 // their shared memory (each lane's fence.proxy.async comes first) to an instruction that the other CTA issues, so
-// the release is at cluster scope. It is restricted to this CTA's shared memory: a full one also waits for the
-// epilogue's stores to global memory (4096 rows, 4096 -> 8192: 218 us with this one, 320 with a full one). Without
+// the release is at cluster scope. It is restricted to this CTA's shared memory (4096 rows, 4096 -> 8192: 217 us; a
+// full one, which covers the epilogue's stores to global memory too, 320). Without
 // DATA it says that TMEM has been read, which the tcgen05 fences around an arrival and a wait order.
 template <bool DATA>
 __device__ __forceinline__ void arrive_pair(uint32_t cluster_bar) {
@@ -832,7 +834,9 @@ cudaError_t with_shape(int bn, int splits, F f) {
 // share inputs: their exchange of 128 KB a CTA cost more than it saved (200 rows, 4096 -> 8192: 40 us split in two,
 // 33 whole). The rounds of
 // tiles over the GPU count too: 1500 rows of f32, 1024 -> 4096, are 96 tiles of 256 rows on 74 pairs (42 us) or 128
-// of 192 (35 us).
+// of 192 (35 us). Against each of the ten choices forced, for 40 to 4096 rows and six shapes (640 -> 1000 to 4096 ->
+// 8192 and 8192 -> 2048, both types): the best one or within 5%, but for 100 and 128 rows of 1024 -> 4096 (10.3 us for
+// 9.4, f32 12.5 for 11.8); the worst choice takes 1.5 to 7 times as long.
 template <bool BF16, int P>
 cudaError_t launch_shape(const void* a, int64_t lda, const GemmParams& p, int sms, cudaStream_t stream) {
     int best_bn = 0, best_splits = 1, best_at_once = 1;

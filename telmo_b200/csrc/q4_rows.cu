@@ -99,14 +99,15 @@ cudaError_t q4_linear_rows(const Q4Args& g, const Q4Planes* planes, cudaStream_t
     p.ldc = g.ldc;
     p.splits = 1;
     const int mode = g.a_type == kQ4BF16 ? kModeBF16 : g.a_type == kQ4F16 ? kModeF16 : kModeF32;
-    // Up to 8 rows of f32 or of any alignment are read as they are (8 f32 rows, 4096 -> 8192: 16 us; as planes
-    // the split kernel's 4 us come before a product), and aligned ones where a warp has one chunk at most, so
-    // that a ring has nothing to run ahead to (1024 -> 4096: 3.3 us, staged 4.3; 4096 -> 4096: 8.6 us, staged 7.3).
+    // Up to 8 rows of f32 or of any alignment are read as they are (f32, 1024 -> 4096: 3.9 us, as two planes 7.8;
+    // 4096 -> 8192: 17.5 and 17.7. 16-bit rows off 16-byte boundaries, copied first: 5.4 us against 4.1, and 12.2
+    // against 13.6), and aligned ones where a warp has one chunk at most, so that a ring has nothing to run ahead
+    // to (1024 -> 4096: 3.3 us, staged 4.2; 4096 -> 4096: 8.7 us, staged 8.3).
     if (!p.vec || mode == kModeF32 ? g.m <= 8 : g.m <= 8 && p.chunks <= kWarps)
         return launch_small(p, mode, g.w->group, stream);
-    // Warps side by side read the same activations; the chunks are split over clusters as long as the
-    // blocks all run at once and a share keeps two chunks (4096 -> 4096: 24 rows 9.2 us, 22 without; 8 rows 7.3,
-    // 10.1 without; 4096 -> 8192, 32 rows: 16.8, 25 without).
+    // Warps side by side read the same activations; the chunks are split over clusters as long as the SMs have
+    // places for all blocks (fewer clusters may fit) and a share keeps two chunks (4096 -> 4096: 24 rows 10.7 us,
+    // 22.2 without; 8 rows 8.3, 10.6 without; 4096 -> 8192, 32 rows: 17.1, 26.4 without).
     const int row_warps = g.m <= 8 ? 2 : 4, shares = kWarps / row_warps;
     const int blocks = (p.n + 32 * row_warps - 1) / (32 * row_warps);
     const int resident = (mode != kModeF32 && g.m <= 24 ? 2 : 1) * g.sms;

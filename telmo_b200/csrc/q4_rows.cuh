@@ -23,12 +23,14 @@
 // in shared memory together with the activations (q4_rows_staged_kernel). Warps that share outputs
 // add up in shared memory, in order. Where n gives too few blocks, the blocks of a cluster take a
 // share of the chunks each and add up through distributed shared memory, in rank order (24 rows,
-// 4096 -> 4096 in groups of 64: 9.2 us, 22 without).
+// 4096 -> 4096 in groups of 64: 10.7 us, 22.2 without).
 //
-// Measured (captured, weights from memory): 8 rows of bf16, 4096 -> 4096: 7.3 us (1.2 TB/s of codes and
-// scales); 24 rows of f16, 11009 -> 4096 with zero points: 17 us, 1.4 TB/s. A launch, the first
-// loads' way and the sums are 3 us of it; then the chunks' latencies: an SM holds 8 to 16 warps at
-// 141 registers, and 30% of its issue slots are used.
+// Measured (captured, weights from memory): 8 rows of bf16, 4096 -> 4096: 8.3 us (1.1 TB/s of codes and
+// scales); 24 rows of f16, 11009 -> 4096 with zero points: 21.2 us with the copy of its rows, 1.1 TB/s; 8 rows of
+// f32, 4096 -> 8192: 17.5 us, 1.0 TB/s (every block reads and splits the activations for itself, and three
+// products take a step). A launch, the first loads' way and the sums are 3 us of it; then the chunks'
+// latencies: up to 24 rows an SM holds two blocks, 16 warps at up to 128 registers, beyond that one, and about
+// 35% of its issue slots are used.
 #pragma once
 
 #include "ptx.cuh"

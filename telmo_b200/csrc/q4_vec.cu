@@ -24,9 +24,10 @@
 // 32 outputs; its eight warps share the chunks, each with a ring of chunks of codes, scales and
 // zero points in shared memory (cp.async), and add up in order.
 //
-// Measured: one bf16 row, 4096 -> 32768, 69 MB of codes and scales from memory, 15.2 us captured: 4.5 TB/s
-// (70% of a copy's rate); the digits of the first block and the rings' first chunks take 3 us before the
-// stream runs.
+// Measured: one bf16 row, 4096 -> 32768, 69 MB of codes and scales from memory, 15.9 us captured: 4.3 TB/s
+// (67% of a copy's rate); the digits of the first block and the rings' first chunks take 3 us before the
+// stream runs. An SM holds two blocks, 16 warps: their digits and rings take 102,400 bytes each (75 registers
+// would let three in).
 #include "q4_device.cuh"
 #include "ptx.cuh"
 #include "q4_async.cuh"
@@ -374,8 +375,8 @@ auto by_shape(int m, int group, bool zeros, F f) {
 
 }  // namespace
 
-// One or two rows whose digits and rings fit into shared memory. 4096 -> 8192, bf16: one row 8.2 us, 10.0 on the
-// row kernels; two rows 10.1 against 10.3. 1024 -> 4096, f32: 2.9 against 4.2, two rows 3.6 against 4.4.
+// One or two rows whose digits and rings fit into shared memory. 4096 -> 8192, bf16: one row 8.5 us, 10.7 on the
+// row kernels; two rows 10.4 against 11.1. 1024 -> 4096, f32: 3.0 against 4.1, two rows 3.5 against 4.2.
 bool q4_vec_fits(const Q4Args& g) {
     if (g.m > 2) return false;
     return by_shape(g.m, g.w->group, g.w->zeros != nullptr, [&](auto m, auto groups, auto zeros) {
